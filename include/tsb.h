@@ -230,6 +230,90 @@ int tsb_tree_attn_noalloc(const void *q,
                           int B, int T, int Hq, int Hkv, int D, int n_kv, int tail, int kv_capacity,
                           float scale, void *out, float *lse, tsb_stream_t stream);
 
+/* One cache as tsb_tree_attn_shared reads it: planes as for tsb_tree_attn
+ * (scales and biases NULL where the format has none), `capacity` rows per
+ * (request, head), of which the first `rows` hold keys. */
+typedef struct {
+  const void *k, *k_scales, *k_biases, *v, *v_scales, *v_biases;
+  int capacity, rows;
+} tsb_kv_t;
+
+/* Tree attention for a batch that shares a long prefix:
+ * out[b, h, t, :] = softmax over the rows of `prefix` (one cache [1, Hkv, cap,
+ * D], every row visible to every node) and request b's own rows (`own`, [B,
+ * Hkv, cap, D]), with G = Hq / Hkv query heads per KV head. The prefix is read
+ * once per 128 packed query rows of the whole batch, not once per request. The
+ * reference has no counterpart (its batched decoding keeps a whole cache per
+ * request, mlx-tree-spec src/mlx_tree_spec/tree_verify.py:340-367); the result
+ * is that of tsb_tree_attn on each request's concatenated cache.
+ *
+ *   q        bf16, element strides q_stride_b / _h / _t (multiples of 8), D
+ *            contiguous
+ *   lengths  int32 [B] on the device: request b's own rows, the tree's own rows
+ *            last (clamped to [0, own->rows]); NULL: own->rows for every request
+ *   parents / bits, tail   as for tsb_tree_attn, over the last `tail` own rows.
+ *            A request with fewer own rows than `tail` has the last ones of them.
+ *   out      bf16 [B, Hq, T, D]; lse float [B, Hq, T] or NULL: as tsb_tree_attn.
+ *            A node that sees nothing gets zeros and -inf.
+ * Either cache may have no rows (its planes are then not read). Planes 16-byte
+ * aligned, MLX scales and biases 8, row scales 4. Requirements: D == 256,
+ * Hq % Hkv == 0, 1 <= T <= 64, tail <= 64, scale > 0, B*Hq*T <= 2^24. No host
+ * read of the lengths: the call can be captured in a graph and replayed with
+ * others. `own->rows` bounds the lengths and sizes the launch. Workspace:
+ * tsb_tree_attn_shared_workspace_bytes(), 16-byte aligned, for this call alone
+ * until it completes. */
+size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows);
+int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride_h, long long q_stride_t,
+                         int kv_format, const tsb_kv_t *prefix, const tsb_kv_t *own, const int32_t *lengths,
+                         const int32_t *parents, const uint64_t *bits, int B, int T, int Hq, int Hkv, int D, int tail,
+                         float scale, void *out, float *lse, void *ws, size_t ws_bytes, tsb_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * After the logits: sampling, the walk down the draft tree, and the commit of
+ * the accepted rows, with no host read in between.
+ * ---------------------------------------------------------------------- */
+
+/* One token per row of logits [rows, vocab] (row_stride elements apart;
+ * logits_dtype TSB_MASK_BF16, TSB_MASK_F16 or TSB_MASK_F32). Order a row's tokens by
+ * (logit descending, index ascending), w_i = exp((x_i - max) / temperature),
+ * and keep of that order the first top_k; of those the shortest prefix whose
+ * mass reaches top_p times theirs; of those the tokens with w >= min_p (always
+ * the first). The token is the first kept one whose cumulative weight exceeds
+ * u[row] times the kept weight, u in [0, 1). logprob (nullable): log of the
+ * token's share of the kept weight. Each parameter is a device array [rows] or,
+ * where that is NULL, the value beside it. temperature <= 0 or NaN: the first
+ * token (greedy). Off: top_k <= 0 or >= vocab, top_p >= 1 or NaN, min_p <= 0 or
+ * NaN. u is clamped to [0, 1]. NaN and -inf logits are never chosen, +inf ones
+ * share all the weight; a row with nothing to choose gives token -1 and
+ * logprob -inf. Weights are summed as integers of 2^-42 of the largest, so the
+ * result does not depend on the order of the sums. vocab <= 2^20. */
+int tsb_sample(const void *logits, int logits_dtype, int rows, int vocab, long long row_stride, const float *u,
+               const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
+               const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *token,
+               float *logprob, tsb_stream_t stream);
+
+/* The accepted path of each request's tree: cur = 0; while a node c > cur has
+ * parents[c] == cur and tokens[c] == samples[cur] >= 0, cur = the lowest such
+ * c. tokens (drafted), parents, samples (the token sampled after each node)
+ * int32 [B, T]. path int32 [B, T]: the nodes, then -1; n_keep int32 [B]: their
+ * number (at least 1, the root); next int32 [B]: the sample after the last.
+ * Padding nodes carry token -1. T <= 64. */
+int tsb_tree_accept(const int32_t *tokens, const int32_t *parents, const int32_t *samples, int B, int T,
+                    int32_t *path, int32_t *n_keep, int32_t *next, tsb_stream_t stream);
+
+/* tsb_kv_commit_layers for paths and lengths on the device, any B: request b's
+ * rows lengths[b] - T + path[b*T + i] move to lengths[b] - T + i for i <
+ * n_keep[b], in every layer's cache (HOST arrays of device pointers). A path
+ * increases (parents precede their children); it ends at its first entry that
+ * is no node of [0, T) or does not increase. new_lengths int32 [B] (nullable;
+ * not lengths itself): lengths[b] - T + kept rows. A request with lengths[b]
+ * outside [T, kv_capacity] is left as it is, with its length. D == 256,
+ * T <= 64, layers <= 48. */
+int tsb_kv_commit_paths(int kv_format, int layers, void *const *k, void *const *k_scales, void *const *k_biases,
+                        void *const *v, void *const *v_scales, void *const *v_biases, int B, int Hkv, int D,
+                        int kv_capacity, int T, const int32_t *lengths, const int32_t *path, const int32_t *n_keep,
+                        int32_t *new_lengths, tsb_stream_t stream);
+
 /* ------------------------------------------------------------------------
  * Verify-step decoder layer: the kernels around the qmm and tree attention
  * (mlx-tree-spec src/mlx_tree_spec/tree_verify.py:311-367 batch_attention /

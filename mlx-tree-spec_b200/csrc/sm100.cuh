@@ -88,6 +88,18 @@ TSB_HD bool mbar_wait(uint64_t *bar, uint32_t parity) {
   }
 }
 
+// Wait, before the CTA may exit, for a copy already in flight: bounded like
+// mbar_wait, but never cut short by an earlier failure elsewhere.
+TSB_HD void mbar_drain(uint64_t *bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer_ns() - t0 > kWaitLimitNs) {
+      record_status(TSB_ETIMEOUT);
+      return;
+    }
+  }
+}
+
 // All 32 lanes wait (each acquires the barrier); the result is warp-uniform so
 // that .sync.aligned instructions after it see a converged warp.
 TSB_HD bool warp_wait(uint64_t *bar, uint32_t parity) {

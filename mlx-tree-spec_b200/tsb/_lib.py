@@ -40,6 +40,13 @@ class GatherT(ctypes.Structure):
                 ("sig", ctypes.c_void_p * TSB_MAX_GATHER_RANKS)]
 
 
+class KVT(ctypes.Structure):
+    """tsb_kv_t: one cache as tsb_tree_attn_shared reads it."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "k_scales", "k_biases", "v", "v_scales", "v_biases")] + [
+        ("capacity", ctypes.c_int), ("rows", ctypes.c_int)]
+
+
 # Every symbol include/tsb.h declares, with (restype, argtypes).
 _P, _I, _Z, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_longlong
 SIGNATURES = {
@@ -64,6 +71,12 @@ SIGNATURES = {
                                    _P, _P, _P]),
     "tsb_kv_commit": (_I, [_I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P]),
     "tsb_kv_commit_layers": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P]),
+    "tsb_tree_attn_shared_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
+    "tsb_tree_attn_shared": (_I, [_P, _LL, _LL, _LL, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _Z,
+                                  _P]),
+    "tsb_sample": (_I, [_P, _I, _I, _I, _LL, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
+    "tsb_tree_accept": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P]),
+    "tsb_kv_commit_paths": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "tsb_gdn_prep": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "tsb_tree_gated_delta": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P]),
     "tsb_gdn_commit": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P]),

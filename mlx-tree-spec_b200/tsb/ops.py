@@ -14,6 +14,8 @@ same argument names and meaning:
   tree_flash(queries, cache, scale, bits, tail=None, stats=False)
       = tree_flash.tree_flash (tree_flash.py:151-196); also takes `parents=`
         so the mask is built inside the kernel.
+  tree_flash_shared(queries, prefix, cache, scale, bits, tail=None, stats=False, parents=None, lengths=None)
+      = tree_flash for a batch whose requests share a prefix cache
   mask_bits(mask, tail)
       = the inverse of Tree.mask (tree_verify.py:131-139): an SDPA mask -> bits
   sdpa(queries, keys, values, cache, scale, mask, fallback=None)
@@ -279,6 +281,113 @@ def tree_flash(queries, cache, scale: float, bits=None, tail: int | None = None,
                            _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, n_kv, tail_v, cap, float(scale),
                            _ptr(out), _ptr(lse), _ptr(ws), ws.numel(), _stream(q))
     if check(st, "tsb_tree_attn") == TSB_EUNSUPPORTED:
+        return None
+    if stats:
+        return out, lse[..., None], torch.ones_like(lse)[..., None]
+    return out
+
+
+_KV_TYPES = {TSB_KV_BF16: torch.bfloat16, TSB_KV_REF_Q8_ROW: torch.int8, TSB_KV_MLX_Q8_G64: None}
+
+
+def _kv_struct(cache, fmt: int, bsz: int, hkv: int, d: int, device):
+    """tsb_kv_t of a cache of `bsz` requests, its planes checked."""
+    planes = _kv_planes(cache)
+    if planes[0] != fmt:
+        raise ValueError("tree_flash_shared: the prefix and the requests' caches must share a format")
+    keys = planes[1]
+    cap, rows = keys.shape[2], int(cache.offset)
+    if not 0 <= rows <= cap:
+        raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
+    lead = (bsz, hkv, cap)
+    if fmt == TSB_KV_MLX_Q8_G64:
+        shapes = ((*lead, d // 4), (*lead, d // 64), (*lead, d // 64)) * 2
+        types = (None, torch.bfloat16, torch.bfloat16) * 2
+    else:
+        shapes = ((*lead, d), lead, None) * 2
+        types = (_KV_TYPES[fmt], torch.float32, None) * 2
+    st = _lib.KVT(capacity=cap, rows=rows)
+    for name, t, shape, dt in zip(("k", "k_scales", "k_biases", "v", "v_scales", "v_biases"), planes[1:], shapes, types):
+        if t is None:
+            continue
+        if t.shape != shape or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"tree_flash_shared: {name} must be a contiguous tensor of shape {tuple(shape)} on "
+                             f"{device}, got {tuple(t.shape)} on {t.device}")
+        if (t.dtype != dt) if dt is not None else t.dtype not in (torch.int32, torch.uint32):
+            raise ValueError(f"tree_flash_shared: {name} has type {t.dtype}")
+        setattr(st, name, t.data_ptr())
+    return st
+
+
+def _tree_rows(t, bsz: int, n: int, dtype, what: str, device):
+    """(n,) or (bsz, n) -> a contiguous (bsz, n) tensor of dtype on device."""
+    t = t.to(device=device, dtype=dtype)
+    if t.shape == (n,):
+        t = t.expand(bsz, n)
+    if t.shape != (bsz, n):
+        raise ValueError(f"{what} must have shape ({n},) or ({bsz}, {n}), got {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int | None = None, stats: bool = False,
+                      parents=None, lengths=None, out=None):
+    """tree_flash for a batch whose requests share a prefix: `queries` (B, Hq,
+    n, D) attend to every row of `prefix`, one cache object of batch 1, and to
+    their own request's rows of `cache` (batch B). The prefix is read once for
+    the whole batch. The result is tree_flash's over each request's
+    concatenated rows.
+
+    Both caches have the same format; their `offset` is the number of valid
+    rows (0: the cache is not read). lengths (optional): int32 (B,) on the
+    device, each request's own rows, its tree's rows last; cache.offset then
+    only bounds them (longer ones count as cache.offset). The lengths are read
+    by the kernel, so a captured call can be replayed with other values in the
+    same tensor. bits / tail / parents / stats / out as for tree_flash, the
+    tail being the last rows of each request's own; a node that sees nothing
+    gets zeros and a log-sum-exp of -inf. queries may have any strides with D
+    contiguous and 16-byte aligned rows (others are copied first)."""
+    fmt, pk = _kv_planes(prefix)[:2]
+    _require_cuda(queries, pk, cache.keys)
+    if queries.dtype != torch.bfloat16 or (parents is None and bits is None):
+        return None
+    bsz, hq, n, d = queries.shape
+    dev = queries.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return tree_flash_shared(queries, prefix, cache, scale, bits, tail, stats, parents, lengths, out)
+    hkv = pk.shape[1]
+    if d != 256 or hq % hkv or n > 64 or bsz < 1 or n < 1:
+        return None
+    pre = _kv_struct(prefix, fmt, 1, hkv, d, dev)
+    own = _kv_struct(cache, fmt, bsz, hkv, d, dev)
+    p = bits_t = None
+    if parents is not None:
+        p = _tree_rows(parents, bsz, n, torch.int32, "tree_flash_shared: parents", dev)
+        tail_v = n
+    else:
+        if not isinstance(bits, torch.Tensor):
+            bits = torch.tensor([int(b) if int(b) < 2**63 else int(b) - 2**64 for b in bits], dtype=torch.int64)
+        bits_t = _tree_rows(bits, bsz, n, torch.int64, "tree_flash_shared: bits", dev)
+        tail_v = n if tail is None else int(tail)
+    if lengths is not None:
+        if lengths.dtype != torch.int32 or lengths.shape != (bsz,) or not lengths.is_contiguous() or lengths.device != dev:
+            raise ValueError(f"tree_flash_shared: lengths must be a contiguous int32 tensor ({bsz},) on {dev}")
+    q = queries
+    if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(2) % 8 or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = torch.empty((bsz, hq, n, d), dtype=torch.bfloat16, device=dev)
+    elif out.shape != queries.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError("tree_flash_shared: out must be a contiguous bf16 tensor of the queries' shape")
+    lse = torch.empty((bsz, hq, n), dtype=torch.float32, device=dev) if stats else None
+    lib = _lib.load()
+    # a workspace of this call's own: calls on other streams and captured graphs share nothing
+    ws = torch.empty(lib.tsb_tree_attn_shared_workspace_bytes(bsz, n, hq, hkv, d, pre.rows, own.rows),
+                     dtype=torch.uint8, device=dev)
+    st = lib.tsb_tree_attn_shared(_ptr(q), q.stride(0), q.stride(1), q.stride(2), fmt, ctypes.byref(pre),
+                                  ctypes.byref(own), _ptr(lengths), _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, tail_v,
+                                  float(scale), _ptr(out), _ptr(lse), _ptr(ws), ws.numel(), _stream(q))
+    if check(st, "tsb_tree_attn_shared") == TSB_EUNSUPPORTED:
         return None
     if stats:
         return out, lse[..., None], torch.ones_like(lse)[..., None]

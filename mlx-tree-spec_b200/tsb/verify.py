@@ -1,0 +1,216 @@
+"""What follows a verify pass, on the device from the logits to the caches.
+
+  sample(logits, u, temperature, top_k, top_p, min_p)   a token for every tree node
+  tree_accept(tokens, parents, samples)                 the accepted path of each request's tree
+  PathCommit(caches)(lengths, path, n_keep)             those rows kept in every layer's cache
+
+Verifying by sampling: a token is drawn from the model's own distribution at
+every node of the drafted tree, and the walk from the root follows the drafted
+child that equals the token drawn at its parent, so the emitted tokens are
+distributed as if they had been decoded one by one. The reference does the
+walk and the commit's indices on the host (mlx-tree-spec
+src/mlx_tree_spec/tree_verify.py:499-516); here no step reads the device, so
+the whole of a verify step can be one captured graph.
+
+As in tsb.ops, an unsupported shape or type returns None, a contract violation
+raises, and work is enqueued on torch's current stream of the tensors' device.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from ._lib import TSB_EUNSUPPORTED, TSB_KV_MLX_Q8_G64, TSB_MASK_BF16, TSB_MASK_F16, TSB_MASK_F32, check
+from .ops import _kv_planes, _ptr, _require_cuda, _stream
+
+_LOGIT_TYPES = {torch.bfloat16: TSB_MASK_BF16, torch.float16: TSB_MASK_F16, torch.float32: TSB_MASK_F32}
+_MAX_LAYERS_PER_LAUNCH = 48
+_MAX_VOCAB = 1 << 20
+
+
+def _per_row(v, rows: int, dtype, name: str, device):
+    """A sampling parameter: (device tensor or None, scalar)."""
+    if not isinstance(v, torch.Tensor):
+        return None, v
+    if v.device != device:
+        raise ValueError(f"sample: {name} must be on {device}")
+    if v.numel() != rows:
+        raise ValueError(f"sample: {name} must have one value per row ({rows}), got {tuple(v.shape)}")
+    if v.dtype != dtype:
+        v = v.to(dtype)
+    return (v if v.is_contiguous() else v.contiguous()), 0
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: bool = False):
+    """One token per row of logits (..., V), bf16, fp16 or float32, with the
+    random numbers u (...,) float32 in [0, 1).
+
+    Order a row's tokens by logit, equal ones by index; w_i = exp((x_i - max) /
+    temperature). Of that order the first top_k are kept, of those the shortest
+    prefix whose weight reaches top_p times theirs, of those the tokens with
+    w_i >= min_p (always the first). The token is the first kept one whose
+    cumulative weight exceeds u times the kept weight: u near 0 gives the likeliest.
+    temperature 0 is greedy. top_k <= 0, top_p >= 1 and min_p <= 0 are off.
+    Each parameter is a number or a tensor of one value per row.
+
+    Returns int32 tokens (...,), or (tokens, logprobs) with float32 log
+    probabilities under the filtered distribution. Logits of -inf or NaN are
+    never chosen; a row of nothing else gives -1 and -inf. None where the type
+    or V (> 2^20) is not taken."""
+    _require_cuda(logits, u)
+    dt = _LOGIT_TYPES.get(logits.dtype)
+    if dt is None or logits.dim() < 1:
+        return None
+    dev = logits.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return sample(logits, u, temperature, top_k, top_p, min_p, logprobs)
+    vocab = logits.shape[-1]
+    lead = logits.shape[:-1]
+    if vocab < 1:
+        raise ValueError("sample: logits have no tokens")
+    if vocab > _MAX_VOCAB:
+        return None
+    if u.shape != lead or u.dtype != torch.float32 or u.device != dev:
+        raise ValueError(f"sample: u must be float32 of shape {tuple(lead)} on {dev}, got {u.dtype} {tuple(u.shape)}")
+    x = logits
+    if x.dim() != 2:
+        x = x.reshape(-1, vocab)
+    rows = x.shape[0]
+    if x.stride(1) != 1 and vocab > 1 or rows > 1 and x.stride(0) < vocab:
+        x = x.contiguous()
+    t_t, t_s = _per_row(temperature, rows, torch.float32, "temperature", dev)
+    k_t, k_s = _per_row(top_k, rows, torch.int32, "top_k", dev)
+    p_t, p_s = _per_row(top_p, rows, torch.float32, "top_p", dev)
+    m_t, m_s = _per_row(min_p, rows, torch.float32, "min_p", dev)
+    token = torch.empty(lead, dtype=torch.int32, device=dev)
+    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if logprobs else None
+    if rows:
+        if not u.is_contiguous():
+            u = u.contiguous()
+        st = _lib.load().tsb_sample(_ptr(x), dt, rows, vocab, x.stride(0) if rows > 1 else vocab, _ptr(u), _ptr(t_t), t_s,
+                                    _ptr(k_t), min(max(int(k_s), 0), vocab), _ptr(p_t), p_s, _ptr(m_t), m_s,
+                                    _ptr(token), _ptr(logprob), _stream(x))
+        if check(st, "tsb_sample") == TSB_EUNSUPPORTED:
+            return None
+    return (token, logprob) if logprobs else token
+
+
+def _i32(t, shape, name: str, device):
+    if t.device != device or t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def tree_accept(tokens, parents, samples):
+    """The accepted path of each request's tree: from node 0, on to the lowest
+    node c below the current one (parents[c] == cur, c > cur) whose drafted token
+    is the one sampled at cur, until there is none.
+
+    tokens, parents, samples (B, T) integers: the drafted tokens (-1 for a
+    padding node), the parents as for tree_flash, and the token sampled after
+    each node (negative: nothing follows). Returns int32 path (B, T), the
+    accepted nodes and then -1; n_keep (B,), their number; next_token (B,), the
+    token sampled after the last of them. None for T > 64."""
+    _require_cuda(tokens, parents, samples)
+    if tokens.dim() != 2:
+        raise ValueError("tree_accept: tokens must be (B, T)")
+    dev = tokens.device
+    if dev.index != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return tree_accept(tokens, parents, samples)
+    b, t = shape = tokens.shape
+    if t > 64:
+        return None
+    if t < 1:
+        raise ValueError("tree_accept: a tree has at least its root")
+    tok = _i32(tokens, shape, "tree_accept: tokens", dev)
+    par = _i32(parents, shape, "tree_accept: parents", dev)
+    smp = _i32(samples, shape, "tree_accept: samples", dev)
+    path = torch.empty((b, t), dtype=torch.int32, device=dev)
+    n_keep = torch.empty(b, dtype=torch.int32, device=dev)
+    nxt = torch.empty(b, dtype=torch.int32, device=dev)
+    if b:
+        check(_lib.load().tsb_tree_accept(_ptr(tok), _ptr(par), _ptr(smp), b, t, _ptr(path), _ptr(n_keep), _ptr(nxt),
+                                          _stream(tok)), "tsb_tree_accept")
+    return path, n_keep, nxt
+
+
+class PathCommit:
+    """The tree commit of a list of caches (every layer's; tree_verify.py:499-516)
+    by lengths and paths on the device.
+
+    plan = PathCommit(caches); new_lengths = plan(lengths, path, n_keep): for
+    request b the last T rows of its lengths[b] are its tree's; rows
+    lengths[b] - T + path[b, i], i < n_keep[b], move to lengths[b] - T + i in
+    every cache, and the new length is lengths[b] - T + n_keep[b]. path (B, T)
+    and n_keep (B,) are tree_accept's; a path must increase and ends where it
+    does not. A request whose length is not in [T, capacity] is left as it is.
+
+    The plan holds the caches' tensors (not their `offset`): make it once per
+    set of caches, and again if a cache gets new tensors. The caches of one
+    request batch B may differ in format, heads and capacity."""
+
+    def __init__(self, caches):
+        self._caches = [(c, _kv_planes(c)) for c in caches]
+        if not self._caches:
+            raise ValueError("PathCommit: no caches")
+        groups: dict = {}
+        k0 = self._caches[0][1][1]
+        planes_seen = [t.data_ptr() for _, planes in self._caches for t in planes[1:] if t is not None]
+        if len(set(planes_seen)) < len(planes_seen):
+            raise ValueError("PathCommit: a tensor appears twice: its rows would move twice")
+        for _, planes in self._caches:
+            k, v = planes[1], planes[4]
+            _require_cuda(*planes[1:])
+            if any(t is not None and not t.is_contiguous() for t in planes[1:]):
+                raise ValueError("PathCommit: cache tensors must be contiguous")
+            width = k.shape[3] * (4 if planes[0] == TSB_KV_MLX_Q8_G64 else 1)
+            if width != 256 or k.shape != v.shape:
+                raise ValueError(f"PathCommit: unsupported cache of shape {tuple(k.shape)}")
+            for t in planes[2:]:
+                if t is not None and (t.device != k0.device or t.shape[:3] != k.shape[:3]):
+                    raise ValueError("PathCommit: a cache's planes must agree in shape and device")
+            if k.device != k0.device or k.shape[0] != k0.shape[0]:
+                raise ValueError("PathCommit: every cache must hold the same requests on the same device")
+            groups.setdefault((planes[0], k.shape[1], k.shape[2]), []).append(planes)
+        self._device, self._batch = k0.device, k0.shape[0]
+        self._launches = []
+        vp = ctypes.c_void_p
+        for (fmt, hkv, cap), members in groups.items():
+            for i in range(0, len(members), _MAX_LAYERS_PER_LAUNCH):
+                part = members[i:i + _MAX_LAYERS_PER_LAUNCH]
+                arrays = [(vp * len(part))(*[_ptr(p[j]) for p in part]) if part[0][j] is not None else None
+                          for j in range(1, 7)]
+                self._launches.append((fmt, len(part), *arrays, self._batch, hkv, 256, cap))
+
+    def __call__(self, lengths, path, n_keep):
+        dev, b = self._device, self._batch
+        if dev.index != torch.cuda.current_device():
+            with torch.cuda.device(dev):
+                return self(lengths, path, n_keep)
+        if path.dim() != 2:
+            raise ValueError("PathCommit: path must be (B, T)")
+        t = path.shape[1]
+        if not 1 <= t <= 64:
+            raise ValueError(f"PathCommit: trees of 1 to 64 nodes, got {t}")
+        p = _i32(path, (b, t), "PathCommit: path", dev)
+        n = _i32(n_keep, (b,), "PathCommit: n_keep", dev)
+        cur = _i32(lengths, (b,), "PathCommit: lengths", dev)
+        new = torch.empty(b, dtype=torch.int32, device=dev)
+        lib = _lib.load()
+        for i, args in enumerate(self._launches):
+            st = lib.tsb_kv_commit_paths(*args, t, _ptr(cur), _ptr(p), _ptr(n), _ptr(new) if i == 0 else None, _stream(p))
+            if check(st, "tsb_kv_commit_paths") == TSB_EUNSUPPORTED:
+                raise ValueError("PathCommit: unsupported caches")
+        return new
+
+
+def commit_paths(caches, lengths, path, n_keep):
+    """PathCommit(caches)(lengths, path, n_keep), for a single commit."""
+    return PathCommit(caches)(lengths, path, n_keep)
