@@ -288,8 +288,8 @@ int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride
  * logprob -inf. Weights are summed as integers of 2^-42 of the largest, so the
  * result does not depend on the order of the sums. vocab <= 2^20. */
 int tsb_sample(const void *logits, int logits_dtype, int rows, int vocab, long long row_stride, const float *u,
-               const float *temperature, float temperature_all, const int32_t *top_k, int top_k_all,
-               const float *top_p, float top_p_all, const float *min_p, float min_p_all, int32_t *token,
+               const float *temperature, double temperature_all, const int32_t *top_k, int top_k_all,
+               const float *top_p, double top_p_all, const float *min_p, double min_p_all, int32_t *token,
                float *logprob, tsb_stream_t stream);
 
 /* The accepted path of each request's tree: cur = 0; while a node c > cur has

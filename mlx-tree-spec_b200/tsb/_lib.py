@@ -49,6 +49,7 @@ class KVT(ctypes.Structure):
 
 # Every symbol include/tsb.h declares, with (restype, argtypes).
 _P, _I, _Z, _F, _LL = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_float, ctypes.c_longlong
+_D = ctypes.c_double
 SIGNATURES = {
     "tsb_strerror": (ctypes.c_char_p, [_I]),
     "tsb_version": (_I, []),
@@ -74,7 +75,7 @@ SIGNATURES = {
     "tsb_tree_attn_shared_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I]),
     "tsb_tree_attn_shared": (_I, [_P, _LL, _LL, _LL, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _Z,
                                   _P]),
-    "tsb_sample": (_I, [_P, _I, _I, _I, _LL, _P, _P, _F, _P, _I, _P, _F, _P, _F, _P, _P, _P]),
+    "tsb_sample": (_I, [_P, _I, _I, _I, _LL, _P, _P, _D, _P, _I, _P, _D, _P, _D, _P, _P, _P]),
     "tsb_tree_accept": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P]),
     "tsb_kv_commit_paths": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),
     "tsb_gdn_prep": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),

@@ -131,6 +131,35 @@ def test_masked_infinite_and_nan_logits(dtype):
         assert got[0][0] == -1 and got[0][1] == -1 and got[0][2] == 1234 and got[0][3] == 5 and got[0][5] == 0
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_tokens_of_nearly_one_logit(dtype):
+    """More tokens in a narrow band than can be listed: equal ones, and neighbours that differ in the last bits."""
+    import tsb
+
+    vocab = 60013
+    g = torch.Generator(device="cuda").manual_seed(11)
+    x = torch.randn(4, vocab, device="cuda", generator=g)
+    x[0, ::2] = 4.0                                                # one tie of 30000 above the rest
+    x[1] = 1.0 + 1e-3 * torch.rand(vocab, device="cuda", generator=g)
+    x[2] = torch.randint(0, 3, (vocab,), device="cuda", generator=g).float()
+    x[3, 1000:] = -60.0                                            # tokens with hardly any weight
+    x = x.to(dtype)
+    for value in (0.0, 0.3, 0.77, 0.999999):
+        u = torch.full((4,), value, device="cuda")
+        for params in ({}, {"top_k": 5000}, {"top_k": 50000, "top_p": 0.6}, {"top_p": 0.9, "min_p": 0.02}, {"temperature": 0.3}):
+            _check(x, u, tsb.sample(x, u, logprobs=True, **params), **params)
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1 << 20), (torch.float32, (1 << 20) - 3), (torch.bfloat16, 700001)])
+def test_the_largest_vocabularies(dtype, vocab):
+    import tsb
+
+    x, u = _logits(2, vocab, dtype, seed=12)
+    for params in ({}, {"temperature": 0.7, "top_k": 50, "top_p": 0.95}, {"top_k": 5000, "top_p": 0.9}):
+        _check(x, u, tsb.sample(x, u, logprobs=True, **params), **params)
+    assert tsb.sample(torch.zeros(1, (1 << 20) + 1, dtype=dtype, device="cuda"), u[:1]) is None
+
+
 def test_random_numbers_at_and_past_the_ends():
     import tsb
 
