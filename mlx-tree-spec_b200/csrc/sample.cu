@@ -2,28 +2,31 @@
 // min-p from given random numbers.
 //
 // Order the tokens by (logit descending, index ascending) and give token i the
-// weight w_i = exp((x_i - max) / temperature). Every filter keeps a prefix of
-// that order: top-k the first k, top-p the shortest prefix whose mass reaches
-// p times the mass of those k, min-p the tokens of weight >= min_p. The sample
-// is the first token whose cumulative mass exceeds u times the mass S kept by
-// all of them. So a row is never sorted: each step asks where the running count
-// or mass along the order crosses a bound.
+// weight w_i = 2^-t_i, t = (max - x) * log2(e) / temperature. Every filter keeps a
+// prefix of that order: top-k the first k, top-p the shortest prefix whose mass
+// reaches p times the mass of those k, min-p the tokens of weight >= min_p. The
+// sample is the first token whose cumulative mass exceeds u times the mass kept
+// by all of them. So a row is never sorted: each step asks where the running
+// count or mass along the order crosses a bound.
 //
 // A cluster of CTAs holds a row's logits in shared memory (one read of HBM).
 //   1. The maximum, exchanged through distributed shared memory.
-//   2. A histogram over t = (max - x) * log2(e) / temperature in steps of 1/32,
-//      fine enough that a bin holds few tokens: counts alone where top-k needs no
-//      more, else counts and masses.
-//   3. CTA 0 adds the histograms up, finds the bins in which the bounds fall,
-//      and the tokens of those bins (or of all bins up to the last one wanted,
-//      when they are few) are gathered in its shared memory, sorted and walked.
-// A bin with more tokens than the list holds (thousands of logits equal or
-// nearly so) is resolved by a radix descent over the logits' bits instead.
+//   2. A histogram over t in steps of 1/32, so fine that a bin holds few tokens:
+//      of counts with top-k, else of masses. The CTAs add theirs into CTA 0's.
+//   3. CTA 0 finds the bins in which the bounds fall; the tokens of those bins
+//      (all bins up to the last one wanted, or the sample's own bin alone) are
+//      gathered in its shared memory, sorted and walked.
+// Where the kept tokens are too many to list, the bounds are resolved one after
+// the other, each inside its bin: by a list of that bin, or, for a bin of
+// thousands of nearly equal logits, by a radix descent over their bits.
 //
 // Masses are integers, units of 2^-42 of the largest weight: sums do not depend
 // on the order of the additions, results repeat bit for bit, and a row's mass
-// stays below 2^62. A weight is a float32 exponential of a 64-bit argument: its
-// roundings are independent from token to token and do not add up.
+// stays below 2^62. A token's mass is m * 2^(19 - t's octave), m of 24 bits from a
+// float32 power series of the exactly reduced t; the roundings of m are independent
+// from token to token and do not add up. A bin lies in one octave, so its sum of
+// m needs two 32-bit shared-memory atomics per token (12 bits each, 2^20 tokens
+// do not overflow them); a 64-bit one would be a compare-and-swap loop.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -39,17 +42,18 @@ typedef unsigned long long u64;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kStep = 32;                // bins per halving of the weight
-constexpr int kBins = 1408;              // 44 halvings; the last bin takes the rest, which have no mass
+constexpr int kStep = 32;              // bins per octave of the weight
+constexpr int kBins = 43 * kStep;      // a token of no bin has a mass of zero
 constexpr int kBinsPerThread = (kBins + kThreads - 1) / kThreads;
-constexpr int kList = 2048;              // tokens CTA 0 can sort
-constexpr int kCountOnlyK = 1024;        // top-k up to here needs no masses in the histogram
-constexpr u64 kOne = 1ull << 42;         // the mass of the largest weight
+constexpr int kList = 2048;            // tokens CTA 0 can sort
+constexpr int kListPerThread = kList / kThreads;
+constexpr u64 kOne = 1ull << 42;       // the mass of the largest weight
+constexpr int kTopM = 1 << 23;         // its m
 constexpr int kMaxVocab = 1 << 20;
-constexpr int kMaxStage = 160 * 1024;    // bytes of logits a CTA holds in shared memory
-
+constexpr int kMaxStage = 160 * 1024;  // bytes of logits a CTA holds in shared memory
 constexpr size_t kSliceBytes = 48 * 1024;  // of logits in a CTA, while there are CTAs to split them over
-constexpr int kSliceMin = 4096;          // logits of a slice that is not split further
+constexpr int kSliceMin = 4096;            // logits of a slice that is not split further
+constexpr double kMinTemperature = 8.673617379884035e-19;  // 2^-60
 
 struct SampleArgs {
   const void *logits;
@@ -68,35 +72,53 @@ TSB_HD float to_float(float x) { return x; }
 TSB_HD float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 TSB_HD float to_float(__half x) { return __half2float(x); }
 
-// Order-preserving bits: a larger logit has a larger key. -0 counts as +0; NaN
-// is below everything.
+// Largest of 16 bytes of logits and m; NaN is skipped.
+TSB_HD float max_of(const uint4 &v, float m, float) {
+  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(v.x), __uint_as_float(v.y))),
+               fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+}
+TSB_HD float max_of(const uint4 &v, float m, __nv_bfloat16) {
+  const __nv_bfloat162 a = __hmax2(__hmax2(u32_as_bf2(v.x), u32_as_bf2(v.y)), __hmax2(u32_as_bf2(v.z), u32_as_bf2(v.w)));
+  return fmaxf(m, fmaxf(__low2float(a), __high2float(a)));
+}
+TSB_HD float max_of(const uint4 &v, float m, __half) {
+  const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+  const __half2 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(m, fmaxf(__low2float(a), __high2float(a)));
+}
+
+// Order-preserving bits: a larger logit has a larger key, -0 that of +0.
 TSB_HD uint32_t logit_key(float x) {
-  if (x != x) return 0u;
   const uint32_t b = __float_as_uint(x + 0.f);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 TSB_HD float key_logit(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
 
+// A row whose largest logit is finite.
 struct RowScale {
   float top;        // the largest logit
-  float bin_scale;  // kStep * log2(e) / temperature
-  double c;         // log2(e) / temperature
+  float bin_scale;  // kStep * c
+  float c, c_low;   // log2(e) / temperature
 };
 
-// Bin of a live logit: never decreases as the logit falls.
-TSB_HD int logit_bin(float x, const RowScale &r) {
-  if (x == r.top) return 0;  // +inf - +inf among them
-  return (int)fminf((r.top - x) * r.bin_scale, (float)(kBins - 1));
+// Bin of a logit, never decreasing as the logit falls: round(kStep * t). At or past
+// kBins for a token without mass, -inf and NaN among them (the float's bits are
+// compared as a number).
+TSB_HD uint32_t logit_bin(float x, const RowScale &r) {
+  return __float_as_uint(fmaf(r.top - x, r.bin_scale, 8388608.f)) - 0x4B000000u;
 }
 
-// Mass of a live logit: 2^42 * 2^-t, t = n + 1/2 - g, 2^g by its power series in
-// g ln 2 (|g ln 2| <= 0.35: the eighth term is below 2^-27).
-TSB_HD u64 logit_mass(float x, const RowScale &r) {
-  if (x == r.top) return kOne;
-  const double t = ((double)r.top - (double)x) * r.c;
-  if (!(t < 43.0)) return 0;  // no mass (and NaN: a finite logit below +inf at an infinite temperature)
-  const int n = (int)t;
-  const float z = (0.5f - (float)(t - (double)n)) * 0.693147180559945f;
+// m of a token of bin < kBins: its weight as m * 2^-(23 + bin / kStep), except that
+// beyond the 19th octave, where units of 2^-42 are coarser, m is already in them.
+// t is d * c with the product's and c's own rounding errors put back; 2^-t from
+// the power series of e^z, |z| <= 0.36 (the next term is below 2^-26).
+TSB_HD uint32_t logit_m(float x, uint32_t bin, const RowScale &r) {
+  const float d = r.top - x;
+  const uint32_t n = bin / kStep;
+  const float t = d * r.c;
+  const float t_low = fmaf(d, r.c_low, fmaf(d, r.c, -t));
+  const float f = (t - (__uint_as_float(0x4B000000u | n) - 8388608.f)) + t_low;
+  const float z = (0.5f - f) * 0.693147180559945f;
   float p = 1.f / 5040.f;
   p = fmaf(p, z, 1.f / 720.f);
   p = fmaf(p, z, 1.f / 120.f);
@@ -105,40 +127,54 @@ TSB_HD u64 logit_mass(float x, const RowScale &r) {
   p = fmaf(p, z, 0.5f);
   p = fmaf(p, z, 1.f);
   p = fmaf(p, z, 1.f);
-  p *= 0.70710678118654752f;
-  return __float2ull_rn(p * __uint_as_float((uint32_t)(127 + 42 - n) << 23));
+  uint32_t m = (uint32_t)__float2int_rn(p * (0.70710678118654752f * 8388608.f));
+  if (t == 0.f) m = kTopM;
+  if (n > 19) m = (m + (1u << (n - 20))) >> (n - 19);
+  return m;
+}
+// Units of 2^-42 in a sum of the m of one bin.
+TSB_HD u64 bin_units(u64 m, uint32_t bin) {
+  const uint32_t n = bin / kStep;
+  return n < 19 ? m << (19 - n) : m;
+}
+TSB_HD u64 logit_mass(float x, const RowScale &r) {
+  const uint32_t bin = logit_bin(x, r);
+  return bin < (uint32_t)kBins ? bin_units(logit_m(x, bin, r), bin) : 0;
+}
+// No more tokens than this can make up `mass` units in a bin (a token's t is
+// within the bin's rounding, with room to spare); past the point where a unit is
+// coarse there is no useful bound.
+TSB_HD u64 most_tokens(u64 mass, int bin) {
+  const float least = exp2f(42.f - ((float)bin + 0.75f) / (float)kStep);
+  return least >= 256.f ? mass / (u64)(least - 2.f) : ~0ull;
 }
 
 // How the tokens that a bound falls among are resolved.
 enum Mode { kFew, kSlow, kOneBin, kRadix, kNoMass };
 
 struct Shared {
-  u64 mass[kBins];        // this CTA's histogram
-  u64 sum_mass[kBins];    // CTA 0: running masses of the row up to and including a bin
-  u64 list[kList];        // CTA 0: gathered tokens, key << 32 | ~index
-  unsigned int count[kBins];
-  unsigned int sum_count[kBins];
-  u64 peer_best[kMaxCluster];
-  u64 peer_floor[kMaxCluster];          // CTA 0
-  unsigned int peer_live[kMaxCluster];
-  unsigned int peer_ties[kMaxCluster];  // CTA 0
+  unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low and high 12 bits of m
+  u64 sums[kBins];                    // CTA 0: running counts or masses up to and including a bin
+  u64 list[kList];                    // CTA 0: gathered tokens, key << 32 | ~index
+  float peer_top[kMaxCluster];
+  u64 peer_floor[kMaxCluster];        // CTA 0
+  unsigned int peer_ties[kMaxCluster];
   u64 red[kWarps];
-  u64 scan_mass[kWarps];
-  unsigned int scan_count[kWarps];
+  u64 scan[kWarps];
   u64 found_mass;
   int found;
-  unsigned int list_n;
+  unsigned int list_n, first;
   // written by CTA 0 into every CTA
   int mode, lo, hi;
   uint32_t prefix;
   int pick_rank, pick_tie;
 };
-
 constexpr size_t kSharedBytes = (sizeof(Shared) + 15) & ~size_t(15);
 static_assert(kSharedBytes + kMaxStage <= 227 * 1024, "shared memory");
+static_assert(sizeof(u64) * 256 + 256 * 4 <= sizeof(u64) * kList, "the radix histogram lies in the list");
 
-// Calls f(token index, logit) for this CTA's live logits: elements [off, off + n)
-// of data, a 16-byte boundary; the first is token lo.
+// Calls f(token index, logit) for this CTA's logits: elements [off, off + n) of
+// data, which is a 16-byte boundary; the first is token lo.
 template <typename T, typename F>
 TSB_HD void for_logits(const T *data, int off, int lo, int n, F f) {
   constexpr int VEC = 16 / sizeof(T);
@@ -147,15 +183,9 @@ TSB_HD void for_logits(const T *data, int off, int lo, int n, F f) {
       const uint4 v = *reinterpret_cast<const uint4 *>(data + c);
       const T *e = reinterpret_cast<const T *>(&v);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const float x = to_float(e[j]);
-        if (x > -INFINITY) f(lo + c + j - off, x);  // false for NaN too
-      }
+      for (int j = 0; j < VEC; ++j) f(lo + c + j - off, to_float(e[j]));
     } else {  // a vector that sticks out of the slice
-      for (int i = max(c, off); i < min(c + VEC, off + n); ++i) {
-        const float x = to_float(data[i]);
-        if (x > -INFINITY) f(lo + i - off, x);
-      }
+      for (int i = max(c, off); i < min(c + VEC, off + n); ++i) f(lo + i - off, to_float(data[i]));
     }
   }
 }
@@ -171,23 +201,20 @@ TSB_HD u64 block_sum(u64 v, Shared &s) {
   return all;
 }
 
-// Inclusive scans of a value per thread over the block.
-TSB_HD void block_scan(u64 &m, unsigned int &c, Shared &s) {
+// Inclusive scan of a value per thread over the block.
+TSB_HD u64 block_scan(u64 v, Shared &s) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 um = __shfl_up_sync(0xffffffffu, m, o);
-    const unsigned int uc = __shfl_up_sync(0xffffffffu, c, o);
-    if (lane >= o) { m += um; c += uc; }
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
   }
   __syncthreads();
-  if (lane == 31) { s.scan_mass[warp] = m; s.scan_count[warp] = c; }
+  if (lane == 31) s.scan[warp] = v;
   __syncthreads();
-  u64 bm = 0;
-  unsigned int bc = 0;
-  for (int w = 0; w < warp; ++w) { bm += s.scan_mass[w]; bc += s.scan_count[w]; }
-  m += bm;
-  c += bc;
+  u64 before = 0;
+  for (int w = 0; w < warp; ++w) before += s.scan[w];
+  return before + v;
 }
 
 // Descending sort of list[0, n), n <= kList (padded with zeros to a power of two).
@@ -208,11 +235,9 @@ TSB_HD void sort_list(Shared &s, int n) {
   }
 }
 
-// Running masses of the sorted list, into sum_mass-like storage of its own.
-constexpr int kListPerThread = kList / kThreads;
+// Masses of the sorted list, running and own: thread t has elements t * kListPerThread + i.
 struct ListMasses {
-  u64 up_to[kListPerThread];  // inclusive running mass of list element thread * kListPerThread + i
-  u64 own[kListPerThread];
+  u64 up_to[kListPerThread], own[kListPerThread];
 };
 TSB_HD void list_masses(Shared &s, int n, const RowScale &r, ListMasses &m) {
   u64 run = 0;
@@ -223,17 +248,15 @@ TSB_HD void list_masses(Shared &s, int n, const RowScale &r, ListMasses &m) {
     run += m.own[i];
     m.up_to[i] = run;
   }
-  u64 all = run;
-  unsigned int unused = 0;
-  block_scan(all, unused, s);
+  const u64 before = block_scan(run, s) - run;
 #pragma unroll
-  for (int i = 0; i < kListPerThread; ++i) m.up_to[i] += all - run;
+  for (int i = 0; i < kListPerThread; ++i) m.up_to[i] += before;
 }
 
 // The first list element at which base + running mass reaches bound, into
-// s.found / s.found_mass (mass through it); found = -1 if none does.
+// s.found / s.found_mass (the mass through it).
 TSB_HD void list_cross(Shared &s, int n, u64 base, u64 bound, const ListMasses &m) {
-  if (threadIdx.x == 0) s.found = -1;
+  if (threadIdx.x == 0) { s.found = 0; s.found_mass = bound; }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kListPerThread; ++i) {
@@ -257,15 +280,15 @@ TSB_HD u64 top_p_bound(double p, u64 total) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared &s = *reinterpret_cast<Shared *>(smem);
   const cg::cluster_group cluster = cg::this_cluster();
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  for (int i = tid; i < kBins; i += kThreads) { s.count[i] = 0; s.mass[i] = 0; }
-  if (tid == 0) s.list_n = 0;
+  for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
+  if (tid == 0) { s.list_n = 0; s.first = 0xffffffffu; }
   griddep_wait();  // programmatic dependent: the logits are the previous kernel's
   griddep_launch_dependents();
 
@@ -276,133 +299,74 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
   const int off = (int)((reinterpret_cast<uintptr_t>(data) & 15) / sizeof(T));
   data -= off;
   const float u = a.u[row];
-  const double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
+  double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
   const double p = a.top_p ? a.top_p[row] : a.top_p_s;
   const double floor_w = a.min_p ? a.min_p[row] : a.min_p_s;
-  const int k = a.top_k ? a.top_k[row] : a.top_k_s;
+  int k = a.top_k ? a.top_k[row] : a.top_k_s;
   const bool greedy = !(temperature > 0.0);
+  temperature = fmax(temperature, kMinTemperature);
 
-  // ---- 1. the largest logit (lowest index first) and the number of live ones
-  u64 best = 0;
-  unsigned int live = 0;
-  if (a.staged) {
+  // ---- 1. the largest logit
+  float top = -INFINITY;
+  {
     constexpr int VEC = 16 / sizeof(T);
     T *stage = reinterpret_cast<T *>(smem + kSharedBytes);
     for (int c = tid * VEC; c < off + n; c += kThreads * VEC) {
       if (c >= off && c + VEC <= off + n) {
-        *reinterpret_cast<uint4 *>(stage + c) = ldg_nc_v4(data + c);
-      } else {
-        for (int i = max(c, off); i < min(c + VEC, off + n); ++i) stage[i] = data[i];
+        const uint4 v = ldg_nc_v4(data + c);
+        if (a.staged) *reinterpret_cast<uint4 *>(stage + c) = v;
+        top = max_of(v, top, T());
+      } else {  // a vector that sticks out of the slice
+        for (int i = max(c, off); i < min(c + VEC, off + n); ++i) {
+          const T v = data[i];
+          if (a.staged) stage[i] = v;
+          top = fmaxf(top, to_float(v));
+        }
       }
     }
-    data = stage;  // every thread reads back only what it wrote itself
+    if (a.staged) data = stage;  // in for_logits a thread reads what it wrote itself
   }
-  for_logits<T>(data, off, lo, n, [&](int i, float v) {
-    best = max(best, (u64)logit_key(v) << 32 | (uint32_t)~i);
-    ++live;
-  });
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    live += __shfl_xor_sync(0xffffffffu, live, o);
-  }
-  if (lane == 0) { s.scan_mass[warp] = best; s.scan_count[warp] = live; }
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if (lane == 0) s.red[warp] = __float_as_uint(top);
   __syncthreads();
-  best = s.scan_mass[0];
-  live = s.scan_count[0];
-  for (int w = 1; w < kWarps; ++w) { best = max(best, s.scan_mass[w]); live += s.scan_count[w]; }
-  if (tid < ctas) {
-    Shared *peer = cluster.map_shared_rank(&s, tid);
-    peer->peer_best[rank] = best;
-    peer->peer_live[rank] = live;
-  }
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, __uint_as_float((uint32_t)s.red[w]));
+  if (tid < ctas) cluster.map_shared_rank(&s, tid)->peer_top[rank] = top;
   cluster.sync();
-  best = 0;
-  live = 0;
-  for (int c = 0; c < ctas; ++c) { best = max(best, s.peer_best[c]); live += s.peer_live[c]; }
-  if (live == 0 || greedy) {  // nothing to choose, or no choice to make
+  for (int c = 0; c < ctas; ++c) top = fmaxf(top, s.peer_top[c]);
+  Shared *const head = cluster.map_shared_rank(&s, 0);
+
+  if (top == -INFINITY) {  // every logit is -inf or NaN: there is no token to choose
     if (rank == 0 && tid == 0) {
-      a.token[row] = live ? (int)~(uint32_t)best : -1;
-      if (a.logprob) a.logprob[row] = live ? 0.f : -INFINITY;
+      a.token[row] = -1;
+      if (a.logprob) a.logprob[row] = -INFINITY;
     }
     return;
   }
-  RowScale r;
-  r.top = key_logit((uint32_t)(best >> 32));
-  r.c = 1.4426950408889634 / temperature;
-  r.bin_scale = (float)(r.c * kStep);
-  const bool use_k = k > 0 && (unsigned int)k < live, use_p = p < 1.0, use_floor = floor_w > 0.0;
-  const u64 floor_mass = use_floor ? (u64)fmin(ceil(floor_w * (double)kOne), 2.0 * (double)kOne) : 0;
+  if (greedy) {
+    unsigned int first = 0xffffffffu;
+    for_logits<T>(data, off, lo, n, [&](int i, float v) { if (v == top) first = min(first, (unsigned int)i); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    if (lane == 0 && first != 0xffffffffu) atomicMin(&head->first, first);
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      a.token[row] = (int)s.first;
+      if (a.logprob) a.logprob[row] = 0.f;
+    }
+    return;
+  }
 
-  // ---- 2. the histogram, and the mass of the weights that min-p keeps
-  Shared *const head = cluster.map_shared_rank(&s, 0);
-  auto histogram = [&](bool with_mass) {
-    u64 above = 0;
-    for_logits<T>(data, off, lo, n, [&](int, float v) {
-      const int bin = logit_bin(v, r);
-      if (with_mass) {
-        const u64 m = logit_mass(v, r);
-        if (m) atomicAdd(&s.mass[bin], m);
-        if (m >= floor_mass) above += m;
-      }
-      atomicAdd(&s.count[bin], 1u);
-    });
-    above = block_sum(above, s);
-    if (tid == 0) head->peer_floor[rank] = above;
-  };
-  // CTA 0: adds the cluster's histograms up into running sums
-  u64 total = 0, above_floor = 0;
-  auto add_up = [&](bool with_mass) {
-    u64 m[kBinsPerThread];
-    unsigned int c[kBinsPerThread];
-    u64 run_m = 0;
-    unsigned int run_c = 0;
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const int bin = tid * kBinsPerThread + i;
-      m[i] = 0;
-      c[i] = 0;
-      if (bin < kBins) {
-        for (int q = 0; q < ctas; ++q) {
-          const Shared *peer = cluster.map_shared_rank(&s, q);
-          c[i] += peer->count[bin];
-          if (with_mass) m[i] += peer->mass[bin];
-        }
-      }
-      run_m += m[i];
-      run_c += c[i];
-    }
-    u64 up_m = run_m;
-    unsigned int up_c = run_c;
-    block_scan(up_m, up_c, s);
-    up_m -= run_m;
-    up_c -= run_c;
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const int bin = tid * kBinsPerThread + i;
-      up_m += m[i];
-      up_c += c[i];
-      if (bin < kBins) { s.sum_mass[bin] = up_m; s.sum_count[bin] = up_c; }
-    }
-    __syncthreads();
-    total = s.sum_mass[kBins - 1];
-    above_floor = 0;
-    for (int q = 0; q < ctas; ++q) above_floor += s.peer_floor[q];
-  };
-  // CTA 0: the bin in which the running count or mass reaches bound (the last one if none does)
-  auto find_bin = [&](bool by_count, u64 bound) -> int {
-    if (tid == 0) s.found = kBins - 1;
-    __syncthreads();
-    for (int bin = tid; bin < kBins; bin += kThreads) {
-      const u64 here = by_count ? s.sum_count[bin] : s.sum_mass[bin];
-      const u64 before = bin == 0 ? 0 : by_count ? s.sum_count[bin - 1] : s.sum_mass[bin - 1];
-      if (here >= bound && before < bound) s.found = bin;
-    }
-    __syncthreads();
-    const int bin = s.found;
-    __syncthreads();
-    return bin;
-  };
+  RowScale r;
+  const double c64 = 1.4426950408889634 / temperature;
+  r.top = top;
+  r.c = (float)c64;
+  r.c_low = (float)(c64 - (double)r.c);
+  r.bin_scale = (float)(c64 * kStep);
+  const bool use_p = p < 1.0, use_floor = floor_w > 0.0;
+  const u64 floor_mass = use_floor ? (u64)fmin(ceil(floor_w * (double)kOne), 2.0 * (double)kOne) : 0;
+  bool use_k = k > 0 && k < a.vocab;
+
   auto tell = [&](int mode, int b0, int b1) {  // CTA 0 to all
     if (tid < ctas) {
       Shared *peer = cluster.map_shared_rank(&s, tid);
@@ -411,52 +375,181 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       peer->hi = b1;
     }
   };
-  auto gather = [&](int b0, int b1) {  // all CTAs, into CTA 0's list
-    for_logits<T>(data, off, lo, n, [&](int i, float v) {
-      const int bin = logit_bin(v, r);
-      if (bin >= b0 && bin <= b1) head->list[atomicAdd(&head->list_n, 1u)] = (u64)logit_key(v) << 32 | (uint32_t)~i;
-    });
-  };
-  auto emit = [&](uint32_t key, int token, u64 kept) {
+  auto emit = [&](float v, int token, u64 kept) {
     if (token >= 0) a.token[row] = token;
     if (a.logprob) {
-      const float v = key_logit(key);
-      const double d = v == r.top ? 0.0 : ((double)v - (double)r.top) / temperature;
+      const double d = v == top ? 0.0 : ((double)v - (double)top) / temperature;
       a.logprob[row] = (float)(d - log((double)kept / (double)kOne));
     }
   };
-
-  const bool with_mass = !(use_k && k <= kCountOnlyK);
-  histogram(with_mass);
-  cluster.sync();
-  u64 base = 0;  // CTA 0: mass before the gathered bins
-  if (rank == 0) {
-    add_up(with_mass);
-    int b0 = 0, b1;
-    if (use_k) {
-      b1 = find_bin(true, (u64)k);
-    } else if (use_p) {
-      b1 = find_bin(false, top_p_bound(p, total));
-    } else {
-      const u64 kept = use_floor ? min(total, max(above_floor, kOne)) : total;
-      b0 = b1 = find_bin(false, sample_bound(u, kept));
-      base = b0 ? s.sum_mass[b0 - 1] : 0;
+  // All CTAs: the token number `tie` (CTA 0 knows it) of those with this logit, in index order.
+  auto pick = [&](float v, u64 kept, auto tie_of) {
+    unsigned int ties = 0;
+    for_logits<T>(data, off, lo, n, [&](int, float e) { ties += e == v; });
+    ties = (unsigned int)block_sum(ties, s);
+    if (tid == 0) head->peer_ties[rank] = ties;
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      unsigned int all = 0;
+      for (int q = 0; q < ctas; ++q) all += s.peer_ties[q];
+      u64 tie = tie_of(all, kept);
+      int q = 0;
+      while (q < ctas - 1 && tie >= s.peer_ties[q]) tie -= s.peer_ties[q++];
+      for (int c = 0; c < ctas; ++c) {
+        Shared *peer = cluster.map_shared_rank(&s, c);
+        peer->pick_rank = q;
+        peer->pick_tie = (int)tie;
+      }
+      emit(v, -1, kept);
     }
-    const unsigned int in = s.sum_count[b1] - (b0 ? s.sum_count[b0 - 1] : 0);
-    tell(in <= kList ? kFew : kSlow, b0, b1);
+    cluster.sync();
+    if (rank != s.pick_rank) return;
+    unsigned int seen = 0;  // ties before this block of tokens
+    for (int at = 0; at < n; at += kThreads) {
+      const bool hit = at + tid < n && to_float(data[off + at + tid]) == v;
+      const unsigned int up = (unsigned int)block_scan(hit, s);
+      if (hit && seen + up - 1 == (unsigned int)s.pick_tie) a.token[row] = lo + at + tid;
+      for (int q = 0; q < kWarps; ++q) seen += (unsigned int)s.scan[q];
+      if (seen > (unsigned int)s.pick_tie) return;
+    }
+  };
+
+  if (top == INFINITY) {  // the +inf logits share all the weight equally
+    pick(top, 0, [&](unsigned int all, u64 &kept) {
+      kept = (u64)(use_k ? min(all, (unsigned int)k) : all) * kOne;
+      if (use_p) kept = (top_p_bound(p, kept) + kOne - 1) / kOne * kOne;
+      if (use_floor && floor_mass > kOne) kept = kOne;
+      return (sample_bound(u, kept) + kOne - 1) / kOne - 1;
+    });
+    return;
   }
+
+  // ---- 2. the histogram, added up in CTA 0
+  auto push = [&](bool both) {
+    __syncthreads();
+    if (rank != 0) {
+      for (int i = tid; i < kBins; i += kThreads) {
+        if (s.h0[i]) atomicAdd(&head->h0[i], s.h0[i]);
+        if (both && s.h1[i]) atomicAdd(&head->h1[i], s.h1[i]);
+      }
+    }
+  };
+  auto count_tokens = [&]() {
+    for_logits<T>(data, off, lo, n, [&](int, float v) {
+      const uint32_t bin = logit_bin(v, r);
+      if (bin < (uint32_t)kBins) atomicAdd(&s.h0[bin], 1u);
+    });
+    push(false);
+  };
+  auto add_masses = [&]() {
+    u64 above = 0;  // what min-p keeps
+    for_logits<T>(data, off, lo, n, [&](int, float v) {
+      const uint32_t bin = logit_bin(v, r);
+      if (bin < (uint32_t)kBins) {
+        const uint32_t m = logit_m(v, bin, r);
+        atomicAdd(&s.h0[bin], m & 4095u);
+        atomicAdd(&s.h1[bin], m >> 12);
+        if (use_floor) {
+          const u64 units = bin_units(m, bin);
+          if (units >= floor_mass) above += units;
+        }
+      }
+    });
+    if (use_floor) {
+      above = block_sum(above, s);
+      if (tid == 0) head->peer_floor[rank] = above;
+    }
+    push(true);
+  };
+  // CTA 0: running sums of the histogram; returns the whole
+  auto run_sums = [&](bool masses) -> u64 {
+    u64 v[kBinsPerThread], run = 0;
+#pragma unroll
+    for (int i = 0; i < kBinsPerThread; ++i) {
+      const int bin = tid * kBinsPerThread + i;
+      v[i] = bin >= kBins ? 0 : masses ? bin_units((u64)s.h0[bin] + ((u64)s.h1[bin] << 12), bin) : s.h0[bin];
+      run += v[i];
+    }
+    u64 up = block_scan(run, s) - run;
+#pragma unroll
+    for (int i = 0; i < kBinsPerThread; ++i) {
+      const int bin = tid * kBinsPerThread + i;
+      up += v[i];
+      if (bin < kBins) s.sums[bin] = up;
+    }
+    __syncthreads();
+    return s.sums[kBins - 1];
+  };
+  // CTA 0: the bin in which the running sum reaches bound
+  auto find_bin = [&](u64 bound) -> int {
+    if (tid == 0) s.found = kBins - 1;
+    __syncthreads();
+    for (int bin = tid; bin < kBins; bin += kThreads)
+      if (s.sums[bin] >= bound && (bin == 0 || s.sums[bin - 1] < bound)) s.found = bin;
+    __syncthreads();
+    const int bin = s.found;
+    __syncthreads();
+    return bin;
+  };
+  auto before_bin = [&](int bin) -> u64 { return bin ? s.sums[bin - 1] : 0; };
+  auto gather = [&](int b0, int b1) {  // all CTAs, into CTA 0's list
+    for_logits<T>(data, off, lo, n, [&](int i, float v) {
+      const uint32_t bin = logit_bin(v, r);
+      if (bin >= (uint32_t)b0 && bin <= (uint32_t)b1) {
+        const unsigned int at = atomicAdd(&head->list_n, 1u);
+        if (at < (unsigned int)kList) head->list[at] = (u64)logit_key(v) << 32 | (uint32_t)~i;
+      }
+    });
+  };
+
+  if (use_k) count_tokens(); else add_masses();
+  cluster.sync();
+
+  // ---- 3. what to gather: CTA 0 decides
+  u64 total = 0, above_floor = 0, base = 0;  // base: mass before the gathered bins
+  int k_bin = 0;
+  u64 k_before = 0, k_in = 0;                // tokens before and in top-k's bin
+  if (rank == 0) {
+    total = run_sums(!use_k);
+    if (use_k) {
+      use_k = (u64)k < total;  // else every token with a mass is among the first k
+      k_bin = use_k ? find_bin((u64)k) : kBins - 1;
+      k_before = before_bin(k_bin);
+      k_in = s.sums[k_bin] - k_before;
+      tell(k_before + k_in <= kList ? kFew : kSlow, 0, k_bin);
+    } else {
+      if (use_floor)
+        for (int q = 0; q < ctas; ++q) above_floor += s.peer_floor[q];
+      int b0 = 0, b1;
+      if (use_p) {
+        b1 = find_bin(top_p_bound(p, total));
+      } else {
+        b0 = b1 = find_bin(sample_bound(u, use_floor ? min(total, max(above_floor, kOne)) : total));
+        base = before_bin(b0);
+      }
+      u64 tokens = 0;  // a bound on the tokens of the bins
+      for (int bin = b0 + tid; bin <= b1; bin += kThreads) {
+        const u64 mass = s.sums[bin] - before_bin(bin);
+        if (mass) tokens += min(most_tokens(mass, bin), (u64)kMaxVocab);
+      }
+      tokens = block_sum(tokens, s);
+      tell(tokens <= kList ? kFew : kSlow, b0, b1);
+    }
+  }
+  const bool counted = k > 0 && k < a.vocab;
   cluster.sync();
   if (s.mode == kFew) {
     gather(s.lo, s.hi);
     cluster.sync();
     if (rank != 0) return;
-    const int m = (int)s.list_n;
+    const int m = min((int)s.list_n, kList);
     sort_list(s, m);
     ListMasses lm;
     list_masses(s, m, r, lm);
     u64 kept = total;
-    if (use_k) {  // mass of the first k: the bins gathered hold them
-      if (tid == (k - 1) / kListPerThread) s.found_mass = lm.up_to[(k - 1) % kListPerThread];
+    if (counted) {  // the list holds the first k, or every token with a mass
+      const int last = min(use_k ? k : m, m) - 1;
+      if (tid == last / kListPerThread) s.found_mass = lm.up_to[last % kListPerThread];
       __syncthreads();
       kept = s.found_mass;
       __syncthreads();
@@ -467,46 +560,55 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       __syncthreads();
     }
     if (use_floor) {
-      u64 above = 0;
-      if (use_k || use_p) {  // min-p's tokens are a prefix of the order: those of them in the list decide
+      if (counted || use_p) {  // min-p keeps a prefix of the order: what of it is in the list decides
+        u64 above = 0;
 #pragma unroll
         for (int i = 0; i < kListPerThread; ++i) above += lm.own[i] >= floor_mass ? lm.own[i] : 0;
-        above = block_sum(above, s);
-      } else {
-        above = above_floor;
+        above_floor = block_sum(above, s);
       }
-      kept = min(kept, max(above, kOne));
+      kept = min(kept, max(above_floor, kOne));
     }
     list_cross(s, m, base, sample_bound(u, kept), lm);
     if (tid == 0) {
-      const u64 e = s.list[max(s.found, 0)];
-      emit((uint32_t)(e >> 32), (int)~(uint32_t)e, kept);
+      const u64 e = s.list[s.found];
+      emit(key_logit((uint32_t)(e >> 32)), (int)~(uint32_t)e, kept);
     }
     return;
   }
 
   // ---- many candidates: one bound after the other, each resolved inside its bin
-  if (!with_mass) {
-    for (int i = tid; i < kBins; i += kThreads) s.count[i] = 0;
-    __syncthreads();
-    histogram(true);
+  if (counted) {  // the masses are still to be added up
+    for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
     cluster.sync();
-    if (rank == 0) add_up(true);
+    add_masses();
+    cluster.sync();
+    if (rank == 0) {
+      total = run_sums(true);
+      if (use_floor)
+        for (int q = 0; q < ctas; ++q) above_floor += s.peer_floor[q];
+    }
   }
   u64 kept = total;  // CTA 0
-  for (int stage = 0; stage < 3; ++stage) {
-    if (stage == 0 ? !use_k : stage == 1 && !use_p) continue;
+  for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, u
+    if (stage == 0 ? !counted : stage == 1 && !use_p) continue;
     u64 bound = 0, mass_before = 0, count_before = 0;
     if (rank == 0) {
       if (stage == 2 && use_floor) kept = min(kept, max(above_floor, kOne));
-      bound = stage == 0 ? (u64)k : stage == 1 ? top_p_bound(p, kept) : sample_bound(u, kept);
-      const int bin = find_bin(stage == 0, bound);
-      mass_before = bin ? s.sum_mass[bin - 1] : 0;
-      count_before = bin ? s.sum_count[bin - 1] : 0;
-      const bool none = s.sum_mass[bin] == mass_before;  // the k-th token has no mass: nor has any after it
+      int bin;
+      if (stage == 0) {
+        bound = (u64)k;
+        bin = k_bin;
+        count_before = k_before;
+      } else {
+        bound = stage == 1 ? top_p_bound(p, kept) : sample_bound(u, kept);
+        bin = find_bin(bound);
+      }
+      mass_before = before_bin(bin);
+      const u64 mass = s.sums[bin] - mass_before;
+      int mode = (stage == 0 ? k_in : most_tokens(mass, bin)) <= kList ? kOneBin : kRadix;
+      if (stage == 0 && !use_k) mode = kNoMass;  // every token with a mass is kept
       if (tid == 0) s.list_n = 0;
-      tell(none ? kNoMass : s.sum_count[bin] - count_before <= kList ? kOneBin : kRadix, bin, bin);
-      if (none) kept = mass_before;
+      tell(mode, bin, bin);
     }
     cluster.sync();
     const int mode = s.mode, bin = s.lo;
@@ -518,7 +620,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       gather(bin, bin);
       cluster.sync();
       if (rank != 0) continue;
-      const int m = (int)s.list_n;
+      const int m = min((int)s.list_n, kList);
       sort_list(s, m);
       ListMasses lm;
       list_masses(s, m, r, lm);
@@ -531,8 +633,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       }
       if (stage == 2) {
         if (tid == 0) {
-          const u64 e = s.list[max(s.found, 0)];
-          emit((uint32_t)(e >> 32), (int)~(uint32_t)e, kept);
+          const u64 e = s.list[s.found];
+          emit(key_logit((uint32_t)(e >> 32)), (int)~(uint32_t)e, kept);
         }
       } else {
         kept = min(kept, s.found_mass);
@@ -540,88 +642,58 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant_
       __syncthreads();
       continue;
     }
-    // radix descent over the keys of the bin, eight bits at a time
+    // radix descent over the keys of the bin, eight bits at a time; its histogram
+    // of masses and counts takes the place of the list
+    u64 *const rmass = s.list;
+    unsigned int *const rcount = reinterpret_cast<unsigned int *>(s.list + 256);
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) { s.count[i] = 0; s.mass[i] = 0; }
+      for (int i = tid; i < 256; i += kThreads) { rmass[i] = 0; rcount[i] = 0; }
       __syncthreads();
       for_logits<T>(data, off, lo, n, [&](int, float v) {
+        if (logit_bin(v, r) != (uint32_t)bin) return;
         const uint32_t key = logit_key(v);
-        if (logit_bin(v, r) != bin || (shift < 24 && (key >> (shift + 8)) != prefix)) return;
-        atomicAdd(&s.count[(key >> shift) & 255u], 1u);
-        atomicAdd(&s.mass[(key >> shift) & 255u], logit_mass(v, r));
+        if (shift < 24 && (key >> (shift + 8)) != prefix) return;
+        atomicAdd(&rcount[(key >> shift) & 255u], 1u);
+        atomicAdd(&rmass[(key >> shift) & 255u], logit_mass(v, r));
       });
       cluster.sync();
       if (rank == 0) {
-        u64 m = 0;
-        unsigned int c = 0;
+        u64 m = 0, c = 0;
         const int digit = 255 - tid;  // descending
         if (tid < 256) {
           for (int q = 0; q < ctas; ++q) {
             const Shared *peer = cluster.map_shared_rank(&s, q);
-            m += peer->mass[digit];
-            c += peer->count[digit];
+            m += peer->list[digit];
+            c += reinterpret_cast<const unsigned int *>(peer->list + 256)[digit];
           }
         }
-        u64 up_m = m;
-        unsigned int up_c = c;
-        if (tid == 0) s.found = -1;
-        block_scan(up_m, up_c, s);
-        const u64 here = stage == 0 ? count_before + up_c : mass_before + up_m;
-        const u64 before = stage == 0 ? here - c : here - m;
-        if (tid < 256 && here >= bound && before < bound) s.found = tid;
-        __syncthreads();
-        if (tid == s.found) {
-          s.red[0] = mass_before + up_m - m;
-          s.red[1] = count_before + up_c - c;
+        if (tid == 0) s.found = 0;
+        const u64 up_m = mass_before + block_scan(m, s);
+        const u64 up_c = count_before + block_scan(c, s);
+        const u64 here = stage == 0 ? up_c : up_m, own = stage == 0 ? c : m;
+        if (tid < 256 && here >= bound && here - own < bound) {
+          s.found = tid;
+          s.found_mass = up_m - m;
+          s.red[0] = up_c - c;
         }
         __syncthreads();
-        mass_before = s.red[0];
-        count_before = s.red[1];
+        mass_before = s.found_mass;
+        count_before = s.red[0];
         if (tid < ctas) cluster.map_shared_rank(&s, tid)->prefix = prefix << 8 | (uint32_t)(255 - s.found);
       }
       cluster.sync();
       prefix = s.prefix;
     }
-    // every token left has the same key: `tie` of them come before the one wanted
-    const u64 w = logit_mass(key_logit(prefix), r);
-    u64 tie = 0;
-    if (rank == 0) {
-      tie = stage == 0 ? bound - count_before - 1 : (bound - mass_before + w - 1) / w - 1;
-      if (stage < 2) kept = min(kept, mass_before + (tie + 1) * w);
+    // every token left has the same logit: some of them come before the one wanted
+    const float v = key_logit(prefix);
+    const u64 w = logit_mass(v, r);
+    const u64 tie = stage == 0 ? bound - count_before - 1 : (bound - mass_before + w - 1) / max(w, 1ull) - 1;
+    if (stage < 2) {
+      kept = min(kept, mass_before + (tie + 1) * w);
+      continue;
     }
-    if (stage < 2) continue;
-    unsigned int ties = 0;
-    for_logits<T>(data, off, lo, n, [&](int, float v) { ties += logit_key(v) == prefix; });
-    ties = (unsigned int)block_sum(ties, s);
-    if (tid == 0) head->peer_ties[rank] = ties;
-    cluster.sync();
-    if (rank == 0) {
-      if (tid == 0) {
-        int q = 0;
-        while (q < ctas - 1 && tie >= s.peer_ties[q]) tie -= s.peer_ties[q++];
-        for (int c = 0; c < ctas; ++c) {
-          Shared *peer = cluster.map_shared_rank(&s, c);
-          peer->pick_rank = q;
-          peer->pick_tie = (int)tie;
-        }
-        emit(prefix, -1, kept);
-      }
-    }
-    cluster.sync();
-    if (rank != s.pick_rank) return;
-    // the tie in index order: this CTA's tokens, a block of them at a time
-    unsigned int seen = 0;
-    for (int at = 0; at < n; at += kThreads) {
-      const bool hit = at + tid < n && logit_key(to_float(data[off + at + tid])) == prefix;
-      u64 unused = 0;
-      unsigned int up = hit;
-      block_scan(unused, up, s);
-      if (hit && seen + up - 1 == (unsigned int)s.pick_tie) a.token[row] = lo + at + tid;
-      __syncthreads();
-      for (int q = 0; q < kWarps; ++q) seen += s.scan_count[q];
-      if (seen > (unsigned int)s.pick_tie) return;
-    }
+    pick(v, kept, [&](unsigned int, u64) { return tie; });
     return;
   }
 }
