@@ -10,15 +10,21 @@
 // count or mass along the order crosses a bound.
 //
 // A cluster of CTAs holds a row's logits in shared memory (one read of HBM).
+// Small top-k (k <= 64): each warp sorts its lanes' maxima; a bound that k lanes
+//   of a CTA reach leaves some tens of tokens per CTA, which CTA 0 gathers, cuts to
+//   the first k and walks with one warp. One cluster barrier in all.
+// Otherwise:
 //   1. The maximum, exchanged through distributed shared memory.
 //   2. A histogram over t in steps of 1/32, so fine that a bin holds few tokens:
 //      of counts with top-k, else of masses. The CTAs add theirs into CTA 0's.
 //   3. CTA 0 finds the bins in which the bounds fall; the tokens of those bins
 //      (all bins up to the last one wanted, or the sample's own bin alone) are
-//      gathered in its shared memory, sorted and walked.
+//      gathered in its shared memory, and a bound is resolved among the tokens of
+//      its bin: histograms over their (logit, index) narrow them down to 32 or
+//      fewer, which one warp sorts and walks.
 // Where the kept tokens are too many to list, the bounds are resolved one after
-// the other, each inside its bin: by a list of that bin, or, for a bin of
-// thousands of nearly equal logits, by a radix descent over their bits.
+// the other, each with a list of its own bin, or, for a bin of thousands of
+// nearly equal logits, by a radix descent over their bits.
 //
 // Masses are integers, units of 2^-42 of the largest weight: sums do not depend
 // on the order of the additions, results repeat bit for bit, and a row's mass
@@ -39,14 +45,15 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kStep = 32;              // bins per octave of the weight
 constexpr int kBins = 43 * kStep;      // a token of no bin has a mass of zero
 constexpr int kBinsPerThread = (kBins + kThreads - 1) / kThreads;
-constexpr int kList = 2048;            // tokens CTA 0 can sort
-constexpr int kListPerThread = kList / kThreads;
+constexpr int kList = 2048;            // tokens CTA 0 can hold
+constexpr int kDirectK = 64;           // top-k up to here is looked for among the lanes' maxima
+constexpr int kSub = kThreads;         // bins of a narrowing histogram, one per thread
 constexpr u64 kOne = 1ull << 42;       // the mass of the largest weight
 constexpr int kTopM = 1 << 23;         // its m
 constexpr int kMaxVocab = 1 << 20;
@@ -153,17 +160,23 @@ TSB_HD u64 most_tokens(u64 mass, int bin) {
 enum Mode { kFew, kSlow, kOneBin, kRadix, kNoMass };
 
 struct Shared {
-  unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low and high 12 bits of m
-  u64 sums[kBins];                    // CTA 0: running counts or masses up to and including a bin
-  u64 list[kList];                    // CTA 0: gathered tokens, key << 32 | ~index
+  union {
+    struct {
+      unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low and high 12 bits of m
+    };
+    u64 sums[kBins];                      // CTA 0: running counts or masses up to and including a bin
+  };
+  u64 list[kList];                        // CTA 0: gathered tokens, key << 32 | ~index
+  u64 few[kDirectK];
+  unsigned int sub0[kSub], sub1[kSub];
   float peer_top[kMaxCluster];
-  u64 peer_floor[kMaxCluster];        // CTA 0
+  u64 peer_floor[kMaxCluster];            // CTA 0
   unsigned int peer_ties[kMaxCluster];
-  u64 red[kWarps];
+  u64 red[kWarps], red2[kWarps];
   u64 scan[kWarps];
-  u64 found_mass;
+  u64 found_mass, found_token;
   int found;
-  unsigned int list_n, first;
+  unsigned int list_n, few_n, first;
   // written by CTA 0 into every CTA
   int mode, lo, hi;
   uint32_t prefix;
@@ -173,21 +186,32 @@ constexpr size_t kSharedBytes = (sizeof(Shared) + 15) & ~size_t(15);
 static_assert(kSharedBytes + kMaxStage <= 227 * 1024, "shared memory");
 static_assert(sizeof(u64) * 256 + 256 * 4 <= sizeof(u64) * kList, "the radix histogram lies in the list");
 
-// Calls f(token index, logit) for this CTA's logits: elements [off, off + n) of
-// data, which is a 16-byte boundary; the first is token lo.
+// Calls g(vector index, its 16 bytes) for the whole vectors of elements [off, off
+// + n) of data, a 16-byte boundary, and e(element index) for those at the ends. A
+// thread gets the same ones every time.
+template <typename T, typename G, typename E>
+TSB_HD void for_vectors(const T *data, int off, int n, G g, E e) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int v0 = (off + VEC - 1) / VEC, v1 = max((off + n) / VEC, v0);
+#pragma unroll 4
+  for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads) g(v);
+  const int head = min(v0 * VEC, off + n) - off, rest = off + n - max(v1 * VEC, off + head);
+  if ((int)threadIdx.x < head) e(off + (int)threadIdx.x);
+  if ((int)threadIdx.x >= 32 && (int)threadIdx.x - 32 < rest) e(max(v1 * VEC, off + head) + (int)threadIdx.x - 32);
+}
+// Calls f(token index, logit) for this CTA's logits, the first of which is token lo.
 template <typename T, typename F>
 TSB_HD void for_logits(const T *data, int off, int lo, int n, F f) {
   constexpr int VEC = 16 / sizeof(T);
-  for (int c = threadIdx.x * VEC; c < off + n; c += kThreads * VEC) {
-    if (c >= off && c + VEC <= off + n) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(data + c);
-      const T *e = reinterpret_cast<const T *>(&v);
+  for_vectors<T>(
+      data, off, n,
+      [&](int v) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(data + v * VEC);
+        const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) f(lo + c + j - off, to_float(e[j]));
-    } else {  // a vector that sticks out of the slice
-      for (int i = max(c, off); i < min(c + VEC, off + n); ++i) f(lo + i - off, to_float(data[i]));
-    }
-  }
+        for (int j = 0; j < VEC; ++j) f(lo + v * VEC + j - off, to_float(e[j]));
+      },
+      [&](int i) { f(lo + i - off, to_float(data[i])); });
 }
 
 TSB_HD u64 block_sum(u64 v, Shared &s) {
@@ -217,53 +241,121 @@ TSB_HD u64 block_scan(u64 v, Shared &s) {
   return before + v;
 }
 
-// Descending sort of list[0, n), n <= kList (padded with zeros to a power of two).
-TSB_HD void sort_list(Shared &s, int n) {
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kThreads) s.list[i] = 0;
-  __syncthreads();
-  for (int k = 2; k <= size; k <<= 1) {
+TSB_HD float token_logit(u64 token) { return key_logit((uint32_t)(token >> 32)); }
+TSB_HD int token_index(u64 token) { return (int)~(uint32_t)token; }
+
+// Descending bitonic sort of N = 32 or 64 values over a warp, element lane + 32 h in v[h].
+template <int N>
+TSB_HD void warp_sort(u64 (&v)[N / 32], int lane) {
+#pragma unroll
+  for (int k = 2; k <= N; k <<= 1) {
+#pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int p = threadIdx.x; p < size / 2; p += kThreads) {
-        const int i = 2 * p - (p & (j - 1)), l = i + j;
-        const u64 a = s.list[i], b = s.list[l];
-        if ((a < b) == ((i & k) == 0)) { s.list[i] = b; s.list[l] = a; }
+      if (j == 32) {
+        const u64 a = v[0], b = v[N / 32 - 1];
+        v[0] = max(a, b);
+        v[N / 32 - 1] = min(a, b);
+      } else {
+#pragma unroll
+        for (int h = 0; h < N / 32; ++h) {
+          const u64 other = __shfl_xor_sync(0xffffffffu, v[h], j);
+          const bool down = ((lane + 32 * h) & k) == 0, low = (lane & j) == 0;
+          v[h] = down == low ? max(v[h], other) : min(v[h], other);
+        }
       }
-      __syncthreads();
     }
   }
 }
-
-// Masses of the sorted list, running and own: thread t has elements t * kListPerThread + i.
-struct ListMasses {
-  u64 up_to[kListPerThread], own[kListPerThread];
-};
-TSB_HD void list_masses(Shared &s, int n, const RowScale &r, ListMasses &m) {
-  u64 run = 0;
+TSB_HD u64 warp_scan(u64 v, int lane) {
 #pragma unroll
-  for (int i = 0; i < kListPerThread; ++i) {
-    const int e = threadIdx.x * kListPerThread + i;
-    m.own[i] = e < n ? logit_mass(key_logit((uint32_t)(s.list[e] >> 32)), r) : 0;
-    run += m.own[i];
-    m.up_to[i] = run;
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
   }
-  const u64 before = block_scan(run, s) - run;
+  return v;
+}
+TSB_HD u64 warp_sum(u64 v) {
 #pragma unroll
-  for (int i = 0; i < kListPerThread; ++i) m.up_to[i] += before;
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
 
-// The first list element at which base + running mass reaches bound, into
-// s.found / s.found_mass (the mass through it).
-TSB_HD void list_cross(Shared &s, int n, u64 base, u64 bound, const ListMasses &m) {
-  if (threadIdx.x == 0) { s.found = 0; s.found_mass = bound; }
-  __syncthreads();
+// CTA 0: the first token, along the order, at which `before` plus the running
+// count or mass of the listed tokens of `bin` (all of the list for bin < 0, counts
+// only) that are at or above `floor_token` reaches bound; into s.found_token and
+// s.found_mass (the count or mass through it).
+TSB_HD void narrow(Shared &s, int n, int bin, u64 floor_token, bool by_count, u64 bound, u64 before, const RowScale &r) {
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  u64 lo = floor_token, hi = ~0ull;
+  auto each = [&](auto f) {
+    for (int e = tid; e < n; e += kThreads) {
+      const u64 t = s.list[e];
+      if (t >= lo && t <= hi && (bin < 0 || logit_bin(token_logit(t), r) == (uint32_t)bin)) f(t);
+    }
+  };
+  for (;;) {
+    u64 least = ~0ull, most = 0;
+    unsigned int count = 0;
+    each([&](u64 t) {
+      least = min(least, t);
+      most = max(most, t);
+      ++count;
+    });
 #pragma unroll
-  for (int i = 0; i < kListPerThread; ++i) {
-    const int e = threadIdx.x * kListPerThread + i;
-    if (e < n && m.own[i] && base + m.up_to[i] >= bound && base + m.up_to[i] - m.own[i] < bound) {
-      s.found = e;
-      s.found_mass = base + m.up_to[i];
+    for (int o = 16; o > 0; o >>= 1) {
+      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+    __syncthreads();
+    if (lane == 0) { s.red[warp] = least; s.red2[warp] = most; s.scan[warp] = count; }
+    s.sub0[tid] = 0;
+    s.sub1[tid] = 0;
+    if (tid == 0) { s.found = 0; s.found_mass = before; s.few_n = 0; }
+    __syncthreads();
+    count = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      least = min(least, s.red[w]);
+      most = max(most, s.red2[w]);
+      count += (unsigned int)s.scan[w];
+    }
+    if (count <= 32) break;
+    const int shift = max(0, 64 - __clzll((long long)(most - least)) - 8);
+    each([&](u64 t) {
+      const unsigned int sub = (unsigned int)((most - t) >> shift);
+      if (by_count) {
+        atomicAdd(&s.sub0[sub], 1u);
+      } else {
+        const uint32_t m = logit_m(token_logit(t), (uint32_t)bin, r);
+        atomicAdd(&s.sub0[sub], m & 4095u);
+        atomicAdd(&s.sub1[sub], m >> 12);
+      }
+    });
+    __syncthreads();
+    const u64 own = by_count ? s.sub0[tid] : bin_units((u64)s.sub0[tid] + ((u64)s.sub1[tid] << 12), (uint32_t)bin);
+    const u64 here = before + block_scan(own, s);
+    if (here >= bound && here - own < bound) {
+      s.found = tid;
+      s.found_mass = here - own;
+    }
+    __syncthreads();
+    before = s.found_mass;
+    hi = most - ((u64)s.found << shift);
+    const u64 width = (1ull << shift) - 1;
+    lo = max(lo, hi > width ? hi - width : 0ull);
+  }
+  each([&](u64 t) { s.few[atomicAdd(&s.few_n, 1u)] = t; });
+  __syncthreads();
+  if (warp == 0) {
+    u64 v[1] = {lane < (int)s.few_n ? s.few[lane] : 0ull};
+    warp_sort<32>(v, lane);
+    const u64 own = v[0] == 0 ? 0 : by_count ? 1 : logit_mass(token_logit(v[0]), r);
+    const u64 here = before + warp_scan(own, lane);
+    const unsigned int at = __ballot_sync(0xffffffffu, here >= bound && own);
+    const int first = at ? __ffs(at) - 1 : 0;
+    if (lane == first) {
+      s.found_token = v[0];
+      s.found_mass = here;
     }
   }
   __syncthreads();
@@ -279,8 +371,11 @@ TSB_HD u64 top_p_bound(double p, u64 total) {
   return min(max(b, 1ull), total);
 }
 
+TSB_HD void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+TSB_HD void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_constant__ SampleArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_constant__ SampleArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   Shared &s = *reinterpret_cast<Shared *>(smem);
   const cg::cluster_group cluster = cg::this_cluster();
@@ -289,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
   if (tid == 0) { s.list_n = 0; s.first = 0xffffffffu; }
+  cluster_arrive();  // waited for before the first access to another CTA's shared memory
   griddep_wait();  // programmatic dependent: the logits are the previous kernel's
   griddep_launch_dependents();
 
@@ -306,26 +402,135 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   const bool greedy = !(temperature > 0.0);
   temperature = fmax(temperature, kMinTemperature);
 
-  // ---- 1. the largest logit
-  float top = -INFINITY;
+  float top = -INFINITY;  // this thread's largest logit
   {
     constexpr int VEC = 16 / sizeof(T);
     T *stage = reinterpret_cast<T *>(smem + kSharedBytes);
-    for (int c = tid * VEC; c < off + n; c += kThreads * VEC) {
-      if (c >= off && c + VEC <= off + n) {
-        const uint4 v = ldg_nc_v4(data + c);
-        if (a.staged) *reinterpret_cast<uint4 *>(stage + c) = v;
-        top = max_of(v, top, T());
-      } else {  // a vector that sticks out of the slice
-        for (int i = max(c, off); i < min(c + VEC, off + n); ++i) {
-          const T v = data[i];
-          if (a.staged) stage[i] = v;
-          top = fmaxf(top, to_float(v));
-        }
+    for_vectors<T>(
+        data, off, n,
+        [&](int v) {
+          const uint4 w = ldg_nc_v4(data + v * VEC);
+          if (a.staged) *reinterpret_cast<uint4 *>(stage + v * VEC) = w;
+          top = max_of(w, top, T());
+        },
+        [&](int i) {
+          const T w = data[i];
+          if (a.staged) stage[i] = w;
+          top = fmaxf(top, to_float(w));
+        });
+    if (a.staged) data = stage;  // a thread reads back what it wrote itself
+  }
+  Shared *const head = cluster.map_shared_rank(&s, 0);
+  auto emit = [&](float v, int token, u64 kept) {
+    if (token >= 0) a.token[row] = token;
+    if (a.logprob) {
+      const double d = v == top ? 0.0 : ((double)v - (double)top) / temperature;
+      a.logprob[row] = (float)(d - log((double)kept / (double)kOne));
+    }
+  };
+  const bool use_p = p < 1.0, use_floor = floor_w > 0.0;
+  const u64 floor_mass = use_floor ? (u64)fmin(ceil(floor_w * (double)kOne), 2.0 * (double)kOne) : 0;
+  const double c64 = 1.4426950408889634 / temperature;
+  RowScale r;
+  r.c = (float)c64;
+  r.c_low = (float)(c64 - (double)r.c);
+  r.bin_scale = (float)(c64 * kStep);
+
+  // ---- small top-k: tokens that some k lanes' maxima reach
+  if (!greedy && k > 0 && k <= kDirectK && k < a.vocab) {
+    float v = top;  // the warp's lanes in descending order
+#pragma unroll
+    for (int g = 2; g <= 32; g <<= 1) {
+#pragma unroll
+      for (int j = g >> 1; j > 0; j >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v, j);
+        v = ((lane & g) == 0) == ((lane & j) == 0) ? fmaxf(v, other) : fminf(v, other);
       }
     }
-    if (a.staged) data = stage;  // in for_logits a thread reads what it wrote itself
+    if (lane == (k - 1) / kWarps) s.red[warp] = __float_as_uint(v);  // ceil(k / warps) lanes of each warp reach it
+    __syncthreads();
+    float cut = __uint_as_float((uint32_t)s.red[0]);
+    for (int w = 1; w < kWarps; ++w) cut = fminf(cut, __uint_as_float((uint32_t)s.red[w]));
+    cluster_wait();
+    for_logits<T>(data, off, lo, n, [&](int i, float e) {
+      if (e >= cut && e > -INFINITY) {
+        const unsigned int at = atomicAdd(&head->list_n, 1u);
+        if (at < (unsigned int)kList) head->list[at] = (u64)logit_key(e) << 32 | (uint32_t)~i;
+      }
+    });
+    cluster.sync();
+    const int m = (int)head->list_n;
+    cluster_arrive();  // CTA 0 stays until every CTA has read it
+    if (m <= kList) {
+      if (rank != 0) {
+        cluster_wait();
+        return;
+      }
+      u64 floor_token = 0;
+      if (m > kDirectK) {
+        narrow(s, m, -1, 0, true, (u64)k, 0, r);
+        floor_token = s.found_token;
+      }
+      if (tid == 0) s.few_n = 0;
+      __syncthreads();
+      for (int e = tid; e < m; e += kThreads) {
+        const u64 t = s.list[e];
+        if (t >= floor_token) s.few[atomicAdd(&s.few_n, 1u)] = t;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        const int have = (int)s.few_n;
+        u64 t[2], own[2], up[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) t[h] = lane + 32 * h < have ? s.few[lane + 32 * h] : 0ull;
+        warp_sort<kDirectK>(t, lane);
+        const int kept_n = min(have, k);
+        top = token_logit(__shfl_sync(0xffffffffu, t[0], 0));
+        r.top = top;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e = token_logit(t[h]);
+          own[h] = lane + 32 * h >= kept_n ? 0 : e == top ? kOne : top == INFINITY ? 0 : logit_mass(e, r);
+        }
+        up[0] = warp_scan(own[0], lane);
+        const u64 first_half = __shfl_sync(0xffffffffu, up[0], 31);
+        up[1] = first_half + warp_scan(own[1], lane);
+        u64 kept = __shfl_sync(0xffffffffu, up[1], 31);
+        // the place of the first token whose running mass reaches a bound
+        auto cross = [&](u64 bound) -> int {
+          const unsigned int a0 = __ballot_sync(0xffffffffu, up[0] >= bound && own[0]);
+          const unsigned int a1 = __ballot_sync(0xffffffffu, up[1] >= bound && own[1]);
+          return a0 ? __ffs(a0) - 1 : a1 ? __ffs(a1) + 31 : 0;
+        };
+        auto at = [&](const u64 (&w)[2], int i) -> u64 {
+          const u64 w0 = __shfl_sync(0xffffffffu, w[0], i & 31), w1 = __shfl_sync(0xffffffffu, w[1], i & 31);
+          return i < 32 ? w0 : w1;
+        };
+        if (kept == 0) {
+          if (lane == 0) {
+            a.token[row] = -1;
+            if (a.logprob) a.logprob[row] = -INFINITY;
+          }
+        } else {
+          if (use_p) kept = min(kept, at(up, cross(top_p_bound(p, kept))));
+          if (use_floor) {
+            const u64 above = warp_sum((own[0] >= floor_mass ? own[0] : 0) + (own[1] >= floor_mass ? own[1] : 0));
+            kept = min(kept, max(above, kOne));
+          }
+          const u64 token = at(t, cross(sample_bound(u, kept)));
+          if (lane == 0) emit(token_logit(token), token_index(token), kept);
+        }
+      }
+      cluster_wait();
+      return;
+    }
+    cluster_wait();  // too many (equal logits, or hardly any live ones): the general way
+    if (tid == 0) s.list_n = 0;
+  } else {
+    cluster_wait();
   }
+
+  // ---- 1. the largest logit
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s.red[warp] = __float_as_uint(top);
@@ -334,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   if (tid < ctas) cluster.map_shared_rank(&s, tid)->peer_top[rank] = top;
   cluster.sync();
   for (int c = 0; c < ctas; ++c) top = fmaxf(top, s.peer_top[c]);
-  Shared *const head = cluster.map_shared_rank(&s, 0);
 
   if (top == -INFINITY) {  // every logit is -inf or NaN: there is no token to choose
     if (rank == 0 && tid == 0) {
@@ -357,15 +561,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
     return;
   }
 
-  RowScale r;
-  const double c64 = 1.4426950408889634 / temperature;
   r.top = top;
-  r.c = (float)c64;
-  r.c_low = (float)(c64 - (double)r.c);
-  r.bin_scale = (float)(c64 * kStep);
-  const bool use_p = p < 1.0, use_floor = floor_w > 0.0;
-  const u64 floor_mass = use_floor ? (u64)fmin(ceil(floor_w * (double)kOne), 2.0 * (double)kOne) : 0;
   bool use_k = k > 0 && k < a.vocab;
+  const bool counted = use_k;
 
   auto tell = [&](int mode, int b0, int b1) {  // CTA 0 to all
     if (tid < ctas) {
@@ -373,13 +571,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       peer->mode = mode;
       peer->lo = b0;
       peer->hi = b1;
-    }
-  };
-  auto emit = [&](float v, int token, u64 kept) {
-    if (token >= 0) a.token[row] = token;
-    if (a.logprob) {
-      const double d = v == top ? 0.0 : ((double)v - (double)top) / temperature;
-      a.logprob[row] = (float)(d - log((double)kept / (double)kOne));
     }
   };
   // All CTAs: the token number `tie` (CTA 0 knows it) of those with this logit, in index order.
@@ -506,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
   cluster.sync();
 
   // ---- 3. what to gather: CTA 0 decides
-  u64 total = 0, above_floor = 0, base = 0;  // base: mass before the gathered bins
+  u64 total = 0, above_floor = 0;
   int k_bin = 0;
   u64 k_before = 0, k_in = 0;                // tokens before and in top-k's bin
   if (rank == 0) {
@@ -525,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
         b1 = find_bin(top_p_bound(p, total));
       } else {
         b0 = b1 = find_bin(sample_bound(u, use_floor ? min(total, max(above_floor, kOne)) : total));
-        base = before_bin(b0);
+        
       }
       u64 tokens = 0;  // a bound on the tokens of the bins
       for (int bin = b0 + tid; bin <= b1; bin += kThreads) {
@@ -536,43 +727,52 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       tell(tokens <= kList ? kFew : kSlow, b0, b1);
     }
   }
-  const bool counted = k > 0 && k < a.vocab;
   cluster.sync();
   if (s.mode == kFew) {
     gather(s.lo, s.hi);
     cluster.sync();
     if (rank != 0) return;
     const int m = min((int)s.list_n, kList);
-    sort_list(s, m);
-    ListMasses lm;
-    list_masses(s, m, r, lm);
-    u64 kept = total;
-    if (counted) {  // the list holds the first k, or every token with a mass
-      const int last = min(use_k ? k : m, m) - 1;
-      if (tid == last / kListPerThread) s.found_mass = lm.up_to[last % kListPerThread];
+    u64 floor_token = 0, kept = total;
+    if (counted) {
+      // the list holds the first k, or every token with a mass: their masses by bin
+      if (use_k) {
+        narrow(s, m, k_bin, 0, true, (u64)k, k_before, r);
+        floor_token = s.found_token;
+      }
+      for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
       __syncthreads();
-      kept = s.found_mass;
+      for (int e = tid; e < m; e += kThreads) {
+        if (s.list[e] < floor_token) continue;
+        const float v = token_logit(s.list[e]);
+        const uint32_t bin = logit_bin(v, r), w = logit_m(v, bin, r);
+        atomicAdd(&s.h0[bin], w & 4095u);
+        atomicAdd(&s.h1[bin], w >> 12);
+      }
       __syncthreads();
+      kept = run_sums(true);
     }
     if (use_p) {
-      list_cross(s, m, 0, top_p_bound(p, kept), lm);
+      const u64 bound = top_p_bound(p, kept);
+      const int bin = find_bin(bound);
+      narrow(s, m, bin, floor_token, false, bound, before_bin(bin), r);
       kept = min(kept, s.found_mass);
-      __syncthreads();
     }
     if (use_floor) {
       if (counted || use_p) {  // min-p keeps a prefix of the order: what of it is in the list decides
         u64 above = 0;
-#pragma unroll
-        for (int i = 0; i < kListPerThread; ++i) above += lm.own[i] >= floor_mass ? lm.own[i] : 0;
+        for (int e = tid; e < m; e += kThreads) {
+          const u64 w = s.list[e] >= floor_token ? logit_mass(token_logit(s.list[e]), r) : 0;
+          above += w >= floor_mass ? w : 0;
+        }
         above_floor = block_sum(above, s);
       }
       kept = min(kept, max(above_floor, kOne));
     }
-    list_cross(s, m, base, sample_bound(u, kept), lm);
-    if (tid == 0) {
-      const u64 e = s.list[s.found];
-      emit(key_logit((uint32_t)(e >> 32)), (int)~(uint32_t)e, kept);
-    }
+    const u64 bound = sample_bound(u, kept);
+    const int bin = find_bin(bound);
+    narrow(s, m, bin, floor_token, false, bound, before_bin(bin), r);
+    if (tid == 0) emit(token_logit(s.found_token), token_index(s.found_token), kept);
     return;
   }
 
@@ -620,24 +820,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const __grid_consta
       gather(bin, bin);
       cluster.sync();
       if (rank != 0) continue;
-      const int m = min((int)s.list_n, kList);
-      sort_list(s, m);
-      ListMasses lm;
-      list_masses(s, m, r, lm);
-      if (stage == 0) {
-        const int e = (int)(bound - count_before) - 1;
-        if (tid == e / kListPerThread) s.found_mass = mass_before + lm.up_to[e % kListPerThread];
-        __syncthreads();
-      } else {
-        list_cross(s, m, mass_before, bound, lm);
-      }
+      narrow(s, min((int)s.list_n, kList), bin, 0, stage == 0, bound, stage == 0 ? count_before : mass_before, r);
+      const u64 token = s.found_token;
       if (stage == 2) {
-        if (tid == 0) {
-          const u64 e = s.list[s.found];
-          emit(key_logit((uint32_t)(e >> 32)), (int)~(uint32_t)e, kept);
-        }
-      } else {
+        if (tid == 0) emit(token_logit(token), token_index(token), kept);
+      } else if (stage == 1) {
         kept = min(kept, s.found_mass);
+      } else {  // the mass of the first k
+        u64 mass = 0;
+        for (int e = tid; e < min((int)s.list_n, kList); e += kThreads)
+          if (s.list[e] >= token) mass += logit_mass(token_logit(s.list[e]), r);
+        kept = mass_before + block_sum(mass, s);
       }
       __syncthreads();
       continue;
