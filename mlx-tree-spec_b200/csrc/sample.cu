@@ -12,7 +12,7 @@
 // A cluster of CTAs holds a row's logits in shared memory (one read of HBM).
 // Small top-k (k <= 64): each warp sorts its lanes' maxima; a bound that k lanes
 //   of a CTA reach leaves some tens of tokens per CTA, which CTA 0 gathers, cuts to
-//   the first k and walks with one warp. One cluster barrier in all.
+//   about k and puts in order. One cluster barrier in all.
 // Otherwise:
 //   1. The maximum, exchanged through distributed shared memory.
 //   2. A histogram over t in steps of 1/32, so fine that a bin holds few tokens:
@@ -20,19 +20,24 @@
 //   3. CTA 0 finds the bins in which the bounds fall; the tokens of those bins
 //      (all bins up to the last one wanted, or the sample's own bin alone) are
 //      gathered in its shared memory, and a bound is resolved among the tokens of
-//      its bin: histograms over their (logit, index) narrow them down to 32 or
-//      fewer, which one warp sorts and walks.
+//      its bin: histograms over t, then over (logit, index), narrow them down to
+//      a hundred or so, which are put in order.
 // Where the kept tokens are too many to list, the bounds are resolved one after
 // the other, each with a list of its own bin, or, for a bin of thousands of
 // nearly equal logits, by a radix descent over their bits.
 //
-// Masses are integers, units of 2^-42 of the largest weight: sums do not depend
-// on the order of the additions, results repeat bit for bit, and a row's mass
-// stays below 2^62. A token's mass is m * 2^(19 - t's octave), m of 24 bits from a
-// float32 power series of the exactly reduced t; the roundings of m are independent
-// from token to token and do not add up. A bin lies in one octave, so its sum of
-// m needs two 32-bit shared-memory atomics per token (12 bits each, 2^20 tokens
-// do not overflow them); a 64-bit one would be a compare-and-swap loop.
+// Masses. Inside a bin (t within 1/64 of bin / 32) a token's weight is m * 2^-22 *
+// 2^(-bin / 32) with m an integer of 23 bits: a float32 series of the exactly
+// reduced t, whose roundings are independent from token to token and do not add
+// up. Sums over a bin's tokens are sums of integers, so they do not depend on the
+// order of the atomics and results repeat bit for bit; sums over bins are taken in
+// 64-bit floats in a fixed order. m goes into two 32-bit shared-memory atomics of 12
+// and 11 bits (2^20 tokens do not overflow them); a 64-bit one would be a
+// compare-and-swap loop.
+//
+// A call of few rows is bound by the latency of these steps one after the other, not
+// by their work: tokens wanted are found as bit masks over 32 logits at a time, and a
+// short list is ordered by counting, for each of its tokens, those before it.
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
@@ -54,13 +59,14 @@ constexpr int kBinsPerThread = (kBins + kThreads - 1) / kThreads;
 constexpr int kList = 2048;            // tokens CTA 0 can hold
 constexpr int kDirectK = 64;           // top-k up to here is looked for among the lanes' maxima
 constexpr int kSub = kThreads;         // bins of a narrowing histogram, one per thread
-constexpr u64 kOne = 1ull << 42;       // the mass of the largest weight
-constexpr int kTopM = 1 << 23;         // its m
+constexpr int kFewest = 128;           // tokens put in order by counting, two threads each
+constexpr int kUnitM = 1 << 22;        // m of a token in the middle of its bin
 constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxStage = 160 * 1024;  // bytes of logits a CTA holds in shared memory
 constexpr size_t kSliceBytes = 48 * 1024;  // of logits in a CTA, while there are CTAs to split them over
 constexpr int kSliceMin = 4096;            // logits of a slice that is not split further
 constexpr double kMinTemperature = 8.673617379884035e-19;  // 2^-60
+constexpr double kMaxTemperature = 1.2676506002282294e30;  // 2^100
 
 struct SampleArgs {
   const void *logits;
@@ -79,82 +85,73 @@ TSB_HD float to_float(float x) { return x; }
 TSB_HD float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 TSB_HD float to_float(__half x) { return __half2float(x); }
 
-// Largest of 16 bytes of logits and m; NaN is skipped.
-TSB_HD float max_of(const uint4 &v, float m, float) {
-  return fmaxf(fmaxf(m, fmaxf(__uint_as_float(v.x), __uint_as_float(v.y))),
-               fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+// Largest of 16 bytes of logits; NaN is skipped.
+TSB_HD float max_of(const uint4 &v, float) {
+  return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
 }
-TSB_HD float max_of(const uint4 &v, float m, __nv_bfloat16) {
+TSB_HD float max_of(const uint4 &v, __nv_bfloat16) {
   const __nv_bfloat162 a = __hmax2(__hmax2(u32_as_bf2(v.x), u32_as_bf2(v.y)), __hmax2(u32_as_bf2(v.z), u32_as_bf2(v.w)));
-  return fmaxf(m, fmaxf(__low2float(a), __high2float(a)));
+  return fmaxf(__low2float(a), __high2float(a));
 }
-TSB_HD float max_of(const uint4 &v, float m, __half) {
+TSB_HD float max_of(const uint4 &v, __half) {
   const __half2 *h = reinterpret_cast<const __half2 *>(&v);
   const __half2 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(m, fmaxf(__low2float(a), __high2float(a)));
+  return fmaxf(__low2float(a), __high2float(a));
 }
 
-// Order-preserving bits: a larger logit has a larger key, -0 that of +0.
-TSB_HD uint32_t logit_key(float x) {
+// A token as a number that orders like the sampling does: order-preserving bits
+// of its logit (-0 as +0), then its index, lower first.
+TSB_HD u64 make_token(float x, int index) {
   const uint32_t b = __float_as_uint(x + 0.f);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+  return (u64)((b & 0x80000000u) ? ~b : (b | 0x80000000u)) << 32 | (uint32_t)~index;
 }
 TSB_HD float key_logit(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k); }
+TSB_HD float token_logit(u64 token) { return key_logit((uint32_t)(token >> 32)); }
+TSB_HD int token_index(u64 token) { return (int)~(uint32_t)token; }
 
-// A row whose largest logit is finite.
 struct RowScale {
-  float top;        // the largest logit
-  float bin_scale;  // kStep * c
-  float c, c_low;   // log2(e) / temperature
+  float top;           // the largest logit
+  float scale, low;    // kStep * log2(e) / temperature, and what the float leaves of it
 };
 
 // Bin of a logit, never decreasing as the logit falls: round(kStep * t). At or past
 // kBins for a token without mass, -inf and NaN among them (the float's bits are
 // compared as a number).
 TSB_HD uint32_t logit_bin(float x, const RowScale &r) {
-  return __float_as_uint(fmaf(r.top - x, r.bin_scale, 8388608.f)) - 0x4B000000u;
+  return __float_as_uint(fmaf(r.top - x, r.scale, 8388608.f)) - 0x4B000000u;
 }
-
-// m of a token of bin < kBins: its weight as m * 2^-(23 + bin / kStep), except that
-// beyond the 19th octave, where units of 2^-42 are coarser, m is already in them.
-// t is d * c with the product's and c's own rounding errors put back; 2^-t from
-// the power series of e^z, |z| <= 0.36 (the next term is below 2^-26).
+// m of a token of bin < kBins: 2^22 * 2^(-g / 32), g = kStep * t - bin in [-1/2, 1/2]
+// up to the roundings of t, from the series of e^z at |z| <= 0.011 (the next term is
+// below 2^-31). The last addition leaves the rounded integer in the mantissa.
 TSB_HD uint32_t logit_m(float x, uint32_t bin, const RowScale &r) {
   const float d = r.top - x;
-  const uint32_t n = bin / kStep;
-  const float t = d * r.c;
-  const float t_low = fmaf(d, r.c_low, fmaf(d, r.c, -t));
-  const float f = (t - (__uint_as_float(0x4B000000u | n) - 8388608.f)) + t_low;
-  const float z = (0.5f - f) * 0.693147180559945f;
-  float p = 1.f / 5040.f;
-  p = fmaf(p, z, 1.f / 720.f);
-  p = fmaf(p, z, 1.f / 120.f);
-  p = fmaf(p, z, 1.f / 24.f);
-  p = fmaf(p, z, 1.f / 6.f);
-  p = fmaf(p, z, 0.5f);
-  p = fmaf(p, z, 1.f);
-  p = fmaf(p, z, 1.f);
-  uint32_t m = (uint32_t)__float2int_rn(p * (0.70710678118654752f * 8388608.f));
-  if (t == 0.f) m = kTopM;
-  if (n > 19) m = (m + (1u << (n - 20))) >> (n - 19);
-  return m;
+  const float b = __uint_as_float(0x4B000000u | bin) - 8388608.f;
+  const float z = fmaf(d, r.low, fmaf(d, r.scale, -b)) * (-0.693147180559945f / kStep);
+  const float p = fmaf(fmaf(fmaf(z, 1.f / 6.f, 0.5f), z, 1.f), z * (float)kUnitM, 8388608.f + (float)kUnitM);
+  return __float_as_uint(p) & 0x7FFFFFu;
 }
-// Units of 2^-42 in a sum of the m of one bin.
-TSB_HD u64 bin_units(u64 m, uint32_t bin) {
-  const uint32_t n = bin / kStep;
-  return n < 19 ? m << (19 - n) : m;
+// Weight of one unit of m in a bin.
+__constant__ double kOctave[kStep] = {
+    1.0, 0.97857206208770013, 0.9576032806985737, 0.93708381705514999, 0.91700404320467123, 0.89735453750155359,
+    0.8781260801866497, 0.85930964906123897, 0.8408964152537145, 0.82287773907698243, 0.80524516597462714,
+    0.78799042255394325, 0.77110541270397037, 0.75458221379671136, 0.73841307296974967, 0.72259040348852331,
+    0.70710678118654752, 0.69195494098191597, 0.67712777346844632, 0.66261832157987064, 0.64841977732550475,
+    0.63452547859586661, 0.62092890603674202, 0.60762367999023449, 0.59460355750136054, 0.58186242938878875,
+    0.5693943173783458, 0.55719337129794622, 0.54525386633262887, 0.53357020033841180, 0.52213689121370688,
+    0.51094857432705836};
+// `octave` is a copy of kOctave in shared memory: lanes ask for different ones.
+TSB_HD double bin_unit(uint32_t bin, const double *octave) {
+  return octave[bin % kStep] * __hiloint2double((int)(1023u - 22u - bin / kStep) << 20, 0);
 }
-TSB_HD u64 logit_mass(float x, const RowScale &r) {
+TSB_HD double logit_mass(float x, const RowScale &r, const double *octave) {
   const uint32_t bin = logit_bin(x, r);
-  return bin < (uint32_t)kBins ? bin_units(logit_m(x, bin, r), bin) : 0;
+  return bin < (uint32_t)kBins ? (double)logit_m(x, bin, r) * bin_unit(bin, octave) : 0.0;
 }
-// No more tokens than this can make up `mass` units in a bin (a token's t is
-// within the bin's rounding, with room to spare); past the point where a unit is
-// coarse there is no useful bound.
-TSB_HD u64 most_tokens(u64 mass, int bin) {
-  const float least = exp2f(42.f - ((float)bin + 0.75f) / (float)kStep);
-  return least >= 256.f ? mass / (u64)(least - 2.f) : ~0ull;
-}
+
+// Masses of tokens of several bins are added up as whole numbers of 2^-40, whose
+// sums do not depend on the list's order either.
+constexpr double kListUnit = 1099511627776.0;
+TSB_HD u64 list_units(double mass) { return (u64)__double2ll_rn(mass * kListUnit); }
 
 // How the tokens that a bound falls among are resolved.
 enum Mode { kFew, kSlow, kOneBin, kRadix, kNoMass };
@@ -162,21 +159,26 @@ enum Mode { kFew, kSlow, kOneBin, kRadix, kNoMass };
 struct Shared {
   union {
     struct {
-      unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low and high 12 bits of m
+      unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low 12 and the high bits of m
     };
-    u64 sums[kBins];                      // CTA 0: running counts or masses up to and including a bin
+    double sums[kBins];                   // CTA 0: running counts or masses up to and including a bin
   };
-  u64 list[kList];                        // CTA 0: gathered tokens, key << 32 | ~index
-  u64 few[kDirectK];
+  u64 list[kList];                        // tokens found; in CTA 0 its own from the front, the others' from the back
+  ulonglong2 few[kFewest];                // tokens and their units of count or mass
+  u64 order[kFewest], up_to[kFewest];     // in order, and the running units
   unsigned int sub0[kSub], sub1[kSub];
+  double octave[kStep];
   float peer_top[kMaxCluster];
-  u64 peer_floor[kMaxCluster];            // CTA 0
+  float peer_cut[kMaxCluster];            // CTA 0
+  double peer_floor[kMaxCluster];         // CTA 0
   unsigned int peer_ties[kMaxCluster];
   u64 red[kWarps], red2[kWarps];
-  u64 scan[kWarps];
-  u64 found_mass, found_token;
+  double scan[kWarps];
+  u64 scan_units[kWarps];
+  double found_mass;
+  u64 found_token, temp;
   int found;
-  unsigned int list_n, few_n, first;
+  unsigned int mine, others, base, few_n, first;
   // written by CTA 0 into every CTA
   int mode, lo, hi;
   uint32_t prefix;
@@ -184,195 +186,304 @@ struct Shared {
 };
 constexpr size_t kSharedBytes = (sizeof(Shared) + 15) & ~size_t(15);
 static_assert(kSharedBytes + kMaxStage <= 227 * 1024, "shared memory");
-static_assert(sizeof(u64) * 256 + 256 * 4 <= sizeof(u64) * kList, "the radix histogram lies in the list");
+static_assert(kSub == 256, "a digit of the radix descent");
 
-// Calls g(vector index, its 16 bytes) for the whole vectors of elements [off, off
-// + n) of data, a 16-byte boundary, and e(element index) for those at the ends. A
+// Calls g(vector index) for the whole 16-byte vectors of elements [off, off + n) of
+// data, which is a 16-byte boundary, and e(element index) for those at the ends. A
 // thread gets the same ones every time.
-template <typename T, typename G, typename E>
-TSB_HD void for_vectors(const T *data, int off, int n, G g, E e) {
+template <typename T, int UNROLL, typename G, typename E>
+TSB_HD void for_vectors(int off, int n, G g, E e) {
   constexpr int VEC = 16 / sizeof(T);
   const int v0 = (off + VEC - 1) / VEC, v1 = max((off + n) / VEC, v0);
-#pragma unroll 4
+#pragma unroll UNROLL
   for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads) g(v);
-  const int head = min(v0 * VEC, off + n) - off, rest = off + n - max(v1 * VEC, off + head);
-  if ((int)threadIdx.x < head) e(off + (int)threadIdx.x);
-  if ((int)threadIdx.x >= 32 && (int)threadIdx.x - 32 < rest) e(max(v1 * VEC, off + head) + (int)threadIdx.x - 32);
+  const int head = min(v0 * VEC, off + n), rest = max(v1 * VEC, head);
+  const int i = off + (int)threadIdx.x, j = rest + (int)threadIdx.x - 32;
+  if (i < head) e(i);
+  if (j >= rest && j < off + n) e(j);
 }
-// Calls f(token index, logit) for this CTA's logits, the first of which is token lo.
+// Calls f(element index, logit) for this CTA's logits.
 template <typename T, typename F>
-TSB_HD void for_logits(const T *data, int off, int lo, int n, F f) {
+TSB_HD void for_logits(const T *data, int off, int n, F f) {
   constexpr int VEC = 16 / sizeof(T);
-  for_vectors<T>(
-      data, off, n,
+  for_vectors<T, 1>(
+      off, n,
       [&](int v) {
         const uint4 w = *reinterpret_cast<const uint4 *>(data + v * VEC);
         const T *e = reinterpret_cast<const T *>(&w);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f(lo + v * VEC + j - off, to_float(e[j]));
+        for (int j = 0; j < VEC; ++j) f(v * VEC + j, to_float(e[j]));
       },
-      [&](int i) { f(lo + i - off, to_float(data[i])); });
+      [&](int i) { f(i, to_float(data[i])); });
+}
+// Calls f(element index, logit) for this CTA's logits that satisfy test.
+template <typename T, typename P, typename F>
+TSB_HD void for_hits(const T *data, int off, int n, P test, F f) {
+  constexpr int VEC = 16 / sizeof(T), GROUP = 32 / VEC;
+  const int v0 = (off + VEC - 1) / VEC, v1 = max((off + n) / VEC, v0);
+#pragma unroll 1
+  for (int v = v0 + (int)threadIdx.x; v < v1; v += kThreads * GROUP) {
+    uint32_t mask = 0;
+#pragma unroll
+    for (int g = 0; g < GROUP; ++g) {
+      if (v + g * kThreads < v1) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(data + (v + g * kThreads) * VEC);
+        const T *e = reinterpret_cast<const T *>(&w);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) mask |= test(to_float(e[j])) ? 1u << (g * VEC + j) : 0u;
+      }
+    }
+    for (; mask; mask &= mask - 1) {
+      const int b = __ffs(mask) - 1;
+      const int i = (v + (b / VEC) * kThreads) * VEC + b % VEC;
+      f(i, to_float(data[i]));
+    }
+  }
+  for_vectors<T, 1>(
+      off, n, [](int) {}, [&](int i) {
+        const float x = to_float(data[i]);
+        if (test(x)) f(i, x);
+      });
 }
 
-TSB_HD u64 block_sum(u64 v, Shared &s) {
+// Sum and inclusive scans over the block, in a fixed order.
+TSB_HD double block_sum(double v, Shared &s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
-  if (threadIdx.x % 32 == 0) s.red[threadIdx.x / 32] = v;
+  if (threadIdx.x % 32 == 0) s.scan[threadIdx.x / 32] = v;
   __syncthreads();
-  u64 all = 0;
-  for (int w = 0; w < kWarps; ++w) all += s.red[w];
+  double all = 0.0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) all += s.scan[w];
   return all;
 }
-
-// Inclusive scan of a value per thread over the block.
-TSB_HD u64 block_scan(u64 v, Shared &s) {
+template <typename V>
+TSB_HD V block_scan(V v, V *per_warp) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
+    const V up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   __syncthreads();
-  if (lane == 31) s.scan[warp] = v;
+  if (lane == 31) per_warp[warp] = v;
   __syncthreads();
-  u64 before = 0;
-  for (int w = 0; w < warp; ++w) before += s.scan[w];
+  V before = V(0);
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? per_warp[w] : V(0);
   return before + v;
 }
 
-TSB_HD float token_logit(u64 token) { return key_logit((uint32_t)(token >> 32)); }
-TSB_HD int token_index(u64 token) { return (int)~(uint32_t)token; }
-
-// Descending bitonic sort of N = 32 or 64 values over a warp, element lane + 32 h in v[h].
-template <int N>
-TSB_HD void warp_sort(u64 (&v)[N / 32], int lane) {
-#pragma unroll
-  for (int k = 2; k <= N; k <<= 1) {
-#pragma unroll
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      if (j == 32) {
-        const u64 a = v[0], b = v[N / 32 - 1];
-        v[0] = max(a, b);
-        v[N / 32 - 1] = min(a, b);
-      } else {
-#pragma unroll
-        for (int h = 0; h < N / 32; ++h) {
-          const u64 other = __shfl_xor_sync(0xffffffffu, v[h], j);
-          const bool down = ((lane + 32 * h) & k) == 0, low = (lane & j) == 0;
-          v[h] = down == low ? max(v[h], other) : min(v[h], other);
-        }
-      }
-    }
+// Appends a token to this CTA's part of the list.
+TSB_HD void append(Shared &s, u64 token) {
+  const unsigned int at = atomicAdd(&s.mine, 1u);
+  if (at < (unsigned int)kList) s.list[at] = token;
+}
+// Hands the list of every other CTA to CTA 0.
+__device__ __noinline__ void send_list(Shared &s, Shared *head, bool is_head) {
+  __syncthreads();
+  if (is_head) return;
+  const int n = min((int)s.mine, kList);
+  if (threadIdx.x == 0) s.base = atomicAdd(&head->others, s.mine);  // all of them: CTA 0 sees a list too long
+  __syncthreads();
+  for (int e = threadIdx.x; e < n; e += kThreads) {
+    const unsigned int at = s.base + e;
+    if (at < (unsigned int)kList) head->list[kList - 1 - at] = s.list[e];
   }
 }
-TSB_HD u64 warp_scan(u64 v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += up;
+TSB_HD u64 listed(const Shared &s, int e) { return s.list[e < (int)s.mine ? e : kList - 1 - (e - (int)s.mine)]; }
+
+// CTA 0: puts few[0, n) in order: order[i] the i-th token, up_to[i] the units of it
+// and those before it. Two threads per token count the tokens before it.
+__device__ __noinline__ void put_in_order(Shared &s, int n) {
+  const int i = threadIdx.x / 2, half = threadIdx.x % 2;
+  const u64 me = i < n ? s.few[i].x : 0;
+  int rank = 0;
+  u64 units = 0;
+#pragma unroll 4
+  for (int j = half; j < n; j += 2) {
+    const ulonglong2 o = s.few[j];
+    rank += o.x > me;
+    units += o.x >= me ? o.y : 0ull;
   }
-  return v;
+  rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+  units += __shfl_xor_sync(0xffffffffu, units, 1);
+  if (half == 0 && i < n) {
+    s.order[rank] = me;
+    s.up_to[rank] = units;
+  }
+  __syncthreads();
 }
-TSB_HD u64 warp_sum(u64 v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+// The place in that order of the token with which before + running units * unit
+// reaches bound: the last one that starts below it.
+TSB_HD int cross(Shared &s, int n, double before, double unit, double bound) {
+  if (threadIdx.x == 0) s.found = 0;
+  __syncthreads();
+  const int i = threadIdx.x;
+  if (i > 0 && i < n && s.up_to[i] > s.up_to[i - 1] && before + (double)s.up_to[i - 1] * unit < bound) atomicMax(&s.found, i);
+  __syncthreads();
+  return s.found;
 }
 
-// CTA 0: the first token, along the order, at which `before` plus the running
-// count or mass of the listed tokens of `bin` (all of the list for bin < 0, counts
-// only) that are at or above `floor_token` reaches bound; into s.found_token and
-// s.found_mass (the count or mass through it).
-TSB_HD void narrow(Shared &s, int n, int bin, u64 floor_token, bool by_count, u64 bound, u64 before, const RowScale &r) {
+// CTA 0: the first of the n listed tokens of `bin` (of any bin for bin < 0, counts
+// only) at or above floor_token, along the order, with which `before` plus the
+// running count or mass reaches bound; into s.found_token and s.found_mass (what has
+// been reached with it).
+__device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, bool by_count, double bound,
+                                    double before, const RowScale &r) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const double unit = by_count ? 1.0 : bin_unit((uint32_t)bin, s.octave);
   u64 lo = floor_token, hi = ~0ull;
-  auto each = [&](auto f) {
-    for (int e = tid; e < n; e += kThreads) {
-      const u64 t = s.list[e];
-      if (t >= lo && t <= hi && (bin < 0 || logit_bin(token_logit(t), r) == (uint32_t)bin)) f(t);
-    }
+  bool by_t = bin >= 0;  // first by t inside the bin, which is known; then by the tokens' own range
+  // a token's sub-bin by t: the fraction that logit_bin rounds away, of 256 parts
+  const float first = (float)bin - 0.5f;
+  auto sub_of = [&](float x) { return (int)fminf(fmaxf((fmaf(r.top - x, r.scale, -first)) * (float)kSub, 0.f), (float)(kSub - 1)); };
+  int by_t_sub = -1;  // the sub-bin by t that is left
+  auto in = [&](u64 t) {
+    return t >= lo && t <= hi && (bin < 0 || (logit_bin(token_logit(t), r) == (uint32_t)bin &&
+                                              (by_t_sub < 0 || sub_of(token_logit(t)) == by_t_sub)));
   };
+  u64 least = 0, most = 0;
   for (;;) {
-    u64 least = ~0ull, most = 0;
-    unsigned int count = 0;
-    each([&](u64 t) {
-      least = min(least, t);
-      most = max(most, t);
-      ++count;
-    });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      count += __shfl_xor_sync(0xffffffffu, count, o);
-    }
-    __syncthreads();
-    if (lane == 0) { s.red[warp] = least; s.red2[warp] = most; s.scan[warp] = count; }
     s.sub0[tid] = 0;
     s.sub1[tid] = 0;
-    if (tid == 0) { s.found = 0; s.found_mass = before; s.few_n = 0; }
-    __syncthreads();
-    count = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      least = min(least, s.red[w]);
-      most = max(most, s.red2[w]);
-      count += (unsigned int)s.scan[w];
-    }
-    if (count <= 32) break;
-    const int shift = max(0, 64 - __clzll((long long)(most - least)) - 8);
-    each([&](u64 t) {
-      const unsigned int sub = (unsigned int)((most - t) >> shift);
-      if (by_count) {
-        atomicAdd(&s.sub0[sub], 1u);
-      } else {
-        const uint32_t m = logit_m(token_logit(t), (uint32_t)bin, r);
-        atomicAdd(&s.sub0[sub], m & 4095u);
-        atomicAdd(&s.sub1[sub], m >> 12);
+    if (tid == 0) { s.found = 0; s.few_n = 0; }
+    int shift = 0;
+    if (!by_t) {
+      least = ~0ull;
+      most = 0;
+      for (int e = tid; e < n; e += kThreads) {
+        const u64 t = listed(s, e);
+        if (in(t)) {
+          least = min(least, t);
+          most = max(most, t);
+        }
       }
-    });
-    __syncthreads();
-    const u64 own = by_count ? s.sub0[tid] : bin_units((u64)s.sub0[tid] + ((u64)s.sub1[tid] << 12), (uint32_t)bin);
-    const u64 here = before + block_scan(own, s);
-    if (here >= bound && here - own < bound) {
-      s.found = tid;
-      s.found_mass = here - own;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+      }
+      if (lane == 0) { s.red[warp] = least; s.red2[warp] = most; }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        least = min(least, s.red[w]);
+        most = max(most, s.red2[w]);
+      }
+      shift = max(0, 64 - __clzll((long long)(most - least)) - 8);
+    } else {
+      __syncthreads();
     }
+    unsigned int count = 0;
+    for (int e = tid; e < n; e += kThreads) {
+      const u64 t = listed(s, e);
+      if (!in(t)) continue;
+      ++count;
+      const int sub = by_t ? sub_of(token_logit(t)) : (int)((most - t) >> shift);
+      const uint32_t m = by_count ? 1u : logit_m(token_logit(t), (uint32_t)bin, r);
+      atomicAdd(&s.sub0[sub], m & 4095u);
+      if (!by_count) atomicAdd(&s.sub1[sub], m >> 12);
+    }
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) atomicAdd(&s.few_n, count);
+    __syncthreads();
+    if (s.few_n <= (unsigned int)kFewest) break;
+    const u64 own = (u64)s.sub0[tid] + ((u64)s.sub1[tid] << 12);
+    const u64 up = block_scan(own, s.scan_units);
+    // the last sub-bin that starts below the bound holds it
+    if (own && before + (double)(up - own) * unit < bound) atomicMax(&s.found, tid);
+    __syncthreads();
+    if (tid == s.found) s.found_mass = before + (double)(up - own) * unit;
     __syncthreads();
     before = s.found_mass;
-    hi = most - ((u64)s.found << shift);
-    const u64 width = (1ull << shift) - 1;
-    lo = max(lo, hi > width ? hi - width : 0ull);
-  }
-  each([&](u64 t) { s.few[atomicAdd(&s.few_n, 1u)] = t; });
-  __syncthreads();
-  if (warp == 0) {
-    u64 v[1] = {lane < (int)s.few_n ? s.few[lane] : 0ull};
-    warp_sort<32>(v, lane);
-    const u64 own = v[0] == 0 ? 0 : by_count ? 1 : logit_mass(token_logit(v[0]), r);
-    const u64 here = before + warp_scan(own, lane);
-    const unsigned int at = __ballot_sync(0xffffffffu, here >= bound && own);
-    const int first = at ? __ffs(at) - 1 : 0;
-    if (lane == first) {
-      s.found_token = v[0];
-      s.found_mass = here;
+    if (by_t) {
+      by_t_sub = s.found;
+      by_t = false;
+    } else {
+      const u64 width = (1ull << shift) - 1, down = (u64)s.found << shift;
+      hi = most > down ? most - down : 0ull;
+      lo = max(lo, hi > width ? hi - width : 0ull);
     }
+    __syncthreads();
+  }
+  const int have = (int)s.few_n;
+  __syncthreads();
+  if (tid == 0) s.few_n = 0;
+  __syncthreads();
+  for (int e = tid; e < n; e += kThreads) {
+    const u64 t = listed(s, e);
+    if (in(t)) {
+      const u64 m = by_count ? 1 : logit_m(token_logit(t), (uint32_t)bin, r);
+      s.few[atomicAdd(&s.few_n, 1u)] = make_ulonglong2(t, m);
+    }
+  }
+  __syncthreads();
+  put_in_order(s, have);
+  const int at = cross(s, have, before, unit, bound);
+  if (tid == 0) {
+    s.found_token = have ? s.order[at] : 0;
+    s.found_mass = have ? before + (double)s.up_to[at] * unit : before;
   }
   __syncthreads();
 }
 
-// u's bound on the running mass: the first token whose cumulative mass exceeds u * total.
-TSB_HD u64 sample_bound(float u, u64 total) {
-  const double want = u > 0.f ? (double)u * (double)total : 0.0;
-  return want >= (double)total ? total : min((u64)want + 1, total);
+// CTA 0: running sums of the histogram; returns the whole.
+__device__ __noinline__ double run_sums(Shared &s, bool masses) {
+  double v[kBinsPerThread], run = 0.0;
+#pragma unroll
+  for (int i = 0; i < kBinsPerThread; ++i) {
+    const int bin = threadIdx.x * kBinsPerThread + i;
+    v[i] = bin >= kBins ? 0.0 : masses ? (double)((u64)s.h0[bin] + ((u64)s.h1[bin] << 12)) * bin_unit(bin, s.octave) : (double)s.h0[bin];
+    run += v[i];
+  }
+  double up = block_scan(run, s.scan) - run;
+#pragma unroll
+  for (int i = 0; i < kBinsPerThread; ++i) {
+    const int bin = threadIdx.x * kBinsPerThread + i;
+    up += v[i];
+    if (bin < kBins) s.sums[bin] = up;
+  }
+  __syncthreads();
+  return s.sums[kBins - 1];
 }
-TSB_HD u64 top_p_bound(double p, u64 total) {
-  const u64 b = p > 0.0 ? (u64)ceil(p * (double)total) : 1ull;
-  return min(max(b, 1ull), total);
+TSB_HD double before_bin(const Shared &s, int bin) { return bin ? s.sums[bin - 1] : 0.0; }
+// CTA 0: the bin in which the running sum reaches bound (the last that adds to it, if none does).
+__device__ __noinline__ int find_bin(Shared &s, double bound) {
+  if (threadIdx.x == 0) s.found = 0;
+  __syncthreads();
+  bound = fmin(bound, s.sums[kBins - 1]);
+#pragma unroll
+  for (int bin = threadIdx.x; bin < kBins; bin += kThreads) {
+    const double here = s.sums[bin], before = before_bin(s, bin);
+    if (here > before && here >= bound && before < bound) atomicMax(&s.found, bin);
+  }
+  __syncthreads();
+  const int bin = s.found;
+  __syncthreads();
+  return bin;
+}
+
+// u's bound on the running mass, which the sample's cumulative mass exceeds: the
+// next number above u * total. Past the last token it is the total.
+TSB_HD double sample_bound(float u, double total) {
+  const double want = u > 0.f ? (double)u * total : 0.0;
+  return fmin(__longlong_as_double(__double_as_longlong(want) + 1), total);
+}
+// Tokens of equal weight w that make up `mass`, at least one.
+TSB_HD double ties_for(double mass, double w) { return fmax(ceil(mass / w), 1.0); }
+// No more tokens than this make up `mass` in a bin (2^-22 * 0.97 is below any m's share of a unit).
+TSB_HD float most_tokens(double mass, int bin) {
+  return (float)mass * exp2f((float)bin * (1.f / kStep)) * 1.03f + 1.f;
 }
 
 TSB_HD void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 TSB_HD void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+TSB_HD void cluster_barrier() {
+  cluster_arrive();
+  cluster_wait();
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_constant__ SampleArgs a) {
@@ -382,36 +493,30 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
-  if (tid == 0) { s.list_n = 0; s.first = 0xffffffffu; }
+  if (tid == 0) { s.mine = 0; s.others = 0; s.first = 0xffffffffu; }
+  for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;  // h0 and h1
+  if (tid < kStep) s.octave[tid] = kOctave[tid];
   cluster_arrive();  // waited for before the first access to another CTA's shared memory
-  griddep_wait();  // programmatic dependent: the logits are the previous kernel's
+  griddep_wait();    // programmatic dependent: the logits are the previous kernel's
   griddep_launch_dependents();
 
-  // ---- this CTA's logits [lo, lo + n), staged or read where they are
+  // ---- this CTA's logits, tokens [lo, lo + n): elements [off, off + n) of data
   const T *x = static_cast<const T *>(a.logits) + (size_t)row * a.row_stride;
   const int lo = min(rank * a.slice, a.vocab), n = min(a.slice, a.vocab - lo);
   const T *data = x + lo;
   const int off = (int)((reinterpret_cast<uintptr_t>(data) & 15) / sizeof(T));
   data -= off;
-  const float u = a.u[row];
-  double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
-  const double p = a.top_p ? a.top_p[row] : a.top_p_s;
-  const double floor_w = a.min_p ? a.min_p[row] : a.min_p_s;
-  int k = a.top_k ? a.top_k[row] : a.top_k_s;
-  const bool greedy = !(temperature > 0.0);
-  temperature = fmax(temperature, kMinTemperature);
-
+  const int index0 = lo - off;  // token of element 0
+  constexpr int VEC = 16 / sizeof(T);
   float top = -INFINITY;  // this thread's largest logit
   {
-    constexpr int VEC = 16 / sizeof(T);
     T *stage = reinterpret_cast<T *>(smem + kSharedBytes);
-    for_vectors<T>(
-        data, off, n,
+    for_vectors<T, 4>(
+        off, n,
         [&](int v) {
           const uint4 w = ldg_nc_v4(data + v * VEC);
           if (a.staged) *reinterpret_cast<uint4 *>(stage + v * VEC) = w;
-          top = max_of(w, top, T());
+          top = fmaxf(top, max_of(w, T()));
         },
         [&](int i) {
           const T w = data[i];
@@ -420,149 +525,171 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         });
     if (a.staged) data = stage;  // a thread reads back what it wrote itself
   }
+  const float u = a.u[row];
+  double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
+  const double p = a.top_p ? a.top_p[row] : a.top_p_s;
+  const double floor_w = a.min_p ? a.min_p[row] : a.min_p_s;
+  const int k = a.top_k ? a.top_k[row] : a.top_k_s;
+  const bool greedy = !(temperature > 0.0), use_p = p < 1.0, use_floor = floor_w > 0.0;
+  bool use_k = k > 0 && k < a.vocab;
+  temperature = fmin(fmax(temperature, kMinTemperature), kMaxTemperature);
+  RowScale r;
+  double per_t;  // 1 / temperature
+  {
+    const float guess = 1.f / (float)temperature;  // one Newton step leaves an error below 2^-44
+    per_t = fma((double)guess, fma(-temperature, (double)guess, 1.0), (double)guess);
+    const double scale = per_t * (1.4426950408889634 * kStep);
+    r.scale = (float)scale;
+    r.low = (float)(scale - (double)r.scale);
+  }
   Shared *const head = cluster.map_shared_rank(&s, 0);
-  auto emit = [&](float v, int token, u64 kept) {
+  auto emit = [&](float v, int token, double kept) {
     if (token >= 0) a.token[row] = token;
     if (a.logprob) {
-      const double d = v == top ? 0.0 : ((double)v - (double)top) / temperature;
-      a.logprob[row] = (float)(d - log((double)kept / (double)kOne));
+      const double d = v == top ? 0.0 : ((double)v - (double)top) * per_t;
+      const float f = (float)kept;  // log(kept) = log(f) + (kept - f) / f
+      a.logprob[row] = (float)(d - ((double)logf(f) + (kept - (double)f) / (double)f));
     }
   };
-  const bool use_p = p < 1.0, use_floor = floor_w > 0.0;
-  const u64 floor_mass = use_floor ? (u64)fmin(ceil(floor_w * (double)kOne), 2.0 * (double)kOne) : 0;
-  const double c64 = 1.4426950408889634 / temperature;
-  RowScale r;
-  r.c = (float)c64;
-  r.c_low = (float)(c64 - (double)r.c);
-  r.bin_scale = (float)(c64 * kStep);
+  auto nothing = [&]() {
+    a.token[row] = -1;
+    if (a.logprob) a.logprob[row] = -INFINITY;
+  };
 
-  // ---- small top-k: tokens that some k lanes' maxima reach
-  if (!greedy && k > 0 && k <= kDirectK && k < a.vocab) {
+  // ---- small top-k: the tokens that some k lanes' maxima reach
+  if (!greedy && use_k && k <= kDirectK) {
     float v = top;  // the warp's lanes in descending order
-#pragma unroll
+#pragma unroll 1
     for (int g = 2; g <= 32; g <<= 1) {
-#pragma unroll
+#pragma unroll 1
       for (int j = g >> 1; j > 0; j >>= 1) {
         const float other = __shfl_xor_sync(0xffffffffu, v, j);
         v = ((lane & g) == 0) == ((lane & j) == 0) ? fmaxf(v, other) : fminf(v, other);
       }
     }
     if (lane == (k - 1) / kWarps) s.red[warp] = __float_as_uint(v);  // ceil(k / warps) lanes of each warp reach it
+    if (lane == 0) s.red2[warp] = __float_as_uint(v);
     __syncthreads();
-    float cut = __uint_as_float((uint32_t)s.red[0]);
-    for (int w = 1; w < kWarps; ++w) cut = fminf(cut, __uint_as_float((uint32_t)s.red[w]));
+    float cut = INFINITY, most = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      cut = fminf(cut, __uint_as_float((uint32_t)s.red[w]));
+      most = fmaxf(most, __uint_as_float((uint32_t)s.red2[w]));
+    }
+    for_hits<T>(
+        data, off, n, [&](float e) { return e >= cut && e > -INFINITY; },
+        [&](int i, float e) { append(s, make_token(e, index0 + i)); });
     cluster_wait();
-    for_logits<T>(data, off, lo, n, [&](int i, float e) {
-      if (e >= cut && e > -INFINITY) {
-        const unsigned int at = atomicAdd(&head->list_n, 1u);
-        if (at < (unsigned int)kList) head->list[at] = (u64)logit_key(e) << 32 | (uint32_t)~i;
-      }
-    });
-    cluster.sync();
-    const int m = (int)head->list_n;
-    cluster_arrive();  // CTA 0 stays until every CTA has read it
-    if (m <= kList) {
+    if (tid == 0) {
+      head->peer_top[rank] = most;
+      head->peer_cut[rank] = cut;
+    }
+    send_list(s, head, rank == 0);
+    cluster_barrier();
+    const unsigned int total = head->mine + head->others;
+    cluster_arrive();  // CTA 0 stays until every CTA has read them
+    if (total <= (unsigned int)kList) {
       if (rank != 0) {
         cluster_wait();
         return;
       }
+      const int m = (int)total;
+      // a histogram of the logits between the lowest cut and the top leaves about k tokens
+      for (int q = 0; q < ctas; ++q) {
+        top = fmaxf(q ? top : -INFINITY, s.peer_top[q]);
+        cut = fminf(cut, s.peer_cut[q]);
+      }
+      r.top = top;
+      const float per_sub = (float)kSub / (top - cut);
+      auto sub_of = [&](u64 t) { return (int)fminf((top - token_logit(t)) * per_sub, (float)(kSub - 1)); };  // NaN: the last
+      s.sub0[tid] = 0;
+      if (tid == 0) { s.found = 0; s.few_n = 0; }
+      __syncthreads();
+      for (int e = tid; e < m; e += kThreads) atomicAdd(&s.sub0[sub_of(listed(s, e))], 1u);
+      __syncthreads();
+      const u64 own = s.sub0[tid], up = block_scan(own, s.scan_units);
+      if (own && up - own < (u64)k) atomicMax(&s.found, tid);
+      __syncthreads();
+      int last = s.found;
+      if (tid == last) s.temp = up;
+      __syncthreads();
       u64 floor_token = 0;
-      if (m > kDirectK) {
-        narrow(s, m, -1, 0, true, (u64)k, 0, r);
+      if (s.temp > (u64)kFewest) {  // many in one part of the histogram: find the k-th itself
+        narrow(s, m, -1, 0, true, (double)k, 0.0, r);
         floor_token = s.found_token;
+        last = kSub;
+        if (tid == 0) s.few_n = 0;
+        __syncthreads();
       }
-      if (tid == 0) s.few_n = 0;
-      __syncthreads();
       for (int e = tid; e < m; e += kThreads) {
-        const u64 t = s.list[e];
-        if (t >= floor_token) s.few[atomicAdd(&s.few_n, 1u)] = t;
+        const u64 t = listed(s, e);
+        if (t < floor_token || sub_of(t) > last) continue;
+        const float v = token_logit(t);
+        const u64 w = v == top ? list_units(1.0) : top == INFINITY ? 0 : list_units(logit_mass(v, r, s.octave));
+        s.few[atomicAdd(&s.few_n, 1u)] = make_ulonglong2(t, w);
       }
       __syncthreads();
-      if (warp == 0) {
-        const int have = (int)s.few_n;
-        u64 t[2], own[2], up[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) t[h] = lane + 32 * h < have ? s.few[lane + 32 * h] : 0ull;
-        warp_sort<kDirectK>(t, lane);
-        const int kept_n = min(have, k);
-        top = token_logit(__shfl_sync(0xffffffffu, t[0], 0));
-        r.top = top;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float e = token_logit(t[h]);
-          own[h] = lane + 32 * h >= kept_n ? 0 : e == top ? kOne : top == INFINITY ? 0 : logit_mass(e, r);
+      const int all = (int)s.few_n;
+      put_in_order(s, all);
+      const int have = min(all, k);
+      if (have == 0) {
+        if (tid == 0) nothing();
+      } else {
+        double kept = (double)s.up_to[have - 1];
+        if (use_p) kept = (double)s.up_to[cross(s, have, 0.0, 1.0, p * kept)];
+        if (use_floor) {  // of those in order the ones up to the last of weight >= min_p, at least the first
+          __syncthreads();
+          if (tid == 0) s.found = 0;
+          __syncthreads();
+          if (tid < have && (double)(s.up_to[tid] - (tid ? s.up_to[tid - 1] : 0ull)) >= floor_w * kListUnit) atomicMax(&s.found, tid);
+          __syncthreads();
+          kept = fmin(kept, (double)s.up_to[s.found]);
         }
-        up[0] = warp_scan(own[0], lane);
-        const u64 first_half = __shfl_sync(0xffffffffu, up[0], 31);
-        up[1] = first_half + warp_scan(own[1], lane);
-        u64 kept = __shfl_sync(0xffffffffu, up[1], 31);
-        // the place of the first token whose running mass reaches a bound
-        auto cross = [&](u64 bound) -> int {
-          const unsigned int a0 = __ballot_sync(0xffffffffu, up[0] >= bound && own[0]);
-          const unsigned int a1 = __ballot_sync(0xffffffffu, up[1] >= bound && own[1]);
-          return a0 ? __ffs(a0) - 1 : a1 ? __ffs(a1) + 31 : 0;
-        };
-        auto at = [&](const u64 (&w)[2], int i) -> u64 {
-          const u64 w0 = __shfl_sync(0xffffffffu, w[0], i & 31), w1 = __shfl_sync(0xffffffffu, w[1], i & 31);
-          return i < 32 ? w0 : w1;
-        };
-        if (kept == 0) {
-          if (lane == 0) {
-            a.token[row] = -1;
-            if (a.logprob) a.logprob[row] = -INFINITY;
-          }
-        } else {
-          if (use_p) kept = min(kept, at(up, cross(top_p_bound(p, kept))));
-          if (use_floor) {
-            const u64 above = warp_sum((own[0] >= floor_mass ? own[0] : 0) + (own[1] >= floor_mass ? own[1] : 0));
-            kept = min(kept, max(above, kOne));
-          }
-          const u64 token = at(t, cross(sample_bound(u, kept)));
-          if (lane == 0) emit(token_logit(token), token_index(token), kept);
-        }
+        __syncthreads();
+        const int at = cross(s, have, 0.0, 1.0, sample_bound(u, kept));
+        if (tid == 0) emit(token_logit(s.order[at]), token_index(s.order[at]), kept / kListUnit);
       }
       cluster_wait();
       return;
     }
     cluster_wait();  // too many (equal logits, or hardly any live ones): the general way
-    if (tid == 0) s.list_n = 0;
+    if (tid == 0) { s.mine = 0; s.others = 0; }
   } else {
     cluster_wait();
   }
 
   // ---- 1. the largest logit
-#pragma unroll
+#pragma unroll 1
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  __syncthreads();
   if (lane == 0) s.red[warp] = __float_as_uint(top);
   __syncthreads();
+#pragma unroll 1
   for (int w = 0; w < kWarps; ++w) top = fmaxf(top, __uint_as_float((uint32_t)s.red[w]));
   if (tid < ctas) cluster.map_shared_rank(&s, tid)->peer_top[rank] = top;
-  cluster.sync();
+  cluster_barrier();
+#pragma unroll 1
   for (int c = 0; c < ctas; ++c) top = fmaxf(top, s.peer_top[c]);
 
   if (top == -INFINITY) {  // every logit is -inf or NaN: there is no token to choose
-    if (rank == 0 && tid == 0) {
-      a.token[row] = -1;
-      if (a.logprob) a.logprob[row] = -INFINITY;
-    }
+    if (rank == 0 && tid == 0) nothing();
     return;
   }
   if (greedy) {
     unsigned int first = 0xffffffffu;
-    for_logits<T>(data, off, lo, n, [&](int i, float v) { if (v == top) first = min(first, (unsigned int)i); });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    for_hits<T>(
+        data, off, n, [&](float v) { return v == top; },
+        [&](int i, float) { first = min(first, (unsigned int)(index0 + i)); });
+    first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0 && first != 0xffffffffu) atomicMin(&head->first, first);
-    cluster.sync();
+    cluster_barrier();
     if (rank == 0 && tid == 0) {
       a.token[row] = (int)s.first;
       if (a.logprob) a.logprob[row] = 0.f;
     }
     return;
   }
-
   r.top = top;
-  bool use_k = k > 0 && k < a.vocab;
   const bool counted = use_k;
 
   auto tell = [&](int mode, int b0, int b1) {  // CTA 0 to all
@@ -573,17 +700,17 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       peer->hi = b1;
     }
   };
-  // All CTAs: the token number `tie` (CTA 0 knows it) of those with this logit, in index order.
-  auto pick = [&](float v, u64 kept, auto tie_of) {
+  // All CTAs: token number `tie` (CTA 0 knows it) of those with this logit, in index order.
+  auto pick = [&](float v, double kept, auto tie_of) {
     unsigned int ties = 0;
-    for_logits<T>(data, off, lo, n, [&](int, float e) { ties += e == v; });
-    ties = (unsigned int)block_sum(ties, s);
+    for_logits<T>(data, off, n, [&](int, float e) { ties += e == v; });
+    ties = (unsigned int)block_sum((double)ties, s);
     if (tid == 0) head->peer_ties[rank] = ties;
-    cluster.sync();
+    cluster_barrier();
     if (rank == 0 && tid == 0) {
       unsigned int all = 0;
       for (int q = 0; q < ctas; ++q) all += s.peer_ties[q];
-      u64 tie = tie_of(all, kept);
+      unsigned int tie = min((unsigned int)tie_of(all, kept), all - 1);
       int q = 0;
       while (q < ctas - 1 && tie >= s.peer_ties[q]) tie -= s.peer_ties[q++];
       for (int c = 0; c < ctas; ++c) {
@@ -593,12 +720,12 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       }
       emit(v, -1, kept);
     }
-    cluster.sync();
+    cluster_barrier();
     if (rank != s.pick_rank) return;
     unsigned int seen = 0;  // ties before this block of tokens
     for (int at = 0; at < n; at += kThreads) {
       const bool hit = at + tid < n && to_float(data[off + at + tid]) == v;
-      const unsigned int up = (unsigned int)block_scan(hit, s);
+      const unsigned int up = (unsigned int)block_scan(hit ? 1.0 : 0.0, s.scan);
       if (hit && seen + up - 1 == (unsigned int)s.pick_tie) a.token[row] = lo + at + tid;
       for (int q = 0; q < kWarps; ++q) seen += (unsigned int)s.scan[q];
       if (seen > (unsigned int)s.pick_tie) return;
@@ -606,11 +733,11 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   };
 
   if (top == INFINITY) {  // the +inf logits share all the weight equally
-    pick(top, 0, [&](unsigned int all, u64 &kept) {
-      kept = (u64)(use_k ? min(all, (unsigned int)k) : all) * kOne;
-      if (use_p) kept = (top_p_bound(p, kept) + kOne - 1) / kOne * kOne;
-      if (use_floor && floor_mass > kOne) kept = kOne;
-      return (sample_bound(u, kept) + kOne - 1) / kOne - 1;
+    pick(top, 0.0, [&](unsigned int all, double &kept) {
+      kept = use_k ? fmin((double)all, (double)k) : (double)all;
+      if (use_p) kept = ties_for(p * kept, 1.0);
+      if (use_floor && floor_w > 1.0) kept = 1.0;
+      return ties_for(sample_bound(u, kept), 1.0) - 1.0;
     });
     return;
   }
@@ -619,6 +746,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   auto push = [&](bool both) {
     __syncthreads();
     if (rank != 0) {
+#pragma unroll 1
       for (int i = tid; i < kBins; i += kThreads) {
         if (s.h0[i]) atomicAdd(&head->h0[i], s.h0[i]);
         if (both && s.h1[i]) atomicAdd(&head->h1[i], s.h1[i]);
@@ -626,267 +754,256 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     }
   };
   auto count_tokens = [&]() {
-    for_logits<T>(data, off, lo, n, [&](int, float v) {
+    for_logits<T>(data, off, n, [&](int, float v) {
       const uint32_t bin = logit_bin(v, r);
       if (bin < (uint32_t)kBins) atomicAdd(&s.h0[bin], 1u);
     });
     push(false);
   };
   auto add_masses = [&]() {
-    u64 above = 0;  // what min-p keeps
-    for_logits<T>(data, off, lo, n, [&](int, float v) {
+    for_logits<T>(data, off, n, [&](int, float v) {
       const uint32_t bin = logit_bin(v, r);
       if (bin < (uint32_t)kBins) {
         const uint32_t m = logit_m(v, bin, r);
         atomicAdd(&s.h0[bin], m & 4095u);
         atomicAdd(&s.h1[bin], m >> 12);
-        if (use_floor) {
-          const u64 units = bin_units(m, bin);
-          if (units >= floor_mass) above += units;
-        }
       }
     });
-    if (use_floor) {
-      above = block_sum(above, s);
-      if (tid == 0) head->peer_floor[rank] = above;
-    }
     push(true);
   };
-  // CTA 0: running sums of the histogram; returns the whole
-  auto run_sums = [&](bool masses) -> u64 {
-    u64 v[kBinsPerThread], run = 0;
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const int bin = tid * kBinsPerThread + i;
-      v[i] = bin >= kBins ? 0 : masses ? bin_units((u64)s.h0[bin] + ((u64)s.h1[bin] << 12), bin) : s.h0[bin];
-      run += v[i];
-    }
-    u64 up = block_scan(run, s) - run;
-#pragma unroll
-    for (int i = 0; i < kBinsPerThread; ++i) {
-      const int bin = tid * kBinsPerThread + i;
-      up += v[i];
-      if (bin < kBins) s.sums[bin] = up;
-    }
-    __syncthreads();
-    return s.sums[kBins - 1];
+  // The mass of the weights that min-p keeps, added up in CTA 0: a prefix of the bins, and part of one.
+  auto add_floor = [&]() {
+    // tokens past this bin weigh less (log2 is good to a small part of a bin)
+    const uint32_t floor_bin = (uint32_t)fminf(fmaxf(-log2f((float)floor_w), 0.f) * kStep + 2.f, (float)(kBins - 1));
+    double above = 0.0;
+    for_hits<T>(
+        data, off, n, [&](float v) { return logit_bin(v, r) <= floor_bin; },
+        [&](int, float v) {
+          const double w = logit_mass(v, r, s.octave);
+          if (w >= floor_w) above += w;
+        });
+    above = block_sum(above, s);
+    if (tid == 0) head->peer_floor[rank] = above;
   };
-  // CTA 0: the bin in which the running sum reaches bound
-  auto find_bin = [&](u64 bound) -> int {
-    if (tid == 0) s.found = kBins - 1;
-    __syncthreads();
-    for (int bin = tid; bin < kBins; bin += kThreads)
-      if (s.sums[bin] >= bound && (bin == 0 || s.sums[bin - 1] < bound)) s.found = bin;
-    __syncthreads();
-    const int bin = s.found;
-    __syncthreads();
-    return bin;
+  auto floor_sum = [&]() {
+    double above = 0.0;
+    for (int q = 0; q < ctas; ++q) above += s.peer_floor[q];
+    return above;
   };
-  auto before_bin = [&](int bin) -> u64 { return bin ? s.sums[bin - 1] : 0; };
   auto gather = [&](int b0, int b1) {  // all CTAs, into CTA 0's list
-    for_logits<T>(data, off, lo, n, [&](int i, float v) {
-      const uint32_t bin = logit_bin(v, r);
-      if (bin >= (uint32_t)b0 && bin <= (uint32_t)b1) {
-        const unsigned int at = atomicAdd(&head->list_n, 1u);
-        if (at < (unsigned int)kList) head->list[at] = (u64)logit_key(v) << 32 | (uint32_t)~i;
-      }
-    });
+    for_hits<T>(
+        data, off, n, [&](float v) { return logit_bin(v, r) - (uint32_t)b0 <= (uint32_t)(b1 - b0); },
+        [&](int i, float v) { append(s, make_token(v, index0 + i)); });
+    send_list(s, head, rank == 0);
   };
 
-  if (use_k) count_tokens(); else add_masses();
-  cluster.sync();
+  if (use_k) {
+    count_tokens();
+  } else {
+    add_masses();
+    if (use_floor && !use_p) add_floor();
+  }
+  cluster_barrier();
 
   // ---- 3. what to gather: CTA 0 decides
-  u64 total = 0, above_floor = 0;
+  double total = 0.0, above_floor = 0.0;
   int k_bin = 0;
-  u64 k_before = 0, k_in = 0;                // tokens before and in top-k's bin
+  double k_before = 0.0, k_in = 0.0;  // tokens before and in top-k's bin
   if (rank == 0) {
-    total = run_sums(!use_k);
+    total = run_sums(s, !use_k);
     if (use_k) {
-      use_k = (u64)k < total;  // else every token with a mass is among the first k
-      k_bin = use_k ? find_bin((u64)k) : kBins - 1;
-      k_before = before_bin(k_bin);
+      use_k = (double)k < total;  // else every token with a mass is among the first k
+      k_bin = use_k ? find_bin(s, (double)k) : kBins - 1;
+      k_before = before_bin(s, k_bin);
       k_in = s.sums[k_bin] - k_before;
-      tell(k_before + k_in <= kList ? kFew : kSlow, 0, k_bin);
+      tell(k_before + k_in <= (double)kList ? kFew : kSlow, 0, k_bin);
     } else {
-      if (use_floor)
-        for (int q = 0; q < ctas; ++q) above_floor += s.peer_floor[q];
       int b0 = 0, b1;
       if (use_p) {
-        b1 = find_bin(top_p_bound(p, total));
+        b1 = find_bin(s, p * total);
       } else {
-        b0 = b1 = find_bin(sample_bound(u, use_floor ? min(total, max(above_floor, kOne)) : total));
-        
+        if (use_floor) above_floor = floor_sum();
+        b0 = b1 = find_bin(s, sample_bound(u, use_floor ? fmin(total, fmax(above_floor, 1.0)) : total));
       }
-      u64 tokens = 0;  // a bound on the tokens of the bins
+      double tokens = 0.0;  // a bound on the tokens of the bins
       for (int bin = b0 + tid; bin <= b1; bin += kThreads) {
-        const u64 mass = s.sums[bin] - before_bin(bin);
-        if (mass) tokens += min(most_tokens(mass, bin), (u64)kMaxVocab);
+        const double mass = s.sums[bin] - before_bin(s, bin);
+        if (mass > 0.0) tokens += (double)most_tokens(mass, bin);
       }
       tokens = block_sum(tokens, s);
-      tell(tokens <= kList ? kFew : kSlow, b0, b1);
+      tell(tokens <= (double)kList ? kFew : kSlow, b0, b1);
     }
   }
-  cluster.sync();
+  cluster_barrier();
   if (s.mode == kFew) {
     gather(s.lo, s.hi);
-    cluster.sync();
+    cluster_barrier();
     if (rank != 0) return;
-    const int m = min((int)s.list_n, kList);
-    u64 floor_token = 0, kept = total;
+    const int m = min((int)(s.mine + s.others), kList);
+    u64 floor_token = 0;
+    double kept = total;
     if (counted) {
       // the list holds the first k, or every token with a mass: their masses by bin
       if (use_k) {
-        narrow(s, m, k_bin, 0, true, (u64)k, k_before, r);
+        narrow(s, m, k_bin, 0, true, (double)k, k_before, r);
         floor_token = s.found_token;
       }
-      for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
+      for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;
       __syncthreads();
       for (int e = tid; e < m; e += kThreads) {
-        if (s.list[e] < floor_token) continue;
-        const float v = token_logit(s.list[e]);
-        const uint32_t bin = logit_bin(v, r), w = logit_m(v, bin, r);
+        const u64 t = listed(s, e);
+        if (t < floor_token) continue;
+        const uint32_t bin = logit_bin(token_logit(t), r), w = logit_m(token_logit(t), bin, r);
         atomicAdd(&s.h0[bin], w & 4095u);
         atomicAdd(&s.h1[bin], w >> 12);
       }
       __syncthreads();
-      kept = run_sums(true);
+      kept = run_sums(s, true);
     }
     if (use_p) {
-      const u64 bound = top_p_bound(p, kept);
-      const int bin = find_bin(bound);
-      narrow(s, m, bin, floor_token, false, bound, before_bin(bin), r);
-      kept = min(kept, s.found_mass);
+      const double bound = p * kept;
+      const int bin = find_bin(s, bound);
+      narrow(s, m, bin, floor_token, false, bound, before_bin(s, bin), r);
+      kept = fmin(kept, s.found_mass);
     }
     if (use_floor) {
       if (counted || use_p) {  // min-p keeps a prefix of the order: what of it is in the list decides
-        u64 above = 0;
+        double above = 0.0;
+#pragma unroll 1
         for (int e = tid; e < m; e += kThreads) {
-          const u64 w = s.list[e] >= floor_token ? logit_mass(token_logit(s.list[e]), r) : 0;
-          above += w >= floor_mass ? w : 0;
+          const u64 t = listed(s, e);
+          const double w = t >= floor_token ? logit_mass(token_logit(t), r, s.octave) : 0.0;
+          above += w >= floor_w ? (double)list_units(w) : 0.0;
         }
-        above_floor = block_sum(above, s);
+        above_floor = block_sum(above, s) / kListUnit;
       }
-      kept = min(kept, max(above_floor, kOne));
+      kept = fmin(kept, fmax(above_floor, 1.0));
     }
-    const u64 bound = sample_bound(u, kept);
-    const int bin = find_bin(bound);
-    narrow(s, m, bin, floor_token, false, bound, before_bin(bin), r);
+    const double bound = sample_bound(u, kept);
+    const int bin = find_bin(s, bound);
+    narrow(s, m, bin, floor_token, false, bound, before_bin(s, bin), r);
     if (tid == 0) emit(token_logit(s.found_token), token_index(s.found_token), kept);
     return;
   }
 
   // ---- many candidates: one bound after the other, each resolved inside its bin
   if (counted) {  // the masses are still to be added up
-    for (int i = tid; i < kBins; i += kThreads) { s.h0[i] = 0; s.h1[i] = 0; }
-    cluster.sync();
+    for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;
+    cluster_barrier();
     add_masses();
-    cluster.sync();
-    if (rank == 0) {
-      total = run_sums(true);
-      if (use_floor)
-        for (int q = 0; q < ctas; ++q) above_floor += s.peer_floor[q];
-    }
   }
-  u64 kept = total;  // CTA 0
+  if (use_floor && (counted || use_p)) add_floor();
+  cluster_barrier();
+  if (rank == 0) {
+    if (counted) total = run_sums(s, true);
+    if (use_floor) above_floor = floor_sum();
+  }
+  double kept = total;  // CTA 0
   for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, u
     if (stage == 0 ? !counted : stage == 1 && !use_p) continue;
-    u64 bound = 0, mass_before = 0, count_before = 0;
+    double bound = 0.0, mass_before = 0.0, count_before = 0.0;
     if (rank == 0) {
-      if (stage == 2 && use_floor) kept = min(kept, max(above_floor, kOne));
+      if (stage == 2 && use_floor) kept = fmin(kept, fmax(above_floor, 1.0));
       int bin;
       if (stage == 0) {
-        bound = (u64)k;
+        bound = (double)k;
         bin = k_bin;
         count_before = k_before;
       } else {
-        bound = stage == 1 ? top_p_bound(p, kept) : sample_bound(u, kept);
-        bin = find_bin(bound);
+        bound = stage == 1 ? p * kept : sample_bound(u, kept);
+        bin = find_bin(s, bound);
       }
-      mass_before = before_bin(bin);
-      const u64 mass = s.sums[bin] - mass_before;
-      int mode = (stage == 0 ? k_in : most_tokens(mass, bin)) <= kList ? kOneBin : kRadix;
-      if (stage == 0 && !use_k) mode = kNoMass;  // every token with a mass is kept
-      if (tid == 0) s.list_n = 0;
+      mass_before = before_bin(s, bin);
+      const double tokens = stage == 0 ? k_in : (double)most_tokens(s.sums[bin] - mass_before, bin);
+      // nothing to resolve where every token with a mass is kept
+      const int mode = stage == 0 && !use_k ? kNoMass : tokens <= (double)kList ? kOneBin : kRadix;
+      if (tid == 0) s.others = 0;
       tell(mode, bin, bin);
     }
-    cluster.sync();
+    if (tid == 0) s.mine = 0;
+    cluster_barrier();
     const int mode = s.mode, bin = s.lo;
     if (mode == kNoMass) {
-      cluster.sync();  // the plan has been read: CTA 0 may write the next one
+      cluster_barrier();  // the plan has been read: CTA 0 may write the next one
       continue;
     }
     if (mode == kOneBin) {
       gather(bin, bin);
-      cluster.sync();
+      cluster_barrier();
       if (rank != 0) continue;
-      narrow(s, min((int)s.list_n, kList), bin, 0, stage == 0, bound, stage == 0 ? count_before : mass_before, r);
+      const int m = min((int)(s.mine + s.others), kList);
+      narrow(s, m, bin, 0, stage == 0, bound, stage == 0 ? count_before : mass_before, r);
       const u64 token = s.found_token;
       if (stage == 2) {
         if (tid == 0) emit(token_logit(token), token_index(token), kept);
       } else if (stage == 1) {
-        kept = min(kept, s.found_mass);
+        kept = fmin(kept, s.found_mass);
       } else {  // the mass of the first k
-        u64 mass = 0;
-        for (int e = tid; e < min((int)s.list_n, kList); e += kThreads)
-          if (s.list[e] >= token) mass += logit_mass(token_logit(s.list[e]), r);
-        kept = mass_before + block_sum(mass, s);
+        double mass = 0.0;
+        for (int e = tid; e < m; e += kThreads) {
+          const u64 t = listed(s, e);
+          if (t >= token) mass += (double)list_units(logit_mass(token_logit(t), r, s.octave));
+        }
+        kept = mass_before + block_sum(mass, s) / kListUnit;
       }
       __syncthreads();
       continue;
     }
-    // radix descent over the keys of the bin, eight bits at a time; its histogram
-    // of masses and counts takes the place of the list
-    u64 *const rmass = s.list;
-    unsigned int *const rcount = reinterpret_cast<unsigned int *>(s.list + 256);
+    // radix descent over the keys of the bin, eight bits at a time: counts in the
+    // narrowing histogram's first half, m in two words of the list
+    unsigned int *const low = reinterpret_cast<unsigned int *>(s.list), *const high = low + kSub;
+    const double unit = bin_unit((uint32_t)bin, s.octave);
     uint32_t prefix = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) { rmass[i] = 0; rcount[i] = 0; }
+      s.sub0[tid] = 0;
+      low[tid] = 0;
+      high[tid] = 0;
       __syncthreads();
-      for_logits<T>(data, off, lo, n, [&](int, float v) {
+      for_logits<T>(data, off, n, [&](int, float v) {
         if (logit_bin(v, r) != (uint32_t)bin) return;
-        const uint32_t key = logit_key(v);
+        const uint32_t key = (uint32_t)(make_token(v, 0) >> 32);
         if (shift < 24 && (key >> (shift + 8)) != prefix) return;
-        atomicAdd(&rcount[(key >> shift) & 255u], 1u);
-        atomicAdd(&rmass[(key >> shift) & 255u], logit_mass(v, r));
+        const uint32_t digit = (key >> shift) & 255u, m = logit_m(v, (uint32_t)bin, r);
+        atomicAdd(&s.sub0[digit], 1u);
+        atomicAdd(&low[digit], m & 4095u);
+        atomicAdd(&high[digit], m >> 12);
       });
-      cluster.sync();
+      cluster_barrier();
       if (rank == 0) {
         u64 m = 0, c = 0;
         const int digit = 255 - tid;  // descending
-        if (tid < 256) {
-          for (int q = 0; q < ctas; ++q) {
-            const Shared *peer = cluster.map_shared_rank(&s, q);
-            m += peer->list[digit];
-            c += reinterpret_cast<const unsigned int *>(peer->list + 256)[digit];
-          }
+        for (int q = 0; q < ctas; ++q) {
+          const Shared *peer = cluster.map_shared_rank(&s, q);
+          const unsigned int *words = reinterpret_cast<const unsigned int *>(peer->list);
+          c += peer->sub0[digit];
+          m += (u64)words[digit] + ((u64)words[kSub + digit] << 12);
         }
+        const double own_m = (double)m * unit, own_c = (double)c;
         if (tid == 0) s.found = 0;
-        const u64 up_m = mass_before + block_scan(m, s);
-        const u64 up_c = count_before + block_scan(c, s);
-        const u64 here = stage == 0 ? up_c : up_m, own = stage == 0 ? c : m;
-        if (tid < 256 && here >= bound && here - own < bound) {
-          s.found = tid;
-          s.found_mass = up_m - m;
-          s.red[0] = up_c - c;
-        }
+        const double up_m = mass_before + block_scan(own_m, s.scan);
+        const double up_c = count_before + block_scan(own_c, s.scan);
+        const double here = stage == 0 ? up_c : up_m, own = stage == 0 ? own_c : own_m;
+        // the last digit with a token that starts below the bound holds it
+        if (c && here - own < bound) atomicMax(&s.found, tid);
+        __syncthreads();
+        if (tid == s.found) { s.found_mass = up_m - own_m; s.temp = (u64)(up_c - own_c); }
         __syncthreads();
         mass_before = s.found_mass;
-        count_before = s.red[0];
+        count_before = (double)s.temp;
         if (tid < ctas) cluster.map_shared_rank(&s, tid)->prefix = prefix << 8 | (uint32_t)(255 - s.found);
       }
-      cluster.sync();
+      cluster_barrier();
       prefix = s.prefix;
     }
     // every token left has the same logit: some of them come before the one wanted
     const float v = key_logit(prefix);
-    const u64 w = logit_mass(v, r);
-    const u64 tie = stage == 0 ? bound - count_before - 1 : (bound - mass_before + w - 1) / max(w, 1ull) - 1;
+    const double w = logit_mass(v, r, s.octave);
+    const double ties = stage == 0 ? bound - count_before : ties_for(bound - mass_before, w);
     if (stage < 2) {
-      kept = min(kept, mass_before + (tie + 1) * w);
+      kept = fmin(kept, mass_before + ties * w);
       continue;
     }
-    pick(v, kept, [&](unsigned int, u64) { return tie; });
+    pick(v, kept, [&](unsigned int, double) { return ties - 1.0; });
     return;
   }
 }
