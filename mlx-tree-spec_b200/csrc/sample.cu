@@ -57,6 +57,7 @@ constexpr int kStep = 32;              // bins per octave of the weight
 constexpr int kBins = 43 * kStep;      // a token of no bin has a mass of zero
 constexpr int kBinsPerThread = (kBins + kThreads - 1) / kThreads;
 constexpr int kList = 2048;            // tokens CTA 0 can hold
+constexpr int kPart = kList / kMaxCluster;  // of them from each CTA, with small top-k: one per thread
 constexpr int kDirectK = 64;           // top-k up to here is looked for among the lanes' maxima
 constexpr int kSub = kThreads;         // bins of a narrowing histogram, one per thread
 constexpr int kFewest = 128;           // tokens put in order by counting, two threads each
@@ -180,13 +181,14 @@ struct Shared {
   int found;
   unsigned int mine, others, base, few_n, first;
   // written by CTA 0 into every CTA
-  int mode, lo, hi;
+  int overflow, mode, lo, hi;
   uint32_t prefix;
   int pick_rank, pick_tie;
 };
 constexpr size_t kSharedBytes = (sizeof(Shared) + 15) & ~size_t(15);
 static_assert(kSharedBytes + kMaxStage <= 227 * 1024, "shared memory");
 static_assert(kSub == 256, "a digit of the radix descent");
+static_assert(kPart <= kThreads, "a thread moves one token of each part");
 
 // Calls g(vector index) for the whole 16-byte vectors of elements [off, off + n) of
 // data, which is a 16-byte boundary, and e(element index) for those at the ends. A
@@ -345,10 +347,11 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
                                               (by_t_sub < 0 || sub_of(token_logit(t)) == by_t_sub)));
   };
   u64 least = 0, most = 0;
-  for (;;) {
+  bool few = n <= kFewest;
+  while (!few) {
     s.sub0[tid] = 0;
     s.sub1[tid] = 0;
-    if (tid == 0) { s.found = 0; s.few_n = 0; }
+    if (tid == 0) s.found = 0;
     int shift = 0;
     if (!by_t) {
       least = ~0ull;
@@ -376,28 +379,27 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
     } else {
       __syncthreads();
     }
-    unsigned int count = 0;
     for (int e = tid; e < n; e += kThreads) {
       const u64 t = listed(s, e);
       if (!in(t)) continue;
-      ++count;
       const int sub = by_t ? sub_of(token_logit(t)) : (int)((most - t) >> shift);
       const uint32_t m = by_count ? 1u : logit_m(token_logit(t), (uint32_t)bin, r);
       atomicAdd(&s.sub0[sub], m & 4095u);
       if (!by_count) atomicAdd(&s.sub1[sub], m >> 12);
     }
-    count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0) atomicAdd(&s.few_n, count);
     __syncthreads();
-    if (s.few_n <= (unsigned int)kFewest) break;
     const u64 own = (u64)s.sub0[tid] + ((u64)s.sub1[tid] << 12);
     const u64 up = block_scan(own, s.scan_units);
     // the last sub-bin that starts below the bound holds it
     if (own && before + (double)(up - own) * unit < bound) atomicMax(&s.found, tid);
     __syncthreads();
-    if (tid == s.found) s.found_mass = before + (double)(up - own) * unit;
+    if (tid == s.found) {
+      s.found_mass = before + (double)(up - own) * unit;
+      s.temp = by_count ? own : own / (kUnitM - (kUnitM >> 6)) + 1;  // no more tokens than this: m > 2^22 * 63 / 64
+    }
     __syncthreads();
     before = s.found_mass;
+    few = s.temp <= (u64)kFewest || (!by_t && shift == 0);
     if (by_t) {
       by_t_sub = s.found;
       by_t = false;
@@ -408,8 +410,6 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
     }
     __syncthreads();
   }
-  const int have = (int)s.few_n;
-  __syncthreads();
   if (tid == 0) s.few_n = 0;
   __syncthreads();
   for (int e = tid; e < n; e += kThreads) {
@@ -420,6 +420,7 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
     }
   }
   __syncthreads();
+  const int have = (int)s.few_n;
   put_in_order(s, have);
   const int at = cross(s, have, before, unit, bound);
   if (tid == 0) {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int row = (int)blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  if (tid == 0) { s.mine = 0; s.others = 0; s.first = 0xffffffffu; }
+  if (tid == 0) { s.mine = 0; s.others = 0; s.first = 0xffffffffu; s.overflow = 0; }
   for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;  // h0 and h1
   if (tid < kStep) s.octave[tid] = kOctave[tid];
   cluster_arrive();  // waited for before the first access to another CTA's shared memory
@@ -508,6 +509,10 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
   data -= off;
   const int index0 = lo - off;  // token of element 0
   constexpr int VEC = 16 / sizeof(T);
+  const float u = a.u[row];
+  const float temperature_row = a.temperature ? a.temperature[row] : 0.f;
+  const float p_row = a.top_p ? a.top_p[row] : 0.f, floor_row = a.min_p ? a.min_p[row] : 0.f;
+  const int k = a.top_k ? a.top_k[row] : a.top_k_s;
   float top = -INFINITY;  // this thread's largest logit
   {
     T *stage = reinterpret_cast<T *>(smem + kSharedBytes);
@@ -525,11 +530,9 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         });
     if (a.staged) data = stage;  // a thread reads back what it wrote itself
   }
-  const float u = a.u[row];
-  double temperature = a.temperature ? a.temperature[row] : a.temperature_s;
-  const double p = a.top_p ? a.top_p[row] : a.top_p_s;
-  const double floor_w = a.min_p ? a.min_p[row] : a.min_p_s;
-  const int k = a.top_k ? a.top_k[row] : a.top_k_s;
+  double temperature = a.temperature ? (double)temperature_row : a.temperature_s;
+  const double p = a.top_p ? (double)p_row : a.top_p_s;
+  const double floor_w = a.min_p ? (double)floor_row : a.min_p_s;
   const bool greedy = !(temperature > 0.0), use_p = p < 1.0, use_floor = floor_w > 0.0;
   bool use_k = k > 0 && k < a.vocab;
   temperature = fmin(fmax(temperature, kMinTemperature), kMaxTemperature);
@@ -548,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
     if (a.logprob) {
       const double d = v == top ? 0.0 : ((double)v - (double)top) * per_t;
       const float f = (float)kept;  // log(kept) = log(f) + (kept - f) / f
-      a.logprob[row] = (float)(d - ((double)logf(f) + (kept - (double)f) / (double)f));
+      a.logprob[row] = (float)(d - ((double)logf(f) + (double)((float)(kept - (double)f) / f)));
     }
   };
   auto nothing = [&]() {
@@ -558,17 +561,15 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
 
   // ---- small top-k: the tokens that some k lanes' maxima reach
   if (!greedy && use_k && k <= kDirectK) {
-    float v = top;  // the warp's lanes in descending order
-#pragma unroll 1
-    for (int g = 2; g <= 32; g <<= 1) {
-#pragma unroll 1
-      for (int j = g >> 1; j > 0; j >>= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, v, j);
-        v = ((lane & g) == 0) == ((lane & j) == 0) ? fmaxf(v, other) : fminf(v, other);
-      }
+    int before = 0;  // lanes of the warp with a larger maximum
+#pragma unroll
+    for (int o = 1; o < 32; ++o) {
+      const int from = (lane + o) % 32;
+      const float other = __shfl_sync(0xffffffffu, top, from);
+      before += other > top || (other == top && from < lane);
     }
-    if (lane == (k - 1) / kWarps) s.red[warp] = __float_as_uint(v);  // ceil(k / warps) lanes of each warp reach it
-    if (lane == 0) s.red2[warp] = __float_as_uint(v);
+    if (before == (k - 1) / kWarps) s.red[warp] = __float_as_uint(top);  // ceil(k / warps) lanes of each warp reach it
+    if (before == 0) s.red2[warp] = __float_as_uint(top);
     __syncthreads();
     float cut = INFINITY, most = -INFINITY;
 #pragma unroll
@@ -576,24 +577,40 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
       cut = fminf(cut, __uint_as_float((uint32_t)s.red[w]));
       most = fmaxf(most, __uint_as_float((uint32_t)s.red2[w]));
     }
+    cluster_wait();
+    // each CTA has a part of CTA 0's list
     for_hits<T>(
         data, off, n, [&](float e) { return e >= cut && e > -INFINITY; },
-        [&](int i, float e) { append(s, make_token(e, index0 + i)); });
-    cluster_wait();
+        [&](int i, float e) {
+          const unsigned int at = atomicAdd(&s.mine, 1u);
+          if (at < (unsigned int)kPart) head->list[rank * kPart + at] = make_token(e, index0 + i);
+        });
+    __syncthreads();
     if (tid == 0) {
       head->peer_top[rank] = most;
       head->peer_cut[rank] = cut;
+      head->peer_ties[rank] = s.mine;
     }
-    send_list(s, head, rank == 0);
+    // too many (equal logits, or hardly any live ones): all CTAs take the general way
+    if (s.mine > (unsigned int)kPart && tid < ctas) cluster.map_shared_rank(&s, tid)->overflow = 1;
     cluster_barrier();
-    const unsigned int total = head->mine + head->others;
-    cluster_arrive();  // CTA 0 stays until every CTA has read them
-    if (total <= (unsigned int)kList) {
-      if (rank != 0) {
-        cluster_wait();
-        return;
+    if (!s.overflow) {
+      if (rank != 0) return;
+      // bring the parts together
+      u64 mine[kMaxCluster];
+      int at[kMaxCluster], m = 0;
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q) {
+        const int part = q < ctas ? (int)s.peer_ties[q] : 0;
+        at[q] = tid < part ? m + tid : -1;
+        mine[q] = tid < part ? s.list[q * kPart + tid] : 0ull;
+        m += part;
       }
-      const int m = (int)total;
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kMaxCluster; ++q)
+        if (at[q] >= 0) s.list[at[q]] = mine[q];
+      if (tid == 0) s.mine = (unsigned int)m;
       // a histogram of the logits between the lowest cut and the top leaves about k tokens
       for (int q = 0; q < ctas; ++q) {
         top = fmaxf(q ? top : -INFINITY, s.peer_top[q]);
@@ -649,11 +666,10 @@ __global__ void __launch_bounds__(kThreads, 3) sample_kernel(const __grid_consta
         const int at = cross(s, have, 0.0, 1.0, sample_bound(u, kept));
         if (tid == 0) emit(token_logit(s.order[at]), token_index(s.order[at]), kept / kListUnit);
       }
-      cluster_wait();
       return;
     }
-    cluster_wait();  // too many (equal logits, or hardly any live ones): the general way
-    if (tid == 0) { s.mine = 0; s.others = 0; }
+    cluster_barrier();  // `overflow` has been read: the CTAs go on together
+    if (tid == 0) s.mine = 0;
   } else {
     cluster_wait();
   }
