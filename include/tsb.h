@@ -257,12 +257,13 @@ typedef struct {
  *            A node that sees nothing gets zeros and -inf.
  * Either cache may have no rows (its planes are then not read). Planes 16-byte
  * aligned, MLX scales and biases 8, row scales 4. Requirements: D == 256,
- * Hq % Hkv == 0, 1 <= T <= 64, tail <= 64, scale > 0, B*Hq*T <= 2^24. No host
+ * Hq % Hkv == 0, 1 <= T <= 64, tail <= 64, scale > 0, B*Hq*T <= 2^22. No host
  * read of the lengths: the call can be captured in a graph and replayed with
  * others. `own->rows` bounds the lengths and sizes the launch. Workspace:
  * tsb_tree_attn_shared_workspace_bytes(), 16-byte aligned, for this call alone
  * until it completes. */
-size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows);
+size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows,
+                                            int kv_format);
 int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride_h, long long q_stride_t,
                          int kv_format, const tsb_kv_t *prefix, const tsb_kv_t *own, const int32_t *lengths,
                          const int32_t *parents, const uint64_t *bits, int B, int T, int Hq, int Hkv, int D, int tail,

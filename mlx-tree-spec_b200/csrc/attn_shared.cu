@@ -1,22 +1,50 @@
 // Tree attention for a batch that shares a long prefix. Each node attends to
-// the P rows of one prefix cache, which every request sees, and to its own
+// the rows of one prefix cache, which every request sees, and to its own
 // request's rows: out = softmax(scale q k) v over both, with the tree rule of
 // tsb_tree_attn on the last `tail` own rows.
 //
 // The prefix is computed once for all: a KV head's query rows of the WHOLE
 // batch (row = (request, head of the group, node)) are packed into blocks of
-// 128, so each block of rows reads the prefix once instead of once per request.
-// A work unit is (KV head, row block) over the prefix or (request, KV head, row
-// block) over that request's own rows, and a CTA takes one key split of a unit.
-// Every split leaves normalised partials with (max, sum), and a combine kernel
-// merges a row's prefix and own partials.
+// 256, so each block of rows reads the prefix once instead of once per request.
+// A unit is (KV head, row block) over the prefix or (request, KV head, row
+// block) over that request's own rows; it is cut along the keys into segments.
+// A pair of CTAs on two SMs works off a list of segments: prefix segments of
+// equal length, laid out so that neighbouring pairs read the same keys at the
+// same time (the row blocks of a head share them through L2), then as many chunks
+// of own rows as even the pairs out. Own lengths are read on the device, so the
+// list is made there too. A segment leaves normalised partials with (max, sum);
+// a combine kernel merges those of each row.
 //
-// The roles and the TMEM plan inside a CTA are those of attn_tc.cu: TMA or
-// converter warps fill K and V tiles of 64 keys, warp 1 issues S = Q K^T (Q in
-// TMEM) and O += P V (P in TMEM), four softmax warps own a query row per
-// thread. Unlike there, Q is gathered row by row from q's strides (a packed
-// block spans requests), and 8-byte cp.async copies bring MLX scales and biases,
-// so a cache of any capacity works. Own lengths are read on the device.
+// With many packed rows the work is bound by the tensor cores: 64 keys x 128 rows
+// are ~1024 cycles of MMA per SM. One SM by itself cannot feed them: a tile's 64 KB of
+// K and V, written to shared memory once and read once at 128 B per cycle, take those
+// 1024 cycles too (measured ~1400-1800 per tile that way, with the softmax's P on
+// top). So two CTAs share each tile (cta_group::2, M = 256): each loads half of it,
+// 32 of the keys and 128 of the value columns, and the MMAs read both halves.
+//   warp 0       TMA of this CTA's half of K tiles of 64 keys (int8 rows: their scales, too)
+//   warp 1       (CTA 0) S_g = Q K_g^T  (M=256, N=64, K=256; Q in TMEM)
+//   warp 2       (CTA 0) O += P_g V_g   (M=256, N=256, K=64; P in shared memory)
+//                An MMA with N=64 takes one thread longer to issue than the tensor
+//                cores to run, so S and P V have an issuer each.
+//   warp 3       TMA of this CTA's half of V tiles
+//   warps 4-11   softmax of this CTA's 128 rows, a thread per row (= TMEM lane): warps
+//                4-7 have the even tiles, 8-11 the odd ones, so that the exponentials
+//                of one tile overlap the loads and stores of the other. The running
+//                maximum is a reference that both use; it moves only when a score
+//                exceeds it by 2^8. A token passes between the two warps of a row block
+//                from tile to tile: its holder looks at the reference and may move it.
+// TMEM (512 columns): O [0, 256), Q [256, 384), S0 [384, 448), S1 [448, 512). P_g goes to
+// shared memory (two buffers), so S_{g+2} waits only until S_g has been read.
+// g counts a pair's tiles over all its segments.
+//
+// 8-bit caches are converted to bf16 in the workspace first, by a kernel at memory
+// speed: each row block would convert every tile again in here, which held a tile to
+// 2.1 us where bf16 takes 1 (32K rows, 160 requests' rows per head: 264 us in all).
+// MLX: the values. int8 rows: the codes, exact in bf16, with the row scales applied in
+// float32 to scores and weights.
+//
+// Rows at or past a cache's valid rows never reach the output, whatever they hold
+// (even NaN): their scores are masked and their V rows are zero in shared memory.
 #include <algorithm>
 
 #include "attn_tile.cuh"
@@ -25,42 +53,42 @@ namespace tsb {
 
 namespace {
 
-constexpr int SH_KT = 64;                  // keys per tile
+constexpr int SH_KT = 64;                    // keys per tile
 constexpr int SH_D = 256;
-constexpr int SH_KVBOX = SH_KT * 128;      // one 64-wide D box of 64 keys (bytes)
-constexpr int SH_KV_BYTES = 4 * SH_KVBOX;  // 32 KB per bf16 K or V tile
+constexpr int SH_ROWS = 256;                 // query rows of a pair, 128 per CTA
+constexpr int SH_KBOX = SH_KT / 2 * 128;     // 64-wide D box of 32 keys (bytes)
+constexpr int SH_VBOX = SH_KT * 128;         // 64-wide D box of 64 keys
+constexpr int SH_K_BYTES = 4 * SH_KBOX;      // a CTA's half of a K tile: 32 keys
+constexpr int SH_V_BYTES = 2 * SH_VBOX;      // a CTA's half of a V tile: 128 columns
+constexpr int SH_P_BYTES = 128 * 128;        // P of a tile: 128 rows of 64 bf16
 constexpr uint32_t SH_O = 0, SH_Q = 256, SH_S0 = 384;
 constexpr float SH_RESCALE_LOG2 = 8.f;
-constexpr int SH_RAW_CODES = SH_KT * SH_D;  // 16 KB: one tile of 8-bit codes
-constexpr int SH_NSC = 8;                   // row-scale ring of the reference format (tiles)
-constexpr int SH_NCONV = 8;                 // converter warps (8-bit formats)
-constexpr int SH_MAX_SPLITS = 64;           // key splits of a unit
+constexpr int SH_NK = 5, SH_NV = 5;          // tiles in flight
+constexpr int SH_NSC = 8;                    // row-scale ring (tiles)
+constexpr int SH_SOFT0 = 4, SH_NSOFT = 8;    // softmax warps
+constexpr int SH_MAX_SPLITS = 64;            // key splits of a prefix unit
+constexpr int SH_MAX_CHUNKS = 16;            // chunks of a request's own rows
+constexpr int SH_MIN_CHUNK = 4;              // tiles
+constexpr int SH_SEG_COST = 3;               // what a segment costs beside its tiles, in tiles
 
-template <int FMT>
+template <bool SCALED>
 struct ShCfg {
-  static constexpr bool Q8 = FMT != TSB_KV_BF16;
-  static constexpr bool MLX = FMT == TSB_KV_MLX_Q8_G64;
-  static constexpr bool REF = FMT == TSB_KV_REF_Q8_ROW;
-  static constexpr int NK = Q8 ? 2 : 3;  // bf16 K tiles in flight
-  static constexpr int NV = Q8 ? 2 : 3;  // bf16 V tiles in flight
-  static constexpr int NR = Q8 ? 5 : 0;  // raw 8-bit tiles in flight
-  // raw stage: codes [64][256] u8, then (MLX) scales [64][4] and biases [64][4] bf16
-  static constexpr int RAW_STAGE = MLX ? SH_RAW_CODES + 2 * SH_KT * 8 : SH_RAW_CODES;
-  static constexpr int SC_BYTES = REF ? SH_NSC * 2 * SH_KT * 4 : 0;
-  static constexpr int NBARS = 1 + 2 * NK + 2 * NV + 8 + 2 * NR + (REF ? SH_NSC : 0);
-  static constexpr int CTRL = 2048;  // barriers, TMEM address, masks, parents
-  static constexpr int THREADS = Q8 ? (6 + SH_NCONV) * 32 : 224;
-  static constexpr size_t SMEM = (size_t)(NK + NV) * SH_KV_BYTES + (size_t)NR * RAW_STAGE + SC_BYTES + CTRL + 1024;
-  static_assert((NBARS + 1) * 8 + 64 * 8 + 64 * 4 <= CTRL, "control block");
+  static constexpr int SC_BYTES = SCALED ? SH_NSC * 2 * SH_KT * 4 : 0;
+  static constexpr int NBARS = 2 * SH_NK + 2 * SH_NV + 11 + (SCALED ? 2 * SH_NSC : 0);
+  static constexpr int CTRL = 6144;  // barriers, TMEM address, schedule, masks of each warp pair, row exchange
+  static constexpr int THREADS = 384;
+  static constexpr size_t SMEM =
+      (size_t)SH_NK * SH_K_BYTES + (size_t)SH_NV * SH_V_BYTES + 2 * SH_P_BYTES + SC_BYTES + CTRL + 1024;
+  static_assert((NBARS + 20) * 8 + 4 * 64 * (8 + 4) + 3 * 128 * 4 <= CTRL, "control block");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// One cache as the kernel reads it.
+// One cache of bf16 rows as the kernel reads it (through tensor maps).
 struct ShSource {
-  const unsigned char *kc, *vc;   // 8-bit codes, D bytes per row
-  const void *ks, *kb, *vs, *vb;  // MLX: bf16 [rows][4]; reference: float [rows] (ks, vs)
-  int cap;                        // rows per (request, head)
-  int rows;                       // valid rows: the prefix's, or the most any request has
+  const float *ks, *vs;  // row scales (int8 rows), in the cache's own layout
+  int sc_cap;            // its rows per (request, head)
+  int cap;               // rows per (request, head) of what the tensor maps cover
+  int rows;              // valid rows: the prefix's, or the most any request has
 };
 
 struct ShArgs {
@@ -71,443 +99,587 @@ struct ShArgs {
   const unsigned long long *bits;
   const int32_t *lengths;
   int B, T, Hq, Hkv, tail;
-  int rb_p, rb_o;          // row blocks of a prefix unit set / of a request's unit set
-  int splits_p, splits_o;  // key splits
-  int tps_p, tps_o;        // tiles per split
-  int ctas_p;              // CTAs of prefix units; the others are own units
+  int rb_p, rb_o;   // row blocks of a KV head's prefix rows / of a request's rows
+  int splits, tps;  // prefix: key splits, tiles per split
+  int items;        // prefix segments: Hkv * splits * rb_p
+  int chunk;        // own: tiles per chunk
+  int chunks;       // the most chunks a request has
   float scale_log2;
-  float *part_o;   // [splits_p + splits_o][B*Hq*T][D]
-  float *part_ml;  // [splits_p + splits_o][B*Hq*T][2]
+  float *part_o;   // [splits + chunks][B*Hq*T][D]
+  float *part_ml;  // [splits + chunks][B*Hq*T][2]
 };
 
-TSB_HD void cp_async8(void *dst, const void *src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
+TSB_HD int own_rows_of(const int32_t *lengths, int b, int most) {
+  return lengths ? min(max(lengths[b], 0), most) : most;
+}
+TSB_HD int ceil_to(int a, int b) { return (a + b - 1) / b; }
+
+// A pair's share of the own chunks: `left` chunks from (b, u, ch) on.
+struct ShShare {
+  int b, u, ch, left;
+};
+
+struct ShSegment {
+  bool own;
+  int b, kh, rb;       // unit
+  int j0, nt;          // tiles
+  int slot, slots;     // the partial it writes, and further slots it covers (marked empty)
+  int n_kv, tail_lo;   // keys, and where the tree rule begins
+};
+
+// Walks a pair's segments; every role does so by itself.
+struct ShWalk {
+  const ShArgs &a;
+  int item, step, len;
+  ShShare w;
+  TSB_HD ShWalk(const ShArgs &args, const ShShare &share, int pair, int pairs)
+      : a(args), item(pair), step(pairs), len(0), w(share) {
+    if (w.left > 0) len = own_rows_of(a.lengths, w.b, a.src[1].rows);
+  }
+  TSB_HD bool next(ShSegment &s) {
+    if (item < a.items) {
+      s.own = false;
+      s.rb = item % a.rb_p;
+      const int split = item / a.rb_p % a.splits;
+      s.kh = item / a.rb_p / a.splits;
+      s.b = 0;
+      s.n_kv = s.tail_lo = a.src[0].rows;
+      s.j0 = split * a.tps;
+      s.nt = min(a.tps, ceil_to(s.n_kv, SH_KT) - s.j0);
+      s.slot = split;
+      s.slots = 1;
+      item += step;
+      return true;
+    }
+    while (w.left > 0) {
+      const int tiles = ceil_to(len, SH_KT), n = ceil_to(tiles, a.chunk);
+      if (w.ch >= n) {  // this unit has no more: on to the next one that has rows
+        w.ch = 0;
+        if (n == 0 || ++w.u == a.Hkv * a.rb_o) {
+          w.u = 0;
+          ++w.b;
+          len = own_rows_of(a.lengths, w.b, a.src[1].rows);
+        }
+        continue;
+      }
+      const int take = min(w.left, n - w.ch);
+      s.own = true;
+      s.b = w.b;
+      s.kh = w.u / a.rb_o;
+      s.rb = w.u % a.rb_o;
+      s.n_kv = len;
+      s.tail_lo = len - a.tail;  // may be negative: fewer own rows than tree rows
+      s.j0 = w.ch * a.chunk;
+      s.nt = min(take * a.chunk, tiles - s.j0);
+      s.slot = a.splits + w.ch;
+      s.slots = take;
+      w.ch += take;
+      w.left -= take;
+      return true;
+    }
+    return false;
+  }
+};
+
+// ---------------------------------------------------------------- pairs of CTAs
+// Address of this CTA's shared-memory object in CTA `rank` of the cluster.
+TSB_HD uint32_t cluster_addr(const void *p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
+  return r;
+}
+TSB_HD void cluster_arrive_on(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+TSB_HD void cluster_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+TSB_HD bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendHintNs)
+      : "memory");
+  return ok != 0;
+}
+// warp_wait for a barrier that the other CTA arrives on, too.
+TSB_HD bool warp_wait_cluster(uint64_t *bar, uint32_t parity) {
+  bool ok = mbar_try_wait_cluster(bar, parity);
+  if (!ok) {
+    const unsigned long long t0 = globaltimer_ns();
+    for (uint32_t it = 1; !ok; ++it) {
+      ok = mbar_try_wait_cluster(bar, parity);
+      if (!ok && (it & 15u) == 0) {
+        if (*(volatile unsigned int *)&g_device_status != 0u) break;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+          record_status(TSB_ETIMEOUT);
+          break;
+        }
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+TSB_HD void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Tiled load into this CTA's shared memory that completes on a barrier of either CTA.
+TSB_HD void tma_load_2d_pair(void *dst, const void *tmap, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 "
+      "[%0], [%1, {%2, %3}], [%4];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+TSB_HD void pair_tmem_alloc(uint32_t *dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(dst_smem)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+}
+TSB_HD void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+// D (+)= A B over both CTAs: each has its 128 rows of A and D, and half of B's columns.
+TSB_HD void pair_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+TSB_HD void pair_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrive on bar in both CTAs once every MMA issued so far by this thread completes.
+TSB_HD void pair_commit(uint64_t *bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_addr(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
+TSB_HD void cp_async4(void *dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_addr(dst)), "l"(src) : "memory");
 }
 // Arrive on bar when this thread's cp.async copies issued so far have landed
 // (counts as one of the barrier's expected arrivals).
 TSB_HD void cp_async_arrive(uint64_t *bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
+TSB_HD void named_barrier_arrive(int id, int count) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(count) : "memory");
+}
 
-template <int FMT>
-__global__ void __launch_bounds__(ShCfg<FMT>::THREADS, 1)
+template <bool SCALED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(ShCfg<SCALED>::THREADS, 1)
 tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __grid_constant__ CUtensorMap tmap_vp,
                         const __grid_constant__ CUtensorMap tmap_ko, const __grid_constant__ CUtensorMap tmap_vo,
                         const __grid_constant__ ShArgs a) {
-  using C = ShCfg<FMT>;
-  constexpr int NK = C::NK, NV = C::NV, NR = C::NR;
+  using C = ShCfg<SCALED>;
+  constexpr int NK = SH_NK, NV = SH_NV;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem =
       reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   unsigned char *sK = smem;
-  unsigned char *sV = sK + NK * SH_KV_BYTES;
-  unsigned char *sRaw = sV + NV * SH_KV_BYTES;
-  float *sSc = reinterpret_cast<float *>(sRaw + NR * C::RAW_STAGE);
+  unsigned char *sV = sK + NK * SH_K_BYTES;
+  unsigned char *sP = sV + NV * SH_V_BYTES;
+  float *sSc = reinterpret_cast<float *>(sP + 2 * SH_P_BYTES);  // [SH_NSC][2][64]: key, then value scales
   uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<unsigned char *>(sSc) + C::SC_BYTES);
-  uint64_t *q_done = bars;
-  uint64_t *k_full = bars + 1, *k_free = k_full + NK;
-  uint64_t *v_full = k_free + NK, *v_free = v_full + NV;
-  uint64_t *s_full = v_free + NV, *s_free = s_full + 2;
-  uint64_t *p_full = s_free + 2, *p_free = p_full + 2;
-  uint64_t *raw_full = p_free + 2, *raw_free = raw_full + NR;  // 8-bit formats
-  uint64_t *sc_full = raw_free + NR;                            // reference format, [SH_NSC]
+  // in CTA 0, both CTAs arrive: tiles loaded, scores read, P written, Q written, O read
+  uint64_t *k_full = bars, *v_full = k_full + NK, *s_free = v_full + NV, *p_full = s_free + 2;
+  uint64_t *q_full = p_full + 2, *o_free = q_full + 1;
+  // in both CTAs: commits of the MMAs
+  uint64_t *k_free = o_free + 1, *v_free = k_free + NK, *s_full = v_free + NV, *pv_done = s_full + 2;
+  uint64_t *v_last = pv_done + 2;                       // a CTA's own: a V tile with rows past the end
+  uint64_t *sc_full = v_last + 1, *sc_free = sc_full + SH_NSC;  // row scales
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::NBARS);
-  unsigned long long *sBits = reinterpret_cast<unsigned long long *>(bars + C::NBARS + 1);  // [T <= 64]
-  int32_t *sPar = reinterpret_cast<int32_t *>(sBits + 64);                                 // [T <= 64]
+  ShShare *sShare = reinterpret_cast<ShShare *>(bars + C::NBARS + 2);
+  int *sSum = reinterpret_cast<int *>(bars + C::NBARS + 4);                                      // [<= 32 warps]
+  unsigned long long *sBits = reinterpret_cast<unsigned long long *>(bars + C::NBARS + 4 + 16);  // [4][T <= 64]
+  int32_t *sPar = reinterpret_cast<int32_t *>(sBits + 4 * 64);                                   // [4][T <= 64]
+  float *sRow = reinterpret_cast<float *>(sPar + 4 * 64);                                        // [2][128]
+  float *sRef = sRow + 2 * 128;                                                                  // [128]
 
-  griddep_wait();  // programmatic dependent: q, the caches and the lengths are the previous kernels'
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int G = a.Hq / a.Hkv, R = G * a.T;
-  // ---- this CTA's unit
-  const bool own = (int)blockIdx.x >= a.ctas_p;
-  int unit = own ? blockIdx.x - a.ctas_p : blockIdx.x;
-  const int splits = own ? a.splits_o : a.splits_p;
-  const int split = unit % splits;
-  unit /= splits;
-  const int rbs = own ? a.rb_o : a.rb_p;
-  const int rb = unit % rbs;
-  unit /= rbs;
-  const int kh = unit % a.Hkv;
-  const int b = own ? unit / a.Hkv : 0;  // prefix units span the batch
-  const ShSource &src = a.src[own];
-  const int n_kv = own && a.lengths ? min(max(a.lengths[b], 0), src.rows) : src.rows;
-  const int tail_lo = own ? n_kv - a.tail : n_kv;  // may be negative: fewer own rows than tree rows
-  const int n_rows = own ? R : a.B * R;
-  const int tps = own ? a.tps_o : a.tps_p;
-  const int n_tiles_total = (n_kv + SH_KT - 1) / SH_KT;
-  const int j_begin = split * tps;
-  const int nt = max(0, min(n_tiles_total, j_begin + tps) - j_begin);
-  const CUtensorMap &tmap_k = own ? tmap_ko : tmap_kp;
-  const CUtensorMap &tmap_v = own ? tmap_vo : tmap_vp;
-  const size_t kv_row0 = ((size_t)b * a.Hkv + kh) * (size_t)src.cap;
-
+  const int rank = blockIdx.x & 1, pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
-    // bf16 tiles are filled by a TMA transaction, 8-bit ones by the converter warps
-    const uint32_t fill = C::Q8 ? SH_NCONV : 1;
-    mbar_init(q_done, 4);
-    for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], fill); mbar_init(&k_free[i], 1); }
-    for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], fill); mbar_init(&v_free[i], 1); }
+    for (int i = 0; i < NK; ++i) { mbar_init(&k_full[i], 2); mbar_init(&k_free[i], 1); }
+    for (int i = 0; i < NV; ++i) { mbar_init(&v_full[i], 2); mbar_init(&v_free[i], 1); }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&s_free[i], 4);
-      mbar_init(&p_full[i], 4);
-      mbar_init(&p_free[i], 1);
+      mbar_init(&s_free[i], SH_NSOFT);  // four warps of each CTA have a tile
+      mbar_init(&p_full[i], SH_NSOFT);
+      mbar_init(&pv_done[i], 1);
     }
-    // raw tiles: the bulk copy's expect, and (MLX) 32 lanes' scale copies
-    for (int i = 0; i < NR; ++i) { mbar_init(&raw_full[i], C::MLX ? 33 : 1); mbar_init(&raw_free[i], SH_NCONV); }
-    if (C::REF)
-      for (int i = 0; i < SH_NSC; ++i) mbar_init(&sc_full[i], SH_NCONV);
+    mbar_init(q_full, 2 * SH_NSOFT);
+    mbar_init(o_free, 2 * SH_NSOFT);
+    mbar_init(v_last, 1);
+    if (SCALED)
+      for (int i = 0; i < SH_NSC; ++i) { mbar_init(&sc_full[i], 32); mbar_init(&sc_free[i], SH_NSOFT / 2); }
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 0) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
+  if (warp == 0) pair_tmem_alloc(tmem_slot, 512);
+  griddep_wait();  // programmatic dependent: q, the caches and the lengths are the previous kernels'
+
+  // ---- this pair's share of the own chunks. A thread adds up a run of requests.
+  {
+    const int per = ceil_to(a.B, C::THREADS);
+    const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+    const int units = a.Hkv * a.rb_o;
+    auto chunks_of = [&](int b) {
+      return ceil_to(ceil_to(own_rows_of(a.lengths, b, a.src[1].rows), SH_KT), a.chunk) * units;
+    };
+    int mine = 0;
+    if (a.src[1].rows > 0)
+      for (int b = b0; b < b1; ++b) mine += chunks_of(b);
+    int up = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += v;
+    }
+    if (lane == 31) sSum[warp] = up;
+    if (threadIdx.x == 0) *sShare = ShShare{0, 0, 0, 0};
+    __syncthreads();
+    int before = up - mine, total = 0;
+    for (int w = 0; w < C::THREADS / 32; ++w) {
+      if (w < warp) before += sSum[w];
+      total += sSum[w];
+    }
+    // pairs with one prefix segment more carry that much less of the rest
+    const long long G = pairs, more = a.items % G;
+    const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk + SH_SEG_COST);
+    const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
+    const long long q_more = all > need ? all - need : 0;
+    const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
+    const double sum = (double)(more * q_more + (G - more) * q_less);
+    auto start = [&](long long i) -> int {
+      const long long q = min(i, more) * q_more + max(i - more, 0ll) * q_less;
+      return i == G ? total : (int)((double)total * ((double)q / sum));
+    };
+    const int w0 = start(pair), w1 = start(pair + 1);
+    if (w1 > w0 && w0 >= before && w0 < before + mine) {
+      int at = w0 - before, b = b0, n = chunks_of(b);
+      while (at >= n) {
+        at -= n;
+        n = chunks_of(++b);
+      }
+      n /= units;
+      *sShare = ShShare{b, at / n, at % n, w1 - w0};
+    }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // the other CTA's barriers are ready
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  const ShShare share = *sShare;
+  ShWalk walk(a, share, pair, pairs);
+  ShSegment sg = {};
+  const int G = a.Hq / a.Hkv, R = G * a.T;
 
   if (warp == 0) {
-    if constexpr (!C::Q8) {
-      // ---------------- K producer
-      if (elect_one()) {
-        tma_prefetch_desc(&tmap_k);
-        int j = 0;
-        for (; j < nt; ++j) {
-          const int key0 = (int)kv_row0 + (j_begin + j) * SH_KT;
-          const int st = j % NK;
-          if (j >= NK && !mbar_wait(&k_free[st], ((j / NK) - 1) & 1)) break;
-          mbar_arrive_expect_tx(&k_full[st], SH_KV_BYTES);
+    // ---------------- K producer: keys 32 rank .. 32 rank + 31 of each tile, and (int8 rows)
+    // the row scales of all its keys and values
+    int g = 0;
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const CUtensorMap *map = sg.own ? &tmap_ko : &tmap_kp;
+      const ShSource &src = a.src[sg.own];
+      const int row0 = (sg.b * a.Hkv + sg.kh) * src.cap + sg.j0 * SH_KT + rank * (SH_KT / 2);
+      const size_t sc0 = (size_t)(sg.b * a.Hkv + sg.kh) * (size_t)src.sc_cap;
+      for (int j = 0; j < sg.nt; ++j, ++g) {
+        const int st = g % NK;
+        if (g >= NK && !warp_wait(&k_free[st], ((g / NK) - 1) & 1)) { ok = false; break; }
+        if (elect_one()) {
+          const uint32_t full = cluster_addr(&k_full[st], 0);
+          cluster_expect_tx(full, SH_K_BYTES);
 #pragma unroll
           for (int d = 0; d < 4; ++d)
-            tma_load_2d(sK + st * SH_KV_BYTES + d * SH_KVBOX, &tmap_k, d * 64, key0, &k_full[st]);
+            tma_load_2d_pair(sK + st * SH_K_BYTES + d * SH_KBOX, map, d * 64, row0 + j * SH_KT, full);
         }
-        // drain: the issued loads have landed before the CTA can exit
-        for (int i = (j > NK ? j - NK : 0); i < j; ++i) mbar_drain(&k_full[i % NK], (i / NK) & 1);
-      }
-    } else {
-      // ---------------- raw 8-bit tiles, rows [key0, min(key0 + 64, cap)) of this head's cache
-      int seq = 0;
-      auto load_raw = [&](bool isv, int j) -> bool {
-        const int rs = seq % NR;
-        if (seq >= NR && !warp_wait(&raw_free[rs], ((seq / NR) - 1) & 1)) return false;
-        const int key0 = (j_begin + j) * SH_KT;
-        const int rows = min(SH_KT, src.cap - key0);
-        const size_t r0 = kv_row0 + key0;
-        unsigned char *dst = sRaw + rs * C::RAW_STAGE;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&raw_full[rs], (uint32_t)rows * SH_D);
-          bulk_load(dst, (isv ? src.vc : src.kc) + r0 * SH_D, (uint32_t)rows * SH_D, &raw_full[rs]);
-        }
-        if (C::MLX) {
-          const uint2 *sc = reinterpret_cast<const uint2 *>(isv ? src.vs : src.ks) + r0;
-          const uint2 *bi = reinterpret_cast<const uint2 *>(isv ? src.vb : src.kb) + r0;
-          for (int r = lane; r < rows; r += 32) {
-            cp_async8(dst + SH_RAW_CODES + r * 8, sc + r);
-            cp_async8(dst + SH_RAW_CODES + SH_KT * 8 + r * 8, bi + r);
-          }
-          cp_async_arrive(&raw_full[rs]);
-        }
-        ++seq;
-        return true;
-      };
-      bool ok = true;
-      for (int j = 0; j < nt && ok; ++j) {
-        if (j == 0) ok = load_raw(false, 0);
-        if (ok && j + 1 < nt) ok = load_raw(false, j + 1);
-        if (ok) ok = load_raw(true, j);
-      }
-      for (int i = (seq > NR ? seq - NR : 0); i < seq; ++i) mbar_drain(&raw_full[i % NR], (i / NR) & 1);
-      __syncwarp();
-    }
-  } else if (warp >= 6) {
-    if constexpr (!C::Q8) {
-      // ---------------- V producer (warp 6)
-      if (elect_one()) {
-        tma_prefetch_desc(&tmap_v);
-        int j = 0;
-        for (; j < nt; ++j) {
-          const int key0 = (int)kv_row0 + (j_begin + j) * SH_KT;
-          const int st = j % NV;
-          if (j >= NV && !mbar_wait(&v_free[st], ((j / NV) - 1) & 1)) break;
-          mbar_arrive_expect_tx(&v_full[st], SH_KV_BYTES);
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            tma_load_2d(sV + st * SH_KV_BYTES + d * SH_KVBOX, &tmap_v, d * 64, key0, &v_full[st]);
-        }
-        for (int i = (j > NV ? j - NV : 0); i < j; ++i) mbar_drain(&v_full[i % NV], (i / NV) & 1);
-      }
-    } else {
-      // ---------------- converters: raw tile -> swizzled bf16 tile. Lane l of
-      // warp w writes 16-byte chunk l&7 of D box l>>3 (the MLX group) of rows
-      // (w - 6) + 8 i: eight lanes fill one 128-byte row of a box.
-      const int r_lo = warp - 6;
-      const int grp = lane >> 3, ch = lane & 7;
-      const int ct = threadIdx.x - 192;
-      int seq = 0;
-      auto convert = [&](bool isv, int j) -> bool {
-        const int rs = seq % NR;
-        uint64_t *full;
-        unsigned char *dst;
-        if (!isv) {
-          const int st = j % NK;
-          if (j >= NK && !warp_wait(&k_free[st], ((j / NK) - 1) & 1)) return false;
-          dst = sK + st * SH_KV_BYTES;
-          full = &k_full[st];
-        } else {
-          const int st = j % NV;
-          if (j >= NV && !warp_wait(&v_free[st], ((j / NV) - 1) & 1)) return false;
-          dst = sV + st * SH_KV_BYTES;
-          full = &v_full[st];
-        }
-        const int key0 = (j_begin + j) * SH_KT;
-        const int nvalid = n_kv - key0;  // rows below this are keys
-        // reference format: the tile's key (threads 0-63) and value (64-127) row scales
-        float rsc = 0.f;
-        if (C::REF && !isv && ct < 2 * SH_KT) {
-          const int r = ct & 63;
-          if (r < nvalid) rsc = reinterpret_cast<const float *>(ct < 64 ? src.ks : src.vs)[kv_row0 + key0 + r];
-        }
-        if (!warp_wait(&raw_full[rs], (seq / NR) & 1)) return false;
-        const unsigned char *raw = sRaw + rs * C::RAW_STAGE;
-        const uint16_t *rsb = reinterpret_cast<const uint16_t *>(raw + SH_RAW_CODES);
-        constexpr int CB = 4, ROWS = SH_KT / SH_NCONV;
-        static_assert(SH_KT % SH_NCONV == 0 && ROWS % CB == 0, "converter rows");
-        // batches of CB rows, loads first; rolled, as the instruction cache also
-        // holds the softmax loop of the same sub-partition
-#pragma unroll 1
-        for (int h = 0; h < ROWS / CB; ++h) {
-          uint2 w[CB];
-          uint32_t sb[CB], bb[CB];
-#pragma unroll
-          for (int i = 0; i < CB; ++i) {
-            const int r = r_lo + SH_NCONV * (CB * h + i);
-            w[i] = make_uint2(0u, 0u);
-            sb[i] = 0u;
-            bb[i] = 0u;
-            if (r < nvalid) {
-              w[i] = *reinterpret_cast<const uint2 *>(raw + r * SH_D + lane * 8);
-              if (C::MLX) {
-                sb[i] = rsb[r * 4 + grp];
-                bb[i] = rsb[SH_KT * 4 + r * 4 + grp];
-              }
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < CB; ++i) {
-            const int r = r_lo + SH_NCONV * (CB * h + i);
-            uint4 o = make_uint4(0u, 0u, 0u, 0u);
-            if (r < nvalid) {
-              if (C::MLX)
-                o = dequant8_mlx(w[i], __uint_as_float(sb[i] << 16), __uint_as_float(bb[i] << 16));
-              else
-                o = convert8_s8(w[i]);
-            }
-            *reinterpret_cast<uint4 *>(dst + grp * SH_KVBOX + r * 128 + ((ch ^ (r & 7)) << 4)) = o;
-          }
-        }
-        if (C::REF && !isv && ct < 2 * SH_KT) sSc[(j % SH_NSC) * 2 * SH_KT + ct] = rsc;
-        fence_proxy_async_smem();  // generic writes -> MMA reads; raw slot reads -> refill
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&raw_free[rs]);
-          mbar_arrive(full);
-          if (C::REF && !isv) mbar_arrive(&sc_full[j % SH_NSC]);
+        if (SCALED) {
+          const int sc = g % SH_NSC;
+          if (g >= SH_NSC && !warp_wait(&sc_free[sc], ((g / SH_NSC) - 1) & 1)) { ++g; ok = false; break; }
+          float *dst = sSc + sc * 2 * SH_KT;
+          for (int r = lane; r < SH_KT; r += 32) {
+            const int key = (sg.j0 + j) * SH_KT + r;
+            if (key < sg.n_kv) {
+              cp_async4(dst + r, src.ks + sc0 + key);
+              cp_async4(dst + SH_KT + r, src.vs + sc0 + key);
+            } else {
+              dst[r] = dst[SH_KT + r] = 0.f;
+            }
+          }
+          cp_async_arrive(&sc_full[sc]);
         }
-        ++seq;
-        return true;
-      };
-      bool ok = true;
-      for (int j = 0; j < nt && ok; ++j) {
-        if (j == 0) ok = convert(false, 0);
-        if (ok && j + 1 < nt) ok = convert(false, j + 1);
-        if (ok) ok = convert(true, j);
       }
     }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer
-    const uint32_t idesc_s = idesc_bf16_f32(128, SH_KT);
-    const uint32_t idesc_o = idesc_bf16_f32(128, SH_D) | (1u << 16);  // B (V) MN-major
-    bool ok = warp_wait(q_done, 0);
-    auto issue_s = [&](int j) -> bool {
-      const int s = j % NK, sb = j & 1;
-      if (!warp_wait(&k_full[s], (j / NK) & 1)) return false;
-      if (j >= 2 && !warp_wait(&s_free[sb], ((j >> 1) - 1) & 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint32_t kb = smem_addr(sK + s * SH_KV_BYTES);
+    // Before the CTA may exit: its tiles have been used, and the commits that say so
+    // have arrived. After a failure, at least the loads have landed (both CTAs' in CTA 0).
+    for (int i = (g > NK ? g - NK : 0); i < g; ++i) ok = ok && warp_wait(&k_free[i % NK], (i / NK) & 1);
+    if (!ok && rank == 0)
+      for (int i = (g > NK ? g - NK : 0); i < g; ++i) mbar_drain(&k_full[i % NK], (i / NK) & 1);
+    if (SCALED) asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+  } else if (warp == 3) {
+    // ---------------- V producer: columns 128 rank .. 128 rank + 127 of each tile
+    int g = 0, lasts = 0;
+    bool ok = true;
+    while (ok && walk.next(sg)) {
+      const CUtensorMap *map = sg.own ? &tmap_vo : &tmap_vp;
+      const int row0 = (sg.b * a.Hkv + sg.kh) * a.src[sg.own].cap + sg.j0 * SH_KT;
+      for (int j = 0; j < sg.nt; ++j, ++g) {
+        const int st = g % NV;
+        if (g >= NV && !warp_wait(&v_free[st], ((g / NV) - 1) & 1)) { ok = false; break; }
+        const uint32_t full = cluster_addr(&v_full[st], 0);
+        unsigned char *dst = sV + st * SH_V_BYTES;
+        const int first = sg.n_kv - (sg.j0 + j) * SH_KT;  // rows past the keys from here on
+        if (first >= SH_KT) {
+          if (elect_one()) {
+            cluster_expect_tx(full, SH_V_BYTES);
 #pragma unroll
-        for (int kk = 0; kk < 16; ++kk) {
-          const uint32_t off_k = (kk >> 2) * SH_KVBOX + (kk & 3) * 32;
-          mma_ts_f16(tmem + SH_S0 + sb * 64, tmem + SH_Q + kk * 8, desc_kmajor_sw128(kb + off_k), idesc_s,
-                     kk > 0 ? 1u : 0u);
-        }
-        mma_commit(&s_full[sb]);
-        mma_commit(&k_free[s]);
-      }
-      __syncwarp();
-      return true;
-    };
-    auto issue_pv = [&](int j) -> bool {
-      const int s = j % NV, pb = j & 1;
-      if (!warp_wait(&v_full[s], (j / NV) & 1)) return false;
-      if (!warp_wait(&p_full[pb], (j >> 1) & 1)) return false;
-      tc_fence_after();
-      if (!C::Q8) {
-        // bf16: the TMA tile holds whatever follows row n_kv; zero those V rows
-        // (their weights are 0, but 0 * NaN would not be 0)
-        const int first = n_kv - (j_begin + j) * SH_KT;
-        if (first < SH_KT) {
-          unsigned char *vt = sV + s * SH_KV_BYTES;
-          for (int i = lane; i < (SH_KT - first) * 32; i += 32) {
-            const int r = first + (i >> 5), c = i & 31;
-            *reinterpret_cast<uint4 *>(vt + (c >> 3) * SH_KVBOX + r * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+            for (int d = 0; d < 2; ++d)
+              tma_load_2d_pair(dst + d * SH_VBOX, map, rank * 128 + d * 64, row0 + j * SH_KT, full);
+          }
+        } else {
+          // the tile holds whatever follows row n_kv; zero those rows before the MMA
+          // reads them (their weights are 0, but 0 * NaN would not be 0)
+          if (elect_one()) {
+            mbar_arrive_expect_tx(v_last, SH_V_BYTES);
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+              tma_load_2d(dst + d * SH_VBOX, map, rank * 128 + d * 64, row0 + j * SH_KT, v_last);
+          }
+          __syncwarp();
+          ok = warp_wait(v_last, lasts & 1);
+          ++lasts;
+          for (int i = lane; i < (SH_KT - first) * 16; i += 32) {
+            const int r = first + (i >> 4), c = i & 15;
+            *reinterpret_cast<uint4 *>(dst + (c >> 3) * SH_VBOX + r * 128 + ((c & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
           }
           fence_proxy_async_smem();
           __syncwarp();
+          if (lane == 0) cluster_arrive_on(full);
         }
+        __syncwarp();
       }
-      if (elect_one()) {
-        const uint32_t vb = smem_addr(sV + s * SH_KV_BYTES);
+    }
+    for (int i = (g > NV ? g - NV : 0); i < g; ++i) ok = ok && warp_wait(&v_free[i % NV], (i / NV) & 1);
+    if (!ok && rank == 0)
+      for (int i = (g > NV ? g - NV : 0); i < g; ++i) mbar_drain(&v_full[i % NV], (i / NV) & 1);
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      // ---------------- S = Q K^T
+      const uint32_t idesc = idesc_bf16_f32(SH_ROWS, SH_KT);
+      int g = 0, seg = 0;
+      bool ok = true;
+      while (ok && walk.next(sg)) {
+        ok = warp_wait_cluster(q_full, seg & 1);
+        ++seg;
+        for (int j = 0; j < sg.nt && ok; ++j, ++g) {
+          const int s = g % NK, sb = g & 1;
+          ok = warp_wait_cluster(&k_full[s], (g / NK) & 1);
+          if (ok && g >= 2) ok = warp_wait_cluster(&s_free[sb], ((g >> 1) - 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t kb = smem_addr(sK + s * SH_K_BYTES);
 #pragma unroll
-        for (int kk = 0; kk < SH_KT / 16; ++kk) {
-          mma_ts_f16(tmem + SH_O, tmem + SH_S0 + pb * 64 + kk * 8, desc_mnmajor_sw128(vb + kk * 2048, SH_KVBOX),
-                     idesc_o, (j > 0 || kk > 0) ? 1u : 0u);
-        }
-        mma_commit(&v_free[s]);
-        mma_commit(&p_free[pb]);  // completes after this and every earlier MMA
-      }
-      __syncwarp();
-      return true;
-    };
-    if (ok && nt > 0) ok = issue_s(0);
-    for (int j = 0; j < nt && ok; ++j) {
-      if (j + 1 < nt) ok = issue_s(j + 1);
-      if (ok) ok = issue_pv(j);
-    }
-  } else if (warp >= 2 && warp <= 5) {
-    // ---------------- softmax / epilogue (thread = query row = TMEM lane)
-    if (own) {  // node masks, from the parent array or given
-      const int st = threadIdx.x - 64;  // 0..127
-      if (st < a.T) sPar[st] = a.parents ? a.parents[(size_t)b * a.T + st] : 0;
-      named_barrier_sync(1, 128);
-      if (st < a.T) {
-        unsigned long long m = 0;
-        if (a.parents) {
-          int j = st;
-          bool okp = true;
-          for (int steps = 0; steps <= a.T && j != -1; ++steps) {
-            m |= 1ull << j;
-            const int pj = sPar[j];
-            if (!(pj == -1 || (pj >= 0 && pj < j))) { okp = false; break; }
-            j = pj;
+            for (int kk = 0; kk < 16; ++kk)
+              pair_mma_ts(tmem + SH_S0 + sb * 64, tmem + SH_Q + kk * 8,
+                          desc_kmajor_sw128(kb + (kk >> 2) * SH_KBOX + (kk & 3) * 32), idesc, kk > 0 ? 1u : 0u);
+            pair_commit(&s_full[sb]);
+            pair_commit(&k_free[s]);
           }
-          if (!okp) m = 0;
-        } else {
-          m = a.bits[(size_t)b * a.T + st];
+          __syncwarp();
         }
-        sBits[st] = m;
       }
-      named_barrier_sync(1, 128);
     }
-    const int q = warp & 3;
+  } else if (warp == 2) {
+    if (rank == 0) {
+      // ---------------- O += P V
+      const uint32_t idesc = idesc_bf16_f32(SH_ROWS, SH_D) | (1u << 16);  // B (V) MN-major
+      int g = 0, seg = 0;
+      bool ok = true;
+      while (ok && walk.next(sg)) {
+        if (seg > 0) ok = warp_wait_cluster(o_free, (seg - 1) & 1);  // the last segment's O has been read
+        ++seg;
+        for (int j = 0; j < sg.nt && ok; ++j, ++g) {
+          const int s = g % NV, pb = g & 1;
+          ok = warp_wait_cluster(&v_full[s], (g / NV) & 1);
+          if (ok) ok = warp_wait_cluster(&p_full[pb], (g >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t vb = smem_addr(sV + s * SH_V_BYTES), pa = smem_addr(sP + pb * SH_P_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < SH_KT / 16; ++kk)
+              pair_mma_ss(tmem + SH_O, desc_kmajor_sw128(pa + kk * 32), desc_mnmajor_sw128(vb + kk * 2048, SH_VBOX),
+                          idesc, (j > 0 || kk > 0) ? 1u : 0u);
+            pair_commit(&v_free[s]);
+            pair_commit(&pv_done[pb]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+  } else {
+    // ---------------- softmax / epilogue
+    const int odd = (warp - SH_SOFT0) >> 2, q = warp & 3;  // this warp's tiles, and its 32 rows
     const int r = q * 32 + lane;
-    const int gr = rb * 128 + r;
-    const bool row_valid = gr < n_rows;
-    // the row's request, head and node
-    const int rq = row_valid ? (own ? b : gr / R) : 0;
-    const int rr = row_valid ? (own ? gr : gr % R) : 0;
-    const int hl = rr / a.T, node = rr % a.T;
-    const int head = kh * G + hl;
-    const unsigned long long mybits = own ? sBits[node] : 0ull;
+    const int bar_rows = 1 + q;                                 // both warps of the rows
+    const int bar_take = 5 + 4 * odd + q, bar_pass = 5 + 4 * (odd ^ 1) + q;  // the token
     const uint32_t lane_base = tmem + ((uint32_t)(q * 32) << 16);
     const float sl2 = a.scale_log2;
-    float m = -INFINITY, l = 0.f;  // running max (log2 domain) and sum
-    if (nt > 0) {
-      // Q row -> TMEM lane r, columns SH_Q + d/2 (the A-operand layout of a K-major M=128 tile)
-      const uint4 *qrow = reinterpret_cast<const uint4 *>(a.q + rq * a.q_sb + head * a.q_sh + node * a.q_st);
-#pragma unroll 1
-      for (int bx = 0; bx < 4; ++bx) {
+    const size_t rows_all = (size_t)a.B * a.Hq * a.T;
+    const uint32_t q_full0 = cluster_addr(q_full, 0), o_free0 = cluster_addr(o_free, 0);
+    const uint32_t s_free0 = cluster_addr(&s_free[odd], 0), p_full0 = cluster_addr(&p_full[odd], 0);
+    int g = 0;
+    // A wait that ran out (never in a healthy run) is not followed by others, but the
+    // barriers among the warps go on: nobody waits for a warp that has left.
+    bool ok = true;
+    bool more = walk.next(sg);
+    // the row of a segment that this thread has
+    int rq = 0, head = 0, node = 0;
+    bool row_valid = false;
+    auto place = [&](const ShSegment &s) {
+      const int gr = s.rb * SH_ROWS + rank * 128 + r;
+      row_valid = gr < (s.own ? R : a.B * R);
+      rq = row_valid && !s.own ? gr / R : s.b;
+      const int rr = row_valid ? (s.own ? gr : gr % R) : 0;
+      head = s.kh * G + rr / a.T;
+      node = rr % a.T;
+    };
+    // Q row -> TMEM lane r, columns SH_Q + d/2 (the A-operand layout of a K-major
+    // M=128 tile), half of D per warp. All S of the segment before are complete.
+    auto load_q = [&]() {
+      const uint4 *qrow = reinterpret_cast<const uint4 *>(a.q + rq * a.q_sb + head * a.q_sh + node * a.q_st) + odd * 16;
+#pragma unroll
+      for (int bx = 0; bx < 2; ++bx) {
         uint32_t qv[32];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
           const uint4 u = row_valid ? __ldg(qrow + bx * 8 + c) : make_uint4(0u, 0u, 0u, 0u);
           qv[4 * c] = u.x; qv[4 * c + 1] = u.y; qv[4 * c + 2] = u.z; qv[4 * c + 3] = u.w;
         }
-        tmem_st32(lane_base + SH_Q + bx * 32, qv);
+        tmem_st32(lane_base + SH_Q + odd * 64 + bx * 32, qv);
       }
       tmem_wait_st();
-    }
-    tc_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(q_done);
-    bool ok = true;
-    for (int j = 0; j < nt && ok; ++j) {
-      const int sb = j & 1;
-      ok = warp_wait(&s_full[sb], (j >> 1) & 1);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t sr[64];
-      {
-        uint32_t (&lo)[32] = *reinterpret_cast<uint32_t (*)[32]>(&sr[0]);
-        uint32_t (&hi)[32] = *reinterpret_cast<uint32_t (*)[32]>(&sr[32]);
-        tmem_ld32(lane_base + SH_S0 + sb * 64, lo);
-        tmem_ld32(lane_base + SH_S0 + sb * 64 + 32, hi);
-      }
-      tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_free[sb]);
-      const float *ksc = sSc + (j % SH_NSC) * 2 * SH_KT;  // reference format: key, then value scales
-      if (C::REF) {
-        ok = warp_wait(&sc_full[j % SH_NSC], (j / SH_NSC) & 1);
-        if (!ok) break;
-#pragma unroll
-        for (int e = 0; e < 64; e += 4) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(ksc + e);
-          sr[e] = __float_as_uint(__uint_as_float(sr[e]) * k4.x);
-          sr[e + 1] = __float_as_uint(__uint_as_float(sr[e + 1]) * k4.y);
-          sr[e + 2] = __float_as_uint(__uint_as_float(sr[e + 2]) * k4.z);
-          sr[e + 3] = __float_as_uint(__uint_as_float(sr[e + 3]) * k4.w);
+      if (lane == 0) cluster_arrive_on(q_full0);
+    };
+    if (more) {
+      place(sg);
+      load_q();
+    }
+    int masks_of = -1;  // the request whose node masks are in sBits
+    while (more) {
+      if (sg.own && masks_of != sg.b) {  // node masks, from the parent array or given; the rows' two warps have their own
+        masks_of = sg.b;
+        const int st = odd * 32 + lane;
+        named_barrier_sync(bar_rows, 64);  // the last request's have been read
+        if (st < a.T) sPar[q * 64 + st] = a.parents ? a.parents[(size_t)sg.b * a.T + st] : 0;
+        named_barrier_sync(bar_rows, 64);
+        if (st < a.T) {
+          unsigned long long mk = 0;
+          if (a.parents) {
+            int j = st;
+            bool okp = true;
+            for (int steps = 0; steps <= a.T && j != -1; ++steps) {
+              mk |= 1ull << j;
+              const int pj = sPar[q * 64 + j];
+              if (!(pj == -1 || (pj >= 0 && pj < j))) { okp = false; break; }
+              j = pj;
+            }
+            if (!okp) mk = 0;
+          } else {
+            mk = a.bits[(size_t)sg.b * a.T + st];
+          }
+          sBits[q * 64 + st] = mk;
         }
+        named_barrier_sync(bar_rows, 64);
       }
-      // mask (only the tail and the last tile need it), then the tile max of the
-      // raw scores in eight independent chains; the scale is applied in the exp
-      const int key0 = (j_begin + j) * SH_KT;
-      if ((key0 + SH_KT > tail_lo) || (key0 + SH_KT > n_kv)) {
-#pragma unroll
-        for (int e = 0; e < 64; ++e) {
-          const int key = key0 + e;
-          bool vis = key < n_kv;
-          if (vis && key >= tail_lo) vis = (mybits >> (key - tail_lo)) & 1ull;
-          if (!vis) sr[e] = __float_as_uint(-INFINITY);
+      const unsigned long long mybits = sg.own ? sBits[q * 64 + node] : 0ull;
+      float m_l = -INFINITY, l = 0.f;  // the sum over this warp's tiles, relative to the reference m_l
+      const int g0 = g, g1 = g + sg.nt;
+      for (g = g0 + ((g0 & 1) ^ odd); g < g1; g += 2) {
+        const int j = g - g0;
+        ok = ok && warp_wait(&s_full[odd], (g >> 1) & 1);
+        tc_fence_after();
+        uint32_t sr[64];
+        {
+          uint32_t (&lo)[32] = *reinterpret_cast<uint32_t (*)[32]>(&sr[0]);
+          uint32_t (&hi)[32] = *reinterpret_cast<uint32_t (*)[32]>(&sr[32]);
+          tmem_ld32(lane_base + SH_S0 + odd * 64, lo);
+          tmem_ld32(lane_base + SH_S0 + odd * 64 + 32, hi);
         }
-      }
-      float mx8[8];
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) cluster_arrive_on(s_free0);
+        const float *ksc = sSc + (g % SH_NSC) * 2 * SH_KT;  // key, then value scales
+        if (SCALED) {
+          ok = ok && warp_wait(&sc_full[g % SH_NSC], (g / SH_NSC) & 1);
 #pragma unroll
-      for (int c = 0; c < 8; ++c) mx8[c] = __uint_as_float(sr[c]);
+          for (int e = 0; e < 64; e += 4) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(ksc + e);
+            sr[e] = __float_as_uint(__uint_as_float(sr[e]) * k4.x);
+            sr[e + 1] = __float_as_uint(__uint_as_float(sr[e + 1]) * k4.y);
+            sr[e + 2] = __float_as_uint(__uint_as_float(sr[e + 2]) * k4.z);
+            sr[e + 3] = __float_as_uint(__uint_as_float(sr[e + 3]) * k4.w);
+          }
+        }
+        // mask (only the tail and the last tile need it), then the maximum of the raw
+        // scores in eight independent chains; the scale is applied in the exp
+        const int key0 = (sg.j0 + j) * SH_KT;
+        if ((key0 + SH_KT > sg.tail_lo) || (key0 + SH_KT > sg.n_kv)) {
 #pragma unroll
-      for (int e = 8; e < 64; ++e) mx8[e & 7] = fmaxf(mx8[e & 7], __uint_as_float(sr[e]));
-      const float traw = fmaxf(fmaxf(fmaxf(mx8[0], mx8[1]), fmaxf(mx8[2], mx8[3])),
-                               fmaxf(fmaxf(mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7])));
-      const float tmax = traw * sl2;  // scale > 0: max commutes with it
-      // P V_{j-2} is done (S_j, written after it, is complete); waiting here
-      // keeps every p_free wait below at most one phase behind.
-      if (j >= 2) {
-        ok = warp_wait(&p_free[sb], ((j >> 1) - 1) & 1);
-        if (!ok) break;
-      }
-      // lazy rescale: move the reference max only when it grows by > 2^8
-      const bool grow = tmax > m + SH_RESCALE_LOG2;
-      if (__any_sync(0xffffffffu, grow)) {
-        const float m_new = grow ? tmax : m;
-        const float alpha = (m == -INFINITY) ? 0.f : ex2(m - m_new);
-        if (j > 0) {  // O holds earlier tiles: wait for P V_{j-1} (and all before), then scale O in place
-          ok = warp_wait(&p_free[sb ^ 1], ((j - 1) >> 1) & 1);
-          if (!ok) break;
+          for (int e = 0; e < 64; ++e) {
+            const int key = key0 + e;
+            bool vis = key < sg.n_kv;
+            if (vis && key >= sg.tail_lo) vis = (mybits >> (key - sg.tail_lo)) & 1ull;
+            if (!vis) sr[e] = __float_as_uint(-INFINITY);
+          }
+        }
+        float mx[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(sr[c]);
+#pragma unroll
+        for (int e = 8; e < 64; ++e) mx[e & 7] = fmaxf(mx[e & 7], __uint_as_float(sr[e]));
+        const float tmax = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                 fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7]))) * sl2;  // scale > 0
+        // the token: tile g - 1 has settled the reference
+        if (j > 0) named_barrier_sync(bar_take, 64);
+        const float m_old = j > 0 ? sRef[r] : -INFINITY;
+        const bool grow = tmax > m_old + SH_RESCALE_LOG2;
+        const float m = grow ? tmax : m_old;
+        const bool moves = __any_sync(0xffffffffu, grow);
+        if (moves || j == 0) sRef[r] = m;
+        if (j + 1 < sg.nt) named_barrier_arrive(bar_pass, 64);
+        if (g >= 2) ok = ok && warp_wait(&pv_done[odd], ((g >> 1) - 1) & 1);  // P_{g-2} has been read
+        if (moves && j > 0) {
+          // O holds earlier tiles: wait for P V_{g-1} (and all before), then scale O in place
+          ok = ok && warp_wait(&pv_done[odd ^ 1], ((g - 1) >> 1) & 1);
           tc_fence_after();
+          const float alpha = (m_old == -INFINITY) ? 0.f : ex2(m_old - m);
 #pragma unroll 1
           for (int c = 0; c < SH_D; c += 32) {
             uint32_t o[32];
@@ -519,80 +691,171 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
           }
           tmem_wait_st();
         }
-        l *= alpha;
-        m = m_new;
-      }
-      const float nbase = (m == -INFINITY) ? 0.f : -m;
-      uint32_t pk[32];
-      float ps[4] = {0.f, 0.f, 0.f, 0.f};
+        if (m != m_l) {  // the reference has moved since this warp's last tile
+          l *= m_l == -INFINITY ? 0.f : ex2(m_l - m);
+          m_l = m;
+        }
+        const float nbase = (m == -INFINITY) ? 0.f : -m;
+        // P_g: row r of a K-major, 128-byte-swizzled tile
+        unsigned char *prow = sP + odd * SH_P_BYTES + r * 128;
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[2 * e]), sl2, nbase));
-        const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[2 * e + 1]), sl2, nbase));
-        ps[e & 3] += p0 + p1;
-        if (C::REF) {
-          // the value rows' scales weight P; the running sum keeps the plain weights
-          const float2 v2 = *reinterpret_cast<const float2 *>(ksc + SH_KT + 2 * e);
-          pk[e] = pack_bf16x2(p0 * v2.x, p1 * v2.y);
-        } else {
-          pk[e] = pack_bf16x2(p0, p1);
+        for (int c = 0; c < 8; ++c) {
+          uint32_t pk[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int i = 8 * c + 2 * e;
+            const float p0 = ex2(__fmaf_rn(__uint_as_float(sr[i]), sl2, nbase));
+            const float p1 = ex2(__fmaf_rn(__uint_as_float(sr[i + 1]), sl2, nbase));
+            ps[e] += p0 + p1;
+            if (SCALED) {
+              // the value rows' scales weight P; the running sum keeps the plain weights
+              const float2 v2 = *reinterpret_cast<const float2 *>(ksc + SH_KT + i);
+              pk[e] = pack_bf16x2(p0 * v2.x, p1 * v2.y);
+            } else {
+              pk[e] = pack_bf16x2(p0, p1);
+            }
+          }
+          *reinterpret_cast<uint4 *>(prow + ((c ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+        }
+        l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        fence_proxy_async_smem();
+        tc_fence_before();  // a rescaled O, too
+        __syncwarp();
+        if (lane == 0) {
+          cluster_arrive_on(p_full0);
+          if (SCALED) mbar_arrive(&sc_free[g % SH_NSC]);
         }
       }
-      l += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-      // P_j into TMEM, over the scores it was made from
+      g = g1;
+      // ---- the next segment's Q (its S can start), then this one's partials. All of
+      // this segment's S are complete only once its last tile's have been seen.
+      const ShSegment done = sg;
+      const bool valid = row_valid;
+      const size_t orow = ((size_t)rq * a.Hq + head) * a.T + node;
+      const int last = g1 - 1;
+      // A warp follows its own buffer's barriers phase by phase; the other buffer's are
+      // looked at only when the phase before is known to be over.
+      if ((last & 1) != odd && last >= 1) ok = ok && warp_wait(&pv_done[odd], ((last - 1) >> 1) & 1);
+      if ((last & 1) == odd && last >= 1) ok = ok && warp_wait(&pv_done[odd ^ 1], ((last - 1) >> 1) & 1);
+      ok = ok && warp_wait(&pv_done[last & 1], (last >> 1) & 1);  // P V of the last tile, after which no S of it runs
       tc_fence_after();
-      tmem_st32(lane_base + SH_S0 + sb * 64, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[sb]);
-    }
-    // ---------------- epilogue: normalised partials and (max, sum)
-    const size_t orow = ((size_t)rq * a.Hq + head) * a.T + node;
-    const size_t prow = (size_t)(own ? a.splits_p + split : split) * a.B * a.Hq * a.T + orow;
-    if (ok && nt > 0 && warp_wait(&p_free[(nt - 1) & 1], ((nt - 1) >> 1) & 1)) {
-      tc_fence_after();
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      named_barrier_sync(bar_rows, 64);  // the last tile has settled the reference
+      const float m = sRef[r];
+      sRow[odd * 128 + r] = l * (m_l == -INFINITY ? 0.f : ex2(m_l - m));
+      named_barrier_sync(bar_rows, 64);
+      const float sum = sRow[r] + sRow[128 + r];
+      named_barrier_sync(bar_rows, 64);
+      more = walk.next(sg);
+      if (more) {
+        place(sg);
+        load_q();
+      }
+      const size_t prow = (size_t)done.slot * rows_all + orow;
+      const float inv = sum > 0.f ? 1.f / sum : 0.f;
 #pragma unroll 1
-      for (int c = 0; c < SH_D; c += 32) {
+      for (int c = 0; c < SH_D / 2; c += 32) {
         uint32_t o[32];
-        tmem_ld32(lane_base + SH_O + c, o);
+        tmem_ld32(lane_base + SH_O + odd * 128 + c, o);
         tmem_wait_ld();
-        if (!row_valid) continue;
-        float4 *dst = reinterpret_cast<float4 *>(a.part_o + prow * SH_D + c);
+        if (!valid) continue;
+        float4 *dst = reinterpret_cast<float4 *>(a.part_o + prow * SH_D + odd * 128 + c);
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
                                __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
       }
-    }
-    if (row_valid) {
-      a.part_ml[prow * 2 + 0] = m;
-      a.part_ml[prow * 2 + 1] = l;  // 0: nothing visible, the partial is not read
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) cluster_arrive_on(o_free0);
+      if (valid && odd == 0) {
+        float2 *ml = reinterpret_cast<float2 *>(a.part_ml);
+        ml[prow] = make_float2(m, sum);  // sum 0: nothing visible, the partial is not read
+        for (int s = 1; s < done.slots; ++s) ml[prow + s * rows_all] = make_float2(-INFINITY, 0.f);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
+  cluster_sync_all();  // the other CTA has no use for this one's shared memory any more
   if (warp == 0) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    pair_tmem_dealloc(tmem, 512);
   }
 }
 
+// ---------------------------------------------------------------- 8-bit caches
+// The valid rows of an 8-bit cache as bf16 rows [heads][rows][D]: MLX values
+// bf16(fmaf(code, s, b)), or the int8 codes themselves. 16 lanes have a row; bound
+// by memory (272 or 256 bytes read and 512 written per row).
+struct ShConvert {
+  const unsigned char *src[2];    // K, V codes
+  const uint2 *scale[2], *bias[2];  // MLX: four bf16 per row
+  uint16_t *dst[2];
+  const int32_t *lengths;  // per request, or NULL
+  int heads;               // KV heads per request
+  int cap, rows;           // of the source per (request, head); of the copy
+};
+
+constexpr int SH_CV_ROWS = 64;  // rows of a CTA
+
+template <bool MLX>
+__global__ void __launch_bounds__(256) tree_attn_shared_convert_kernel(const __grid_constant__ ShConvert a) {
+  griddep_wait();  // programmatic dependent: the caches are the previous kernels'
+  griddep_launch_dependents();
+  const int head = blockIdx.y, v = blockIdx.z;
+  const int n = own_rows_of(a.lengths, head / a.heads, a.rows);
+  const int row0 = blockIdx.x * SH_CV_ROWS;
+  if (row0 >= n) return;
+  const int c = threadIdx.x & 15;
+#pragma unroll
+  for (int i = 0; i < SH_CV_ROWS / 16; ++i) {
+    const int row = row0 + i * 16 + (threadIdx.x >> 4);
+    if (row >= n) break;
+    const size_t at = (size_t)head * a.cap + row;
+    const uint4 w = ldg_nc_v4(a.src[v] + at * SH_D + c * 16);
+    uint4 lo, hi;
+    if (MLX) {
+      const uint16_t *sc = reinterpret_cast<const uint16_t *>(a.scale[v] + at), *bi = reinterpret_cast<const uint16_t *>(a.bias[v] + at);
+      const float s = bf16_bits_to_float(__ldg(sc + (c >> 2))), b = bf16_bits_to_float(__ldg(bi + (c >> 2)));
+      lo = dequant8_mlx(make_uint2(w.x, w.y), s, b);
+      hi = dequant8_mlx(make_uint2(w.z, w.w), s, b);
+    } else {
+      lo = convert8_s8(make_uint2(w.x, w.y));
+      hi = convert8_s8(make_uint2(w.z, w.w));
+    }
+    uint4 *dst = reinterpret_cast<uint4 *>(a.dst[v] + ((size_t)head * a.rows + row) * SH_D) + c * 2;
+    dst[0] = lo;
+    dst[1] = hi;
+  }
+}
+
+template <bool MLX>
+int launch_convert(const ShConvert &a, int requests, cudaStream_t st) {
+  const long long heads = (long long)requests * a.heads;
+  if (heads > 65535) return TSB_EUNSUPPORTED;
+  const dim3 grid((unsigned)((a.rows + SH_CV_ROWS - 1) / SH_CV_ROWS), (unsigned)heads, 2);
+  const cudaError_t e = launch_pdl(tree_attn_shared_convert_kernel<MLX>, grid, dim3(256), 0, st, a);
+  return e == cudaSuccess ? TSB_OK : TSB_ECUDA;
+}
+
 // ---------------------------------------------------------------- combine
-// out = sum_s w_s o_s, w_s = l_s 2^(m_s - m) / sum. Partials of empty splits
-// (l = 0) are not read. A warp per row: lane = 8 of the 256 columns.
+// out = sum_s w_s o_s, w_s = l_s 2^(m_s - m) / sum, over the prefix's splits and the
+// chunks that the request's length has. Partials with l = 0 are not read. A warp
+// per row, eight of the 256 columns per lane; bound by the partials' bytes (from L2).
 constexpr int SH_CB_WARPS = 4;
 
 __global__ void __launch_bounds__(SH_CB_WARPS * 32)
-tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_ml, int slots,
+tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_ml, int splits,
+                                const int32_t *__restrict__ lengths, int own_rows, int chunk_rows, int rows_per_b,
                                 int rows, uint16_t *__restrict__ out, float *__restrict__ lse) {
   griddep_wait();  // programmatic dependent: the partials are the attention kernel's
   griddep_launch_dependents();
   const int lane = threadIdx.x % 32;
   const int row = blockIdx.x * SH_CB_WARPS + threadIdx.x / 32;
   if (row >= rows) return;
+  const int slots = splits + ceil_to(own_rows_of(lengths, row / rows_per_b, own_rows), chunk_rows);
   const float2 *ml = reinterpret_cast<const float2 *>(part_ml) + row;
   float m = -INFINITY;
   for (int s = lane; s < slots; s += 32) {
@@ -613,11 +876,13 @@ tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *_
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     den += part;
-    for (int s = 0; s < min(32, slots - s0); ++s) {
+    const int n = min(32, slots - s0);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
       const float ws = __shfl_sync(0xffffffffu, w, s);
       if (ws == 0.f) continue;
       const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)(s0 + s) * rows + row) * SH_D) + lane;
-      const float4 x = src[0], y = src[32];
+      const float4 x = __ldg(src), y = __ldg(src + 32);
       acc[0] = fmaf(ws, x.x, acc[0]); acc[1] = fmaf(ws, x.y, acc[1]);
       acc[2] = fmaf(ws, x.z, acc[2]); acc[3] = fmaf(ws, x.w, acc[3]);
       acc[4] = fmaf(ws, y.x, acc[4]); acc[5] = fmaf(ws, y.y, acc[5]);
@@ -631,40 +896,65 @@ tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *_
   if (lse && lane == 0) lse[row] = den > 0.f ? (m + log2f(den)) * 0.69314718055994531f : -INFINITY;
 }
 
+// ---------------------------------------------------------------- plan
 struct ShPlan {
-  int rb_p, rb_o, splits_p, splits_o, tps_p, tps_o;
+  int rb_p, rb_o, splits, tps, items, chunk, chunks, pairs;
 };
 
-int split_tiles(int tiles, int units, int &tps) {
-  if (tiles <= 0) { tps = 0; return 0; }
-  int s = sm_count() / units;
-  s = std::min(std::min(s, tiles / 4), SH_MAX_SPLITS);
-  s = std::max(s, 1);
-  tps = (tiles + s - 1) / s;
-  return (tiles + tps - 1) / tps;
-}
-
 ShPlan plan_shared(int B, int T, int Hq, int Hkv, int P, int own_rows) {
-  ShPlan p;
-  const int R = (Hq / Hkv) * T;
-  p.rb_p = (int)(((long long)B * R + 127) / 128);
-  p.rb_o = (R + 127) / 128;
-  p.splits_p = split_tiles((P + SH_KT - 1) / SH_KT, Hkv * p.rb_p, p.tps_p);
-  p.splits_o = split_tiles((own_rows + SH_KT - 1) / SH_KT, B * Hkv * p.rb_o, p.tps_o);
+  ShPlan p = {};
+  const int pairs = std::max(1, sm_count() / 2), R = (Hq / Hkv) * T;
+  p.rb_p = (int)(((long long)B * R + SH_ROWS - 1) / SH_ROWS);
+  p.rb_o = (R + SH_ROWS - 1) / SH_ROWS;
+  // prefix: the number of key splits with the shortest longest pair
+  const int tiles = (P + SH_KT - 1) / SH_KT;
+  if (tiles > 0) {
+    const long long units = (long long)Hkv * p.rb_p;
+    long long best = -1;
+    for (int s = 1; s <= std::min(SH_MAX_SPLITS, std::max(1, tiles / 4)); ++s) {
+      const int tps = (tiles + s - 1) / s, n = (tiles + tps - 1) / tps;
+      const long long cost = ((units * n + pairs - 1) / pairs) * (tps + SH_SEG_COST);
+      if (best < 0 || cost < best) {
+        best = cost;
+        p.splits = n;
+        p.tps = tps;
+      }
+    }
+    p.items = (int)std::min(units * p.splits, 0x7fffffffLL);
+  }
+  // own rows: chunks small enough to even the pairs out, at most SH_MAX_CHUNKS a request
+  const int own_tiles = (own_rows + SH_KT - 1) / SH_KT;
+  const long long own_units = (long long)B * Hkv * p.rb_o;
+  p.chunk = SH_MIN_CHUNK;
+  if (own_tiles > 0) {
+    p.chunk = std::max(p.chunk, (own_tiles + SH_MAX_CHUNKS - 1) / SH_MAX_CHUNKS);
+    p.chunk = std::max(p.chunk, (int)std::min<long long>(own_tiles, own_units * own_tiles / (2LL * pairs)));
+    p.chunks = (own_tiles + p.chunk - 1) / p.chunk;
+  }
+  p.pairs = (int)std::min<long long>(pairs, (long long)p.items + own_units * p.chunks);
   return p;
 }
 
 bool sizes_ok(int B, int T, int Hq, int Hkv, int P, int own_rows) {
-  return B > 0 && T > 0 && Hq > 0 && Hkv > 0 && P >= 0 && own_rows >= 0 && (long long)B * Hq * T <= (1 << 24);
+  return B > 0 && T > 0 && Hq > 0 && Hkv > 0 && P >= 0 && own_rows >= 0 && (long long)B * Hq * T <= (1 << 22);
 }
 
-template <int FMT>
-int launch_fmt(const CUtensorMap *maps, const ShArgs &a, int ctas, cudaStream_t st) {
-  using C = ShCfg<FMT>;
-  if (cudaFuncSetAttribute(tree_attn_shared_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM) !=
-      cudaSuccess)
+// Bytes of the workspace's parts: partials, then (8-bit formats) the bf16 copies.
+size_t partial_bytes(const ShPlan &p, int B, int T, int Hq) {
+  const size_t n = (size_t)(p.splits + p.chunks) * B * Hq * T * (SH_D + 2) * sizeof(float);
+  return (n + 255) & ~size_t(255);
+}
+size_t copy_bytes(int B, int Hkv, int P, int own_rows) {  // of K or of V
+  return ((size_t)Hkv * P + (size_t)B * Hkv * own_rows) * SH_D * 2;
+}
+
+template <bool SCALED>
+int launch_attn(const CUtensorMap *maps, const ShArgs &a, int pairs, cudaStream_t st) {
+  using C = ShCfg<SCALED>;
+  if (cudaFuncSetAttribute(tree_attn_shared_kernel<SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)C::SMEM) != cudaSuccess)
     return TSB_ECUDA;
-  const cudaError_t e = launch_pdl(tree_attn_shared_kernel<FMT>, dim3((unsigned)ctas), dim3(C::THREADS),
+  const cudaError_t e = launch_pdl(tree_attn_shared_kernel<SCALED>, dim3((unsigned)pairs * 2), dim3(C::THREADS),
                                    (size_t)C::SMEM, st, maps[0], maps[1], maps[2], maps[3], a);
   return e == cudaSuccess ? TSB_OK : TSB_ECUDA;
 }
@@ -698,11 +988,12 @@ unsigned int status_attn_shared(bool reset) {
 
 using namespace tsb;
 
-extern "C" size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows) {
+extern "C" size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows,
+                                                       int kv_format) {
   (void)D;
   if (!sizes_ok(B, T, Hq, Hkv, P, own_rows) || Hq % Hkv) return 0;
-  const ShPlan p = plan_shared(B, T, Hq, Hkv, P, own_rows);
-  return (size_t)(p.splits_p + p.splits_o) * B * Hq * T * (SH_D + 2) * sizeof(float);
+  const size_t n = partial_bytes(plan_shared(B, T, Hq, Hkv, P, own_rows), B, T, Hq);
+  return kv_format == TSB_KV_BF16 ? n : n + 2 * copy_bytes(B, Hkv, P, own_rows);
 }
 
 extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride_h, long long q_stride_t,
@@ -723,24 +1014,57 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   if (!(scale > 0.f)) return TSB_EUNSUPPORTED;  // the kernel takes row maxima of unscaled scores
   if (!aligned(q, 16) || q_stride_b % 8 || q_stride_h % 8 || q_stride_t % 8) return TSB_EINVAL;
   if (!aligned(out, 16) || !aligned(lse, 4)) return TSB_EINVAL;
-  int st = check_source(kv_format, prefix, P > 0);
-  if (st == TSB_OK) st = check_source(kv_format, own, own_rows > 0);
-  if (st != TSB_OK) return st;
+  const tsb_kv_t *srcs[2] = {prefix, own};
+  for (int i = 0; i < 2; ++i) {
+    const int st = check_source(kv_format, srcs[i], srcs[i]->rows > 0);
+    if (st != TSB_OK) return st;
+  }
   if ((long long)Hkv * prefix->capacity > 0x7fffffc0LL || (long long)B * Hkv * own->capacity > 0x7fffffc0LL)
     return TSB_EUNSUPPORTED;  // tensor-map row coordinates are 32-bit
-  const size_t need = tsb_tree_attn_shared_workspace_bytes(B, T, Hq, Hkv, D, P, own_rows);
+  if (kv_format != TSB_KV_BF16 && (long long)B * Hkv > 65535) return TSB_EUNSUPPORTED;  // the converting grid
+  const ShPlan p = plan_shared(B, T, Hq, Hkv, P, own_rows);
+  const size_t part = partial_bytes(p, B, T, Hq);
+  const size_t need = tsb_tree_attn_shared_workspace_bytes(B, T, Hq, Hkv, D, P, own_rows, kv_format);
   if (need && (!ws || ws_bytes < need)) return TSB_EWORKSPACE;
   if (!aligned(ws, 16)) return TSB_EINVAL;
 
-  const ShPlan p = plan_shared(B, T, Hq, Hkv, P, own_rows);
   const size_t rows = (size_t)B * Hq * T;
-  const int slots = p.splits_p + p.splits_o;
+  cudaStream_t stm = (cudaStream_t)stream;
   ShArgs a = {};
-  const tsb_kv_t *srcs[2] = {prefix, own};
-  for (int i = 0; i < 2; ++i)
-    a.src[i] = ShSource{reinterpret_cast<const unsigned char *>(srcs[i]->k),
-                        reinterpret_cast<const unsigned char *>(srcs[i]->v), srcs[i]->k_scales, srcs[i]->k_biases,
-                        srcs[i]->v_scales, srcs[i]->v_biases, srcs[i]->capacity, srcs[i]->rows};
+  CUtensorMap maps[4] = {};
+  // the bf16 rows to attend to: the caches themselves, or copies of them
+  char *copy = (char *)ws + part;
+  for (int i = 0; i < 2; ++i) {
+    const tsb_kv_t *c = srcs[i];
+    const int requests = i ? B : 1;
+    const void *kv[2] = {c->k, c->v};
+    int cap = c->capacity;
+    if (kv_format != TSB_KV_BF16 && c->rows > 0) {
+      ShConvert cv = {};
+      const size_t bytes = (size_t)requests * Hkv * c->rows * SH_D * 2;
+      const void *scales[2] = {c->k_scales, c->v_scales}, *biases[2] = {c->k_biases, c->v_biases};
+      for (int v = 0; v < 2; ++v) {
+        cv.src[v] = (const unsigned char *)kv[v];
+        cv.scale[v] = (const uint2 *)scales[v];
+        cv.bias[v] = (const uint2 *)biases[v];
+        cv.dst[v] = (uint16_t *)(copy + v * bytes);
+        kv[v] = cv.dst[v];
+      }
+      copy += 2 * bytes;
+      cv.lengths = i ? lengths : nullptr;
+      cv.heads = Hkv;
+      cv.cap = cap;
+      cv.rows = cap = c->rows;
+      const int e = kv_format == TSB_KV_MLX_Q8_G64 ? launch_convert<true>(cv, requests, stm) : launch_convert<false>(cv, requests, stm);
+      if (e != TSB_OK) return e;
+    }
+    a.src[i] = ShSource{(const float *)c->k_scales, (const float *)c->v_scales, c->capacity, cap, c->rows};
+    for (int v = 0; v < 2 && c->rows > 0; ++v)
+      if (make_tmap_2d(&maps[2 * i + v], kv[v], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, SH_D,
+                       (uint64_t)requests * Hkv * cap, SH_D * 2, 64, v ? SH_KT : SH_KT / 2,
+                       CU_TENSOR_MAP_SWIZZLE_128B) != TSB_OK)
+        return TSB_ECUDA;
+  }
   a.q = (const uint16_t *)q;
   a.q_sb = q_stride_b;
   a.q_sh = q_stride_h;
@@ -750,36 +1074,19 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   a.lengths = lengths;
   a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.tail = tail;
   a.rb_p = p.rb_p; a.rb_o = p.rb_o;
-  a.splits_p = p.splits_p; a.splits_o = p.splits_o;
-  a.tps_p = p.tps_p; a.tps_o = p.tps_o;
-  a.ctas_p = Hkv * p.rb_p * p.splits_p;
+  a.splits = p.splits; a.tps = p.tps; a.items = p.items;
+  a.chunk = p.chunk; a.chunks = p.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part_o = (float *)ws;
-  a.part_ml = a.part_o + (size_t)slots * rows * SH_D;
-  const long long ctas = (long long)a.ctas_p + (long long)B * Hkv * p.rb_o * p.splits_o;
-  if (ctas > 0x7fffffffLL) return TSB_EUNSUPPORTED;
-  cudaStream_t stm = (cudaStream_t)stream;
-  if (ctas > 0) {
-    CUtensorMap maps[4] = {};
-    if (kv_format == TSB_KV_BF16) {
-      for (int i = 0; i < 2; ++i) {
-        if (!(i ? own_rows : P)) continue;
-        const uint64_t n = (uint64_t)(i ? B : 1) * Hkv * srcs[i]->capacity;
-        for (int v = 0; v < 2; ++v)
-          if (make_tmap_2d(&maps[2 * i + v], v ? srcs[i]->v : srcs[i]->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, SH_D, n,
-                           SH_D * 2, 64, SH_KT, CU_TENSOR_MAP_SWIZZLE_128B) != TSB_OK)
-            return TSB_ECUDA;
-      }
-    }
-    int e;
-    if (kv_format == TSB_KV_BF16) e = launch_fmt<TSB_KV_BF16>(maps, a, (int)ctas, stm);
-    else if (kv_format == TSB_KV_MLX_Q8_G64) e = launch_fmt<TSB_KV_MLX_Q8_G64>(maps, a, (int)ctas, stm);
-    else e = launch_fmt<TSB_KV_REF_Q8_ROW>(maps, a, (int)ctas, stm);
+  a.part_ml = a.part_o + (size_t)(p.splits + p.chunks) * rows * SH_D;
+  if (p.pairs > 0) {
+    const int e = kv_format == TSB_KV_REF_Q8_ROW ? launch_attn<true>(maps, a, p.pairs, stm)
+                                                 : launch_attn<false>(maps, a, p.pairs, stm);
     if (e != TSB_OK) return e;
   }
   const cudaError_t e =
       launch_pdl(tree_attn_shared_combine_kernel, dim3((unsigned)((rows + SH_CB_WARPS - 1) / SH_CB_WARPS)),
-                 dim3(SH_CB_WARPS * 32), 0, stm, (const float *)a.part_o, (const float *)a.part_ml, slots, (int)rows,
-                 (uint16_t *)out, lse);
+                 dim3(SH_CB_WARPS * 32), 0, stm, (const float *)a.part_o, (const float *)a.part_ml, p.splits, lengths,
+                 own_rows, p.chunk * SH_KT, Hq * T, (int)rows, (uint16_t *)out, lse);
   return e == cudaSuccess ? TSB_OK : TSB_ECUDA;
 }

@@ -382,7 +382,7 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
     lse = torch.empty((bsz, hq, n), dtype=torch.float32, device=dev) if stats else None
     lib = _lib.load()
     # a workspace of this call's own: calls on other streams and captured graphs share nothing
-    ws = torch.empty(lib.tsb_tree_attn_shared_workspace_bytes(bsz, n, hq, hkv, d, pre.rows, own.rows),
+    ws = torch.empty(lib.tsb_tree_attn_shared_workspace_bytes(bsz, n, hq, hkv, d, pre.rows, own.rows, fmt),
                      dtype=torch.uint8, device=dev)
     st = lib.tsb_tree_attn_shared(_ptr(q), q.stride(0), q.stride(1), q.stride(2), fmt, ctypes.byref(pre),
                                   ctypes.byref(own), _ptr(lengths), _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, tail_v,
