@@ -101,7 +101,7 @@ struct ShArgs {
   int B, T, Hq, Hkv, tail;
   int rb_p, rb_o;   // row blocks of a KV head's prefix rows / of a request's rows
   int splits, tps;  // prefix: key splits, tiles per split
-  int items;        // prefix segments: Hkv * splits * rb_p
+  int items, more;  // prefix segments: Hkv * splits * rb_p; how many pairs have one more than the others
   int chunk;        // own: tiles per chunk
   int chunks;       // the most chunks a request has
   float scale_log2;
@@ -188,41 +188,15 @@ TSB_HD uint32_t cluster_addr(const void *p, uint32_t rank) {
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr(p)), "r"(rank));
   return r;
 }
+// Arrivals on a barrier of either CTA. What they announce is read by MMAs alone
+// (tiles, P and O), behind the writer's own proxy and tcgen05 fences, so the barrier
+// need not order ordinary accesses across the cluster: a cluster-scope release per
+// arrival cost ~500 cycles, twice a tile.
 TSB_HD void cluster_arrive_on(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 TSB_HD void cluster_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-               : "memory");
-}
-TSB_HD bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_addr(bar)), "r"(parity), "r"(kSuspendHintNs)
-      : "memory");
-  return ok != 0;
-}
-// warp_wait for a barrier that the other CTA arrives on, too.
-TSB_HD bool warp_wait_cluster(uint64_t *bar, uint32_t parity) {
-  bool ok = mbar_try_wait_cluster(bar, parity);
-  if (!ok) {
-    const unsigned long long t0 = globaltimer_ns();
-    for (uint32_t it = 1; !ok; ++it) {
-      ok = mbar_try_wait_cluster(bar, parity);
-      if (!ok && (it & 15u) == 0) {
-        if (*(volatile unsigned int *)&g_device_status != 0u) break;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
-          record_status(TSB_ETIMEOUT);
-          break;
-        }
-      }
-    }
-  }
-  return __all_sync(0xffffffffu, ok) != 0;
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 TSB_HD void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -361,15 +335,15 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       total += sSum[w];
     }
     // pairs with one prefix segment more carry that much less of the rest
-    const long long G = pairs, more = a.items % G;
+    const long long G = pairs, more = a.more;
     const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk + SH_SEG_COST);
     const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
     const long long q_more = all > need ? all - need : 0;
     const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
-    const double sum = (double)(more * q_more + (G - more) * q_less);
-    auto start = [&](long long i) -> int {
-      const long long q = min(i, more) * q_more + max(i - more, 0ll) * q_less;
-      return i == G ? total : (int)((double)total * ((double)q / sum));
+    const double per_q = (double)total / (double)(more * q_more + (G - more) * q_less);
+    auto start = [&](int i) -> int {
+      const long long q = min((long long)i, more) * q_more + max(i - more, 0ll) * q_less;
+      return i == pairs ? total : min((int)((double)q * per_q), total);
     };
     const int w0 = start(pair), w1 = start(pair + 1);
     if (w1 > w0 && w0 >= before && w0 < before + mine) {
@@ -491,12 +465,12 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       int g = 0, seg = 0;
       bool ok = true;
       while (ok && walk.next(sg)) {
-        ok = warp_wait_cluster(q_full, seg & 1);
+        ok = warp_wait(q_full, seg & 1);
         ++seg;
         for (int j = 0; j < sg.nt && ok; ++j, ++g) {
           const int s = g % NK, sb = g & 1;
-          ok = warp_wait_cluster(&k_full[s], (g / NK) & 1);
-          if (ok && g >= 2) ok = warp_wait_cluster(&s_free[sb], ((g >> 1) - 1) & 1);
+          ok = warp_wait(&k_full[s], (g / NK) & 1);
+          if (ok && g >= 2) ok = warp_wait(&s_free[sb], ((g >> 1) - 1) & 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -519,12 +493,12 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       int g = 0, seg = 0;
       bool ok = true;
       while (ok && walk.next(sg)) {
-        if (seg > 0) ok = warp_wait_cluster(o_free, (seg - 1) & 1);  // the last segment's O has been read
+        if (seg > 0) ok = warp_wait(o_free, (seg - 1) & 1);  // the last segment's O has been read
         ++seg;
         for (int j = 0; j < sg.nt && ok; ++j, ++g) {
           const int s = g % NV, pb = g & 1;
-          ok = warp_wait_cluster(&v_full[s], (g / NV) & 1);
-          if (ok) ok = warp_wait_cluster(&p_full[pb], (g >> 1) & 1);
+          ok = warp_wait(&v_full[s], (g / NV) & 1);
+          if (ok) ok = warp_wait(&p_full[pb], (g >> 1) & 1);
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
@@ -567,16 +541,36 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       head = s.kh * G + rr / a.T;
       node = rr % a.T;
     };
+    // A warp's own 32 rows of its P buffer, 4 KB: nobody else touches them, and between
+    // segments (after the last P V) no MMA reads them. Rows of 128 bytes pass through it
+    // on their way between memory, where eight lanes have 16 bytes each of a row, and
+    // TMEM, where a lane has a row: a lane reading its own row alone took ~8000 cycles
+    // a segment for Q and as many for O.
+    unsigned char *const stage = sP + odd * SH_P_BYTES + q * 4096;
+    const int s_row = lane >> 3, s_ch = lane & 7;  // this lane's row (of four at a time) and 16-byte chunk
+    auto stage_at = [&](int row, int ch) { return reinterpret_cast<uint4 *>(stage + row * 128 + ((ch ^ (row & 7)) << 4)); };
     // Q row -> TMEM lane r, columns SH_Q + d/2 (the A-operand layout of a K-major
     // M=128 tile), half of D per warp. All S of the segment before are complete.
     auto load_q = [&]() {
-      const uint4 *qrow = reinterpret_cast<const uint4 *>(a.q + rq * a.q_sb + head * a.q_sh + node * a.q_st) + odd * 16;
+      const long long off = row_valid ? rq * a.q_sb + head * a.q_sh + node * a.q_st + odd * 128 : -1ll;
+      uint4 v[2][8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const long long o = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
+#pragma unroll
+        for (int bx = 0; bx < 2; ++bx)
+          v[bx][i] = o >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + o + bx * 64) + s_ch) : make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
       for (int bx = 0; bx < 2; ++bx) {
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *stage_at(i * 4 + s_row, s_ch) = v[bx][i];
+        __syncwarp();
         uint32_t qv[32];
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-          const uint4 u = row_valid ? __ldg(qrow + bx * 8 + c) : make_uint4(0u, 0u, 0u, 0u);
+          const uint4 u = *stage_at(lane, c);
           qv[4 * c] = u.x; qv[4 * c + 1] = u.y; qv[4 * c + 2] = u.z; qv[4 * c + 3] = u.w;
         }
         tmem_st32(lane_base + SH_Q + odd * 64 + bx * 32, qv);
@@ -753,18 +747,28 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       }
       const size_t prow = (size_t)done.slot * rows_all + orow;
       const float inv = sum > 0.f ? 1.f / sum : 0.f;
+      const long long off = valid ? (long long)(prow * SH_D + odd * 128) : -1ll;
 #pragma unroll 1
       for (int c = 0; c < SH_D / 2; c += 32) {
         uint32_t o[32];
         tmem_ld32(lane_base + SH_O + odd * 128 + c, o);
         tmem_wait_ld();
-        if (!valid) continue;
-        float4 *dst = reinterpret_cast<float4 *>(a.part_o + prow * SH_D + odd * 128 + c);
+        __syncwarp();
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          dst[e] = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                               __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+        for (int e = 0; e < 8; ++e) {
+          float4 f = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+          *reinterpret_cast<float4 *>(stage_at(lane, e)) = f;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
+          const uint4 u = *stage_at(i * 4 + s_row, s_ch);
+          if (at >= 0) *(reinterpret_cast<uint4 *>(a.part_o + at + c) + s_ch) = u;
+        }
       }
+      __syncwarp();  // the stage is P's again
       tc_fence_before();
       __syncwarp();
       if (lane == 0) cluster_arrive_on(o_free0);
@@ -1075,6 +1079,7 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   a.B = B; a.T = T; a.Hq = Hq; a.Hkv = Hkv; a.tail = tail;
   a.rb_p = p.rb_p; a.rb_o = p.rb_o;
   a.splits = p.splits; a.tps = p.tps; a.items = p.items;
+  a.more = p.pairs ? p.items % p.pairs : 0;
   a.chunk = p.chunk; a.chunks = p.chunks;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part_o = (float *)ws;
