@@ -69,7 +69,9 @@ constexpr int SH_SOFT0 = 4, SH_NSOFT = 8;    // softmax warps
 constexpr int SH_MAX_SPLITS = 64;            // key splits of a prefix unit
 constexpr int SH_MAX_CHUNKS = 16;            // chunks of a request's own rows
 constexpr int SH_MIN_CHUNK = 4;              // tiles
-constexpr int SH_SEG_COST = 3;               // what a segment costs beside its tiles, in tiles
+// What a segment costs beside its tiles (Q in, partials out, ~9000 cycles of ~1060 a
+// tile), and an own tile in units of a prefix tile (shorter runs, masks, cold rows).
+constexpr int SH_SEG_COST = 9, SH_OWN_COST = 2;
 
 template <bool SCALED>
 struct ShCfg {
@@ -336,7 +338,7 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
     }
     // pairs with one prefix segment more carry that much less of the rest
     const long long G = pairs, more = a.more;
-    const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk + SH_SEG_COST);
+    const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk * SH_OWN_COST + SH_SEG_COST);
     const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
     const long long q_more = all > need ? all - need : 0;
     const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
@@ -529,7 +531,6 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
     // A wait that ran out (never in a healthy run) is not followed by others, but the
     // barriers among the warps go on: nobody waits for a warp that has left.
     bool ok = true;
-    bool more = walk.next(sg);
     // the row of a segment that this thread has
     int rq = 0, head = 0, node = 0;
     bool row_valid = false;
@@ -551,41 +552,104 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
     auto stage_at = [&](int row, int ch) { return reinterpret_cast<uint4 *>(stage + row * 128 + ((ch ^ (row & 7)) << 4)); };
     // Q row -> TMEM lane r, columns SH_Q + d/2 (the A-operand layout of a K-major
     // M=128 tile), half of D per warp. All S of the segment before are complete.
-    auto load_q = [&]() {
-      const long long off = row_valid ? rq * a.q_sb + head * a.q_sh + node * a.q_st + odd * 128 : -1ll;
-      uint4 v[2][8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const long long o = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
-#pragma unroll
-        for (int bx = 0; bx < 2; ++bx)
-          v[bx][i] = o >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + o + bx * 64) + s_ch) : make_uint4(0u, 0u, 0u, 0u);
-      }
-#pragma unroll
-      for (int bx = 0; bx < 2; ++bx) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) *stage_at(i * 4 + s_row, s_ch) = v[bx][i];
-        __syncwarp();
-        uint32_t qv[32];
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 u = *stage_at(lane, c);
-          qv[4 * c] = u.x; qv[4 * c + 1] = u.y; qv[4 * c + 2] = u.z; qv[4 * c + 3] = u.w;
-        }
-        tmem_st32(lane_base + SH_Q + odd * 64 + bx * 32, qv);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) cluster_arrive_on(q_full0);
-    };
-    if (more) {
-      place(sg);
-      load_q();
-    }
     int masks_of = -1;  // the request whose node masks are in sBits
-    while (more) {
+    float m_l = -INFINITY, l = 0.f;  // the sum over this warp's tiles, relative to the reference m_l
+    bool had = false, had_rows = false;  // the segment before: its partial is still to be written
+    int had_slots = 0;
+    size_t had_row = 0;
+    bool had_valid = false;
+    for (;;) {
+      const bool more = walk.next(sg);
+      float sum = 0.f, m_ref = -INFINITY;
+      if (had) {
+        // All S of the segment before are complete once P V of its last tile is. A warp
+        // follows its own buffer's barriers phase by phase; the other buffer's are looked
+        // at only when the phase before is known to be over.
+        const int last = g - 1;
+        if (last >= 1) ok = ok && warp_wait(&pv_done[(last - 1) & 1], ((last - 1) >> 1) & 1);
+        ok = ok && warp_wait(&pv_done[last & 1], (last >> 1) & 1);
+        tc_fence_after();
+        named_barrier_sync(bar_rows, 64);  // the last tile has settled the reference
+        m_ref = sRef[r];
+        sRow[odd * 128 + r] = l * (m_l == -INFINITY ? 0.f : ex2(m_l - m_ref));
+        named_barrier_sync(bar_rows, 64);
+        sum = sRow[r] + sRow[128 + r];
+        named_barrier_sync(bar_rows, 64);
+      }
+      // ---- the next segment's Q: its S can start
+      bool any_row = false;
+      if (more) {
+        place(sg);
+        any_row = __any_sync(0xffffffffu, row_valid);
+        if (any_row) {  // else whatever Q is in TMEM: nobody reads what comes of it
+          const long long off = row_valid ? rq * a.q_sb + head * a.q_sh + node * a.q_st + odd * 128 : -1ll;
+          uint4 qv[2][8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const long long o = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
+#pragma unroll
+            for (int bx = 0; bx < 2; ++bx)
+              qv[bx][i] = o >= 0 ? __ldg(reinterpret_cast<const uint4 *>(a.q + o + bx * 64) + s_ch) : make_uint4(0u, 0u, 0u, 0u);
+          }
+#pragma unroll
+          for (int bx = 0; bx < 2; ++bx) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) *stage_at(i * 4 + s_row, s_ch) = qv[bx][i];
+            __syncwarp();
+            uint32_t w[32];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const uint4 u = *stage_at(lane, c);
+              w[4 * c] = u.x; w[4 * c + 1] = u.y; w[4 * c + 2] = u.z; w[4 * c + 3] = u.w;
+            }
+            tmem_st32(lane_base + SH_Q + odd * 64 + bx * 32, w);
+          }
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) cluster_arrive_on(q_full0);
+      }
+      // ---- the partial of the segment before, normalised
+      if (had) {
+        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const long long off = had_valid ? (long long)(had_row * SH_D + odd * 128) : -1ll;
+#pragma unroll 1
+        for (int c = 0; c < SH_D / 2 && had_rows; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(lane_base + SH_O + odd * 128 + c, o);
+          tmem_wait_ld();
+          __syncwarp();
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float4 f = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
+                                   __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
+            *reinterpret_cast<float4 *>(stage_at(lane, e)) = f;
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const long long at = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
+            const uint4 u = *stage_at(i * 4 + s_row, s_ch);
+            if (at >= 0) *(reinterpret_cast<uint4 *>(a.part_o + at + c) + s_ch) = u;
+          }
+        }
+        tc_fence_before();
+        __syncwarp();  // the stage is P's again
+        if (lane == 0) cluster_arrive_on(o_free0);
+        if (had_valid && odd == 0) {
+          float2 *ml = reinterpret_cast<float2 *>(a.part_ml);
+          ml[had_row] = make_float2(m_ref, sum);  // sum 0: nothing visible, the partial is not read
+          for (int s = 1; s < had_slots; ++s) ml[had_row + s * rows_all] = make_float2(-INFINITY, 0.f);
+        }
+      }
+      if (!more) break;
+      had = true;
+      had_rows = any_row;
+      had_valid = row_valid;
+      had_slots = sg.slots;
+      had_row = (size_t)sg.slot * rows_all + ((size_t)rq * a.Hq + head) * a.T + node;
       if (sg.own && masks_of != sg.b) {  // node masks, from the parent array or given; the rows' two warps have their own
         masks_of = sg.b;
         const int st = odd * 32 + lane;
@@ -612,7 +676,8 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         named_barrier_sync(bar_rows, 64);
       }
       const unsigned long long mybits = sg.own ? sBits[q * 64 + node] : 0ull;
-      float m_l = -INFINITY, l = 0.f;  // the sum over this warp's tiles, relative to the reference m_l
+      m_l = -INFINITY;
+      l = 0.f;
       const int g0 = g, g1 = g + sg.nt;
       for (g = g0 + ((g0 & 1) ^ odd); g < g1; g += 2) {
         const int j = g - g0;
@@ -722,61 +787,6 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         }
       }
       g = g1;
-      // ---- the next segment's Q (its S can start), then this one's partials. All of
-      // this segment's S are complete only once its last tile's have been seen.
-      const ShSegment done = sg;
-      const bool valid = row_valid;
-      const size_t orow = ((size_t)rq * a.Hq + head) * a.T + node;
-      const int last = g1 - 1;
-      // A warp follows its own buffer's barriers phase by phase; the other buffer's are
-      // looked at only when the phase before is known to be over.
-      if ((last & 1) != odd && last >= 1) ok = ok && warp_wait(&pv_done[odd], ((last - 1) >> 1) & 1);
-      if ((last & 1) == odd && last >= 1) ok = ok && warp_wait(&pv_done[odd ^ 1], ((last - 1) >> 1) & 1);
-      ok = ok && warp_wait(&pv_done[last & 1], (last >> 1) & 1);  // P V of the last tile, after which no S of it runs
-      tc_fence_after();
-      named_barrier_sync(bar_rows, 64);  // the last tile has settled the reference
-      const float m = sRef[r];
-      sRow[odd * 128 + r] = l * (m_l == -INFINITY ? 0.f : ex2(m_l - m));
-      named_barrier_sync(bar_rows, 64);
-      const float sum = sRow[r] + sRow[128 + r];
-      named_barrier_sync(bar_rows, 64);
-      more = walk.next(sg);
-      if (more) {
-        place(sg);
-        load_q();
-      }
-      const size_t prow = (size_t)done.slot * rows_all + orow;
-      const float inv = sum > 0.f ? 1.f / sum : 0.f;
-      const long long off = valid ? (long long)(prow * SH_D + odd * 128) : -1ll;
-#pragma unroll 1
-      for (int c = 0; c < SH_D / 2; c += 32) {
-        uint32_t o[32];
-        tmem_ld32(lane_base + SH_O + odd * 128 + c, o);
-        tmem_wait_ld();
-        __syncwarp();
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float4 f = make_float4(__uint_as_float(o[4 * e]) * inv, __uint_as_float(o[4 * e + 1]) * inv,
-                                 __uint_as_float(o[4 * e + 2]) * inv, __uint_as_float(o[4 * e + 3]) * inv);
-          *reinterpret_cast<float4 *>(stage_at(lane, e)) = f;
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const long long at = __shfl_sync(0xffffffffu, off, i * 4 + s_row);
-          const uint4 u = *stage_at(i * 4 + s_row, s_ch);
-          if (at >= 0) *(reinterpret_cast<uint4 *>(a.part_o + at + c) + s_ch) = u;
-        }
-      }
-      __syncwarp();  // the stage is P's again
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) cluster_arrive_on(o_free0);
-      if (valid && odd == 0) {
-        float2 *ml = reinterpret_cast<float2 *>(a.part_ml);
-        ml[prow] = make_float2(m, sum);  // sum 0: nothing visible, the partial is not read
-        for (int s = 1; s < done.slots; ++s) ml[prow + s * rows_all] = make_float2(-INFINITY, 0.f);
-      }
     }
   }
   tc_fence_before();
