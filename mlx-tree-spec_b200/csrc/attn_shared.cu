@@ -46,6 +46,7 @@
 // Rows at or past a cache's valid rows never reach the output, whatever they hold
 // (even NaN): their scores are masked and their V rows are zero in shared memory.
 #include <algorithm>
+#include <atomic>
 
 #include "attn_tile.cuh"
 
@@ -76,12 +77,12 @@ constexpr int SH_SEG_COST = 9, SH_OWN_COST = 2;
 template <bool SCALED>
 struct ShCfg {
   static constexpr int SC_BYTES = SCALED ? SH_NSC * 2 * SH_KT * 4 : 0;
-  static constexpr int NBARS = 2 * SH_NK + 2 * SH_NV + 11 + (SCALED ? 2 * SH_NSC : 0);
+  static constexpr int NBARS = 2 * SH_NK + 2 * SH_NV + 12 + (SCALED ? 2 * SH_NSC : 0);
   static constexpr int CTRL = 6144;  // barriers, TMEM address, schedule, masks of each warp pair, row exchange
   static constexpr int THREADS = 384;
   static constexpr size_t SMEM =
       (size_t)SH_NK * SH_K_BYTES + (size_t)SH_NV * SH_V_BYTES + 2 * SH_P_BYTES + SC_BYTES + CTRL + 1024;
-  static_assert((NBARS + 20) * 8 + 4 * 64 * (8 + 4) + 3 * 128 * 4 <= CTRL, "control block");
+  static_assert((NBARS + 4) * 8 + 4 * 64 * (8 + 4) + 3 * 128 * 4 <= CTRL, "control block");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -116,9 +117,9 @@ TSB_HD int own_rows_of(const int32_t *lengths, int b, int most) {
 }
 TSB_HD int ceil_to(int a, int b) { return (a + b - 1) / b; }
 
-// A pair's share of the own chunks: `left` chunks from (b, u, ch) on.
+// A pair's share of the own chunks: `left` chunks from (b, u, ch) on; len = b's rows.
 struct ShShare {
-  int b, u, ch, left;
+  int b, u, ch, left, len;
 };
 
 struct ShSegment {
@@ -129,15 +130,17 @@ struct ShSegment {
   int n_kv, tail_lo;   // keys, and where the tree rule begins
 };
 
-// Walks a pair's segments; every role does so by itself.
+// Walks a pair's segments; every role does so by itself. The share of the own chunks
+// is looked at when the prefix segments are done: it is found meanwhile.
 struct ShWalk {
   const ShArgs &a;
+  const ShShare *share;
+  uint64_t *ready;
   int item, step, len;
+  bool waiting;
   ShShare w;
-  TSB_HD ShWalk(const ShArgs &args, const ShShare &share, int pair, int pairs)
-      : a(args), item(pair), step(pairs), len(0), w(share) {
-    if (w.left > 0) len = own_rows_of(a.lengths, w.b, a.src[1].rows);
-  }
+  TSB_HD ShWalk(const ShArgs &args, const ShShare *sh, uint64_t *bar, int pair, int pairs)
+      : a(args), share(sh), ready(bar), item(pair), step(pairs), len(0), waiting(true), w{0, 0, 0, 0, 0} {}
   TSB_HD bool next(ShSegment &s) {
     if (item < a.items) {
       s.own = false;
@@ -152,6 +155,11 @@ struct ShWalk {
       s.slots = 1;
       item += step;
       return true;
+    }
+    if (waiting) {
+      waiting = false;
+      if (mbar_wait(ready, 0)) w = *share;
+      len = w.len;
     }
     while (w.left > 0) {
       const int tiles = ceil_to(len, SH_KT), n = ceil_to(tiles, a.chunk);
@@ -280,11 +288,11 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
   // in both CTAs: commits of the MMAs
   uint64_t *k_free = o_free + 1, *v_free = k_free + NK, *s_full = v_free + NV, *pv_done = s_full + 2;
   uint64_t *v_last = pv_done + 2;                       // a CTA's own: a V tile with rows past the end
-  uint64_t *sc_full = v_last + 1, *sc_free = sc_full + SH_NSC;  // row scales
+  uint64_t *share_ready = v_last + 1;
+  uint64_t *sc_full = share_ready + 1, *sc_free = sc_full + SH_NSC;  // row scales
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + C::NBARS);
-  ShShare *sShare = reinterpret_cast<ShShare *>(bars + C::NBARS + 2);
-  int *sSum = reinterpret_cast<int *>(bars + C::NBARS + 4);                                      // [<= 32 warps]
-  unsigned long long *sBits = reinterpret_cast<unsigned long long *>(bars + C::NBARS + 4 + 16);  // [4][T <= 64]
+  ShShare *sShare = reinterpret_cast<ShShare *>(tmem_slot + 1);
+  unsigned long long *sBits = reinterpret_cast<unsigned long long *>(bars + C::NBARS + 4);  // [4][T <= 64]
   int32_t *sPar = reinterpret_cast<int32_t *>(sBits + 4 * 64);                                   // [4][T <= 64]
   float *sRow = reinterpret_cast<float *>(sPar + 4 * 64);                                        // [2][128]
   float *sRef = sRow + 2 * 128;                                                                  // [128]
@@ -303,68 +311,20 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
     mbar_init(q_full, 2 * SH_NSOFT);
     mbar_init(o_free, 2 * SH_NSOFT);
     mbar_init(v_last, 1);
+    mbar_init(share_ready, 1);
     if (SCALED)
       for (int i = 0; i < SH_NSC; ++i) { mbar_init(&sc_full[i], 32); mbar_init(&sc_free[i], SH_NSOFT / 2); }
     fence_mbar_init();
     fence_proxy_async_smem();
   }
   if (warp == 0) pair_tmem_alloc(tmem_slot, 512);
-  griddep_wait();  // programmatic dependent: q, the caches and the lengths are the previous kernels'
-
-  // ---- this pair's share of the own chunks. A thread adds up a run of requests.
-  {
-    const int per = ceil_to(a.B, C::THREADS);
-    const int b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
-    const int units = a.Hkv * a.rb_o;
-    auto chunks_of = [&](int b) {
-      return ceil_to(ceil_to(own_rows_of(a.lengths, b, a.src[1].rows), SH_KT), a.chunk) * units;
-    };
-    int mine = 0;
-    if (a.src[1].rows > 0)
-      for (int b = b0; b < b1; ++b) mine += chunks_of(b);
-    int up = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += v;
-    }
-    if (lane == 31) sSum[warp] = up;
-    if (threadIdx.x == 0) *sShare = ShShare{0, 0, 0, 0};
-    __syncthreads();
-    int before = up - mine, total = 0;
-    for (int w = 0; w < C::THREADS / 32; ++w) {
-      if (w < warp) before += sSum[w];
-      total += sSum[w];
-    }
-    // pairs with one prefix segment more carry that much less of the rest
-    const long long G = pairs, more = a.more;
-    const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk * SH_OWN_COST + SH_SEG_COST);
-    const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
-    const long long q_more = all > need ? all - need : 0;
-    const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
-    const double per_q = (double)total / (double)(more * q_more + (G - more) * q_less);
-    auto start = [&](int i) -> int {
-      const long long q = min((long long)i, more) * q_more + max(i - more, 0ll) * q_less;
-      return i == pairs ? total : min((int)((double)q * per_q), total);
-    };
-    const int w0 = start(pair), w1 = start(pair + 1);
-    if (w1 > w0 && w0 >= before && w0 < before + mine) {
-      int at = w0 - before, b = b0, n = chunks_of(b);
-      while (at >= n) {
-        at -= n;
-        n = chunks_of(++b);
-      }
-      n /= units;
-      *sShare = ShShare{b, at / n, at % n, w1 - w0};
-    }
-  }
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();  // the other CTA's barriers are ready
   tc_fence_after();
+  griddep_wait();  // programmatic dependent: q, the caches and the lengths are the previous kernels'
   const uint32_t tmem = *tmem_slot;
-  const ShShare share = *sShare;
-  ShWalk walk(a, share, pair, pairs);
+  ShWalk walk(a, sShare, share_ready, pair, pairs);
   ShSegment sg = {};
   const int G = a.Hq / a.Hkv, R = G * a.T;
 
@@ -489,6 +449,50 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       }
     }
   } else if (warp == 2) {
+    // ---------------- this pair's share of the own chunks. A lane adds up a run of requests.
+    {
+      const int per = ceil_to(a.B, 32);
+      const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
+      const int units = a.Hkv * a.rb_o;
+      auto chunks_of = [&](int b) {
+        return ceil_to(ceil_to(own_rows_of(a.lengths, b, a.src[1].rows), SH_KT), a.chunk) * units;
+      };
+      int mine = 0;
+      if (a.src[1].rows > 0)
+        for (int b = b0; b < b1; ++b) mine += chunks_of(b);
+      int up = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+      }
+      const int before = up - mine, total = __shfl_sync(0xffffffffu, up, 31);
+      // pairs with one prefix segment more carry that much less of the rest
+      const long long G = pairs, more = a.more;
+      const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk * SH_OWN_COST + SH_SEG_COST);
+      const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
+      const long long q_more = all > need ? all - need : 0;
+      const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
+      const double per_q = (double)total / (double)(more * q_more + (G - more) * q_less);
+      auto start = [&](int i) -> int {
+        const long long q = min((long long)i, more) * q_more + max(i - more, 0ll) * q_less;
+        return i == pairs ? total : min((int)((double)q * per_q), total);
+      };
+      const int w0 = start(pair), w1 = start(pair + 1);
+      if (lane == 0) *sShare = ShShare{0, 0, 0, 0, 0};
+      __syncwarp();
+      if (w1 > w0 && w0 >= before && w0 < before + mine) {
+        int at = w0 - before, b = b0, n = chunks_of(b);
+        while (at >= n) {
+          at -= n;
+          n = chunks_of(++b);
+        }
+        n /= units;
+        *sShare = ShShare{b, at / n, at % n, w1 - w0, own_rows_of(a.lengths, b, a.src[1].rows)};
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(share_ready);
+    }
     if (rank == 0) {
       // ---------------- O += P V
       const uint32_t idesc = idesc_bf16_f32(SH_ROWS, SH_D) | (1u << 16);  // B (V) MN-major
@@ -891,16 +895,27 @@ tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *_
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
     den += part;
     const int n = min(32, slots - s0);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      if (ws == 0.f) continue;
-      const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)(s0 + s) * rows + row) * SH_D) + lane;
-      const float4 x = __ldg(src), y = __ldg(src + 32);
-      acc[0] = fmaf(ws, x.x, acc[0]); acc[1] = fmaf(ws, x.y, acc[1]);
-      acc[2] = fmaf(ws, x.z, acc[2]); acc[3] = fmaf(ws, x.w, acc[3]);
-      acc[4] = fmaf(ws, y.x, acc[4]); acc[5] = fmaf(ws, y.y, acc[5]);
-      acc[6] = fmaf(ws, y.z, acc[6]); acc[7] = fmaf(ws, y.w, acc[7]);
+    for (int s = 0; s < n; s += 4) {  // four partials' loads in flight
+      float ws[4];
+      float4 x[4], y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ws[i] = __shfl_sync(0xffffffffu, w, (s + i) & 31);
+        if (s + i >= n) ws[i] = 0.f;
+        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (ws[i] != 0.f) {
+          const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)(s0 + s + i) * rows + row) * SH_D) + lane;
+          x[i] = __ldg(src);
+          y[i] = __ldg(src + 32);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[0] = fmaf(ws[i], x[i].x, acc[0]); acc[1] = fmaf(ws[i], x[i].y, acc[1]);
+        acc[2] = fmaf(ws[i], x[i].z, acc[2]); acc[3] = fmaf(ws[i], x[i].w, acc[3]);
+        acc[4] = fmaf(ws[i], y[i].x, acc[4]); acc[5] = fmaf(ws[i], y[i].y, acc[5]);
+        acc[6] = fmaf(ws[i], y[i].z, acc[6]); acc[7] = fmaf(ws[i], y[i].w, acc[7]);
+      }
     }
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
@@ -965,9 +980,16 @@ size_t copy_bytes(int B, int Hkv, int P, int own_rows) {  // of K or of V
 template <bool SCALED>
 int launch_attn(const CUtensorMap *maps, const ShArgs &a, int pairs, cudaStream_t st) {
   using C = ShCfg<SCALED>;
-  if (cudaFuncSetAttribute(tree_attn_shared_kernel<SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)C::SMEM) != cudaSuccess)
-    return TSB_ECUDA;
+  static std::atomic<unsigned long long> ready{0};  // devices on which the attribute is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TSB_ECUDA;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(tree_attn_shared_kernel<SCALED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)C::SMEM) != cudaSuccess)
+      return TSB_ECUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   const cudaError_t e = launch_pdl(tree_attn_shared_kernel<SCALED>, dim3((unsigned)pairs * 2), dim3(C::THREADS),
                                    (size_t)C::SMEM, st, maps[0], maps[1], maps[2], maps[3], a);
   return e == cudaSuccess ? TSB_OK : TSB_ECUDA;

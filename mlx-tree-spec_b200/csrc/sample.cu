@@ -41,6 +41,8 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "sm100.cuh"
 
 namespace cg = cooperative_groups;
@@ -1037,9 +1039,16 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
   const size_t stage = ((size_t)a.slice + 16 / sizeof(T)) * sizeof(T);
   a.staged = stage <= kMaxStage;
   const size_t smem = kSharedBytes + (a.staged ? stage : 0);
-  if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(kSharedBytes + kMaxStage)) != cudaSuccess)
-    return TSB_ECUDA;
+  static std::atomic<unsigned long long> ready{0};  // devices on which the attribute is set
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return TSB_ECUDA;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if (dev > 63 || !(ready.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(kSharedBytes + kMaxStage)) != cudaSuccess)
+      return TSB_ECUDA;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows * ctas);
   cfg.blockDim = dim3(kThreads);

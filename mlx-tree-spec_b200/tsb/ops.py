@@ -287,46 +287,65 @@ def tree_flash(queries, cache, scale: float, bits=None, tail: int | None = None,
     return out
 
 
-_KV_TYPES = {TSB_KV_BF16: torch.bfloat16, TSB_KV_REF_Q8_ROW: torch.int8, TSB_KV_MLX_Q8_G64: None}
+# The current device, by torch's own C++ accessor where this build has it (as _RAW_STREAM).
+_GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _kv_struct(cache, fmt: int, bsz: int, hkv: int, d: int, device):
+def _bad_plane(name: str, t, shape, device):
+    return ValueError(f"tree_flash_shared: {name} must be a contiguous tensor of shape {tuple(shape)} on {device}, "
+                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def _kv_struct(cache, planes, bsz: int, hkv: int, d: int, device):
     """tsb_kv_t of a cache of `bsz` requests, its planes checked."""
-    planes = _kv_planes(cache)
-    if planes[0] != fmt:
-        raise ValueError("tree_flash_shared: the prefix and the requests' caches must share a format")
-    keys = planes[1]
-    cap, rows = keys.shape[2], int(cache.offset)
+    fmt, k, ks, kb, v, vs, vb = planes
+    cap, rows = k.shape[2], int(cache.offset)
     if not 0 <= rows <= cap:
         raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
-    lead = (bsz, hkv, cap)
-    if fmt == TSB_KV_MLX_Q8_G64:
-        shapes = ((*lead, d // 4), (*lead, d // 64), (*lead, d // 64)) * 2
-        types = (None, torch.bfloat16, torch.bfloat16) * 2
-    else:
-        shapes = ((*lead, d), lead, None) * 2
-        types = (_KV_TYPES[fmt], torch.float32, None) * 2
-    st = _lib.KVT(capacity=cap, rows=rows)
-    for name, t, shape, dt in zip(("k", "k_scales", "k_biases", "v", "v_scales", "v_biases"), planes[1:], shapes, types):
-        if t is None:
-            continue
+    words = fmt == TSB_KV_MLX_Q8_G64
+    shape = (bsz, hkv, cap, d // 4 if words else d)
+    for name, t in (("keys", k), ("values", v)):
         if t.shape != shape or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"tree_flash_shared: {name} must be a contiguous tensor of shape {tuple(shape)} on "
-                             f"{device}, got {tuple(t.shape)} on {t.device}")
-        if (t.dtype != dt) if dt is not None else t.dtype not in (torch.int32, torch.uint32):
-            raise ValueError(f"tree_flash_shared: {name} has type {t.dtype}")
-        setattr(st, name, t.data_ptr())
-    return st
+            raise _bad_plane(name, t, shape, device)
+    if fmt == TSB_KV_BF16:
+        if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+            raise _bad_plane("keys and values in bf16", v, shape, device)
+        return _lib.KVT(k.data_ptr(), None, None, v.data_ptr(), None, None, cap, rows)
+    types = (torch.int32, torch.uint32) if words else (torch.int8,)
+    if k.dtype not in types or v.dtype not in types:
+        raise _bad_plane("keys and values in 8-bit codes", v, shape, device)
+    shape = (bsz, hkv, cap, d // 64) if words else (bsz, hkv, cap)
+    dt = torch.bfloat16 if words else torch.float32
+    for name, t in (("scales", ks), ("scales", vs), ("biases", kb), ("biases", vb)):
+        if name == "biases" and not words:
+            continue
+        if t is None or t.shape != shape or t.dtype != dt or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"tree_flash_shared: {name} must be a contiguous {dt} tensor of shape {shape} on {device}")
+    return _lib.KVT(k.data_ptr(), ks.data_ptr(), _ptr(kb), v.data_ptr(), vs.data_ptr(), _ptr(vb), cap, rows)
 
 
 def _tree_rows(t, bsz: int, n: int, dtype, what: str, device):
     """(n,) or (bsz, n) -> a contiguous (bsz, n) tensor of dtype on device."""
-    t = t.to(device=device, dtype=dtype)
-    if t.shape == (n,):
+    if t.dtype != dtype or t.device != device:
+        t = t.to(device=device, dtype=dtype)
+    if t.dim() == 1 and t.shape[0] == n:
         t = t.expand(bsz, n)
     if t.shape != (bsz, n):
         raise ValueError(f"{what} must have shape ({n},) or ({bsz}, {n}), got {tuple(t.shape)}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+_SHARED_WS_BYTES: dict[tuple, int] = {}
+
+
+def _shared_ws_bytes(lib, *key) -> int:
+    """tsb_tree_attn_shared_workspace_bytes, remembered per shape and device on the host side."""
+    v = _SHARED_WS_BYTES.get(key)
+    if v is None:
+        if len(_SHARED_WS_BYTES) > 4096:
+            _SHARED_WS_BYTES.clear()
+        v = _SHARED_WS_BYTES[key] = lib.tsb_tree_attn_shared_workspace_bytes(*key[:-1])
+    return v
 
 
 def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int | None = None, stats: bool = False,
@@ -346,20 +365,24 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
     tail being the last rows of each request's own; a node that sees nothing
     gets zeros and a log-sum-exp of -inf. queries may have any strides with D
     contiguous and 16-byte aligned rows (others are copied first)."""
-    fmt, pk = _kv_planes(prefix)[:2]
-    _require_cuda(queries, pk, cache.keys)
+    if not queries.is_cuda:
+        raise ValueError("tsb operators take CUDA tensors (there is no CPU path)")
     if queries.dtype != torch.bfloat16 or (parents is None and bits is None):
         return None
-    bsz, hq, n, d = queries.shape
     dev = queries.device
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _GET_DEVICE():
         with torch.cuda.device(dev):
             return tree_flash_shared(queries, prefix, cache, scale, bits, tail, stats, parents, lengths, out)
-    hkv = pk.shape[1]
+    bsz, hq, n, d = queries.shape
+    pre_planes, own_planes = _kv_planes(prefix), _kv_planes(cache)
+    fmt = pre_planes[0]
+    if own_planes[0] != fmt:
+        raise ValueError("tree_flash_shared: the prefix and the requests' caches must share a format")
+    hkv = pre_planes[1].shape[1]
     if d != 256 or hq % hkv or n > 64 or bsz < 1 or n < 1:
         return None
-    pre = _kv_struct(prefix, fmt, 1, hkv, d, dev)
-    own = _kv_struct(cache, fmt, bsz, hkv, d, dev)
+    pre = _kv_struct(prefix, pre_planes, 1, hkv, d, dev)
+    own = _kv_struct(cache, own_planes, bsz, hkv, d, dev)
     p = bits_t = None
     if parents is not None:
         p = _tree_rows(parents, bsz, n, torch.int32, "tree_flash_shared: parents", dev)
@@ -373,8 +396,10 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
         if lengths.dtype != torch.int32 or lengths.shape != (bsz,) or not lengths.is_contiguous() or lengths.device != dev:
             raise ValueError(f"tree_flash_shared: lengths must be a contiguous int32 tensor ({bsz},) on {dev}")
     q = queries
-    if q.stride(3) != 1 or q.stride(0) % 8 or q.stride(1) % 8 or q.stride(2) % 8 or q.data_ptr() % 16:
+    sb, sh, st, sd = q.stride()
+    if sd != 1 or (sb | sh | st) % 8 or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
+        sb, sh, st, sd = q.stride()
     if out is None:
         out = torch.empty((bsz, hq, n, d), dtype=torch.bfloat16, device=dev)
     elif out.shape != queries.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
@@ -382,12 +407,13 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
     lse = torch.empty((bsz, hq, n), dtype=torch.float32, device=dev) if stats else None
     lib = _lib.load()
     # a workspace of this call's own: calls on other streams and captured graphs share nothing
-    ws = torch.empty(lib.tsb_tree_attn_shared_workspace_bytes(bsz, n, hq, hkv, d, pre.rows, own.rows, fmt),
-                     dtype=torch.uint8, device=dev)
-    st = lib.tsb_tree_attn_shared(_ptr(q), q.stride(0), q.stride(1), q.stride(2), fmt, ctypes.byref(pre),
-                                  ctypes.byref(own), _ptr(lengths), _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, tail_v,
-                                  float(scale), _ptr(out), _ptr(lse), _ptr(ws), ws.numel(), _stream(q))
-    if check(st, "tsb_tree_attn_shared") == TSB_EUNSUPPORTED:
+    nbytes = _shared_ws_bytes(lib, bsz, n, hq, hkv, d, pre.rows, own.rows, fmt, dev.index)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    status = lib.tsb_tree_attn_shared(q.data_ptr(), sb, sh, st, fmt, ctypes.byref(pre), ctypes.byref(own), _ptr(lengths),
+                                      _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, tail_v, scale, out.data_ptr(), _ptr(lse),
+                                      ws.data_ptr(), nbytes, _stream(q))
+    if status:
+        check(status, "tsb_tree_attn_shared")
         return None
     if stats:
         return out, lse[..., None], torch.ones_like(lse)[..., None]

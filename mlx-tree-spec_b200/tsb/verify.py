@@ -24,7 +24,7 @@ import torch
 
 from . import _lib
 from ._lib import TSB_EUNSUPPORTED, TSB_KV_MLX_Q8_G64, TSB_MASK_BF16, TSB_MASK_F16, TSB_MASK_F32, check
-from .ops import _kv_planes, _ptr, _require_cuda, _stream
+from .ops import _GET_DEVICE, _kv_planes, _ptr, _require_cuda, _stream
 
 _LOGIT_TYPES = {torch.bfloat16: TSB_MASK_BF16, torch.float16: TSB_MASK_F16, torch.float32: TSB_MASK_F32}
 _MAX_LAYERS_PER_LAUNCH = 48
@@ -32,16 +32,18 @@ _MAX_VOCAB = 1 << 20
 
 
 def _per_row(v, rows: int, dtype, name: str, device):
-    """A sampling parameter: (device tensor or None, scalar)."""
+    """A sampling parameter: (device pointer or None, scalar, what keeps the pointer alive)."""
     if not isinstance(v, torch.Tensor):
-        return None, v
+        return None, v, None
     if v.device != device:
         raise ValueError(f"sample: {name} must be on {device}")
     if v.numel() != rows:
         raise ValueError(f"sample: {name} must have one value per row ({rows}), got {tuple(v.shape)}")
     if v.dtype != dtype:
         v = v.to(dtype)
-    return (v if v.is_contiguous() else v.contiguous()), 0
+    if not v.is_contiguous():
+        v = v.contiguous()
+    return v.data_ptr(), 0, v
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: bool = False):
@@ -60,41 +62,42 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: 
     probabilities under the filtered distribution. Logits of -inf or NaN are
     never chosen; a row of nothing else gives -1 and -inf. None where the type
     or V (> 2^20) is not taken."""
-    _require_cuda(logits, u)
     dt = _LOGIT_TYPES.get(logits.dtype)
+    if not logits.is_cuda:
+        raise ValueError("tsb operators take CUDA tensors (there is no CPU path)")
     if dt is None or logits.dim() < 1:
         return None
     dev = logits.device
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _GET_DEVICE():
         with torch.cuda.device(dev):
             return sample(logits, u, temperature, top_k, top_p, min_p, logprobs)
-    vocab = logits.shape[-1]
-    lead = logits.shape[:-1]
+    *lead, vocab = logits.shape
     if vocab < 1:
         raise ValueError("sample: logits have no tokens")
     if vocab > _MAX_VOCAB:
         return None
-    if u.shape != lead or u.dtype != torch.float32 or u.device != dev:
+    if u.dtype != torch.float32 or list(u.shape) != lead or u.device != dev:
         raise ValueError(f"sample: u must be float32 of shape {tuple(lead)} on {dev}, got {u.dtype} {tuple(u.shape)}")
-    x = logits
-    if x.dim() != 2:
-        x = x.reshape(-1, vocab)
+    x = logits if len(lead) == 1 else logits.reshape(-1, vocab)
     rows = x.shape[0]
-    if x.stride(1) != 1 and vocab > 1 or rows > 1 and x.stride(0) < vocab:
+    stride = x.stride(0) if rows > 1 else vocab
+    if stride < vocab or (vocab > 1 and x.stride(1) != 1):
         x = x.contiguous()
-    t_t, t_s = _per_row(temperature, rows, torch.float32, "temperature", dev)
-    k_t, k_s = _per_row(top_k, rows, torch.int32, "top_k", dev)
-    p_t, p_s = _per_row(top_p, rows, torch.float32, "top_p", dev)
-    m_t, m_s = _per_row(min_p, rows, torch.float32, "min_p", dev)
+        stride = vocab
+    t_p, t_s, t_ref = _per_row(temperature, rows, torch.float32, "temperature", dev)
+    k_p, k_s, k_ref = _per_row(top_k, rows, torch.int32, "top_k", dev)
+    p_p, p_s, p_ref = _per_row(top_p, rows, torch.float32, "top_p", dev)
+    m_p, m_s, m_ref = _per_row(min_p, rows, torch.float32, "min_p", dev)
     token = torch.empty(lead, dtype=torch.int32, device=dev)
     logprob = torch.empty(lead, dtype=torch.float32, device=dev) if logprobs else None
     if rows:
         if not u.is_contiguous():
             u = u.contiguous()
-        st = _lib.load().tsb_sample(_ptr(x), dt, rows, vocab, x.stride(0) if rows > 1 else vocab, _ptr(u), _ptr(t_t), t_s,
-                                    _ptr(k_t), min(max(int(k_s), 0), vocab), _ptr(p_t), p_s, _ptr(m_t), m_s,
-                                    _ptr(token), _ptr(logprob), _stream(x))
-        if check(st, "tsb_sample") == TSB_EUNSUPPORTED:
+        status = _lib.load().tsb_sample(x.data_ptr(), dt, rows, vocab, stride, u.data_ptr(), t_p, t_s, k_p,
+                                        min(max(int(k_s), 0), vocab), p_p, p_s, m_p, m_s, token.data_ptr(), _ptr(logprob),
+                                        _stream(x))
+        if status:
+            check(status, "tsb_sample")
             return None
     return (token, logprob) if logprobs else token
 
@@ -117,14 +120,16 @@ def tree_accept(tokens, parents, samples):
     each node (negative: nothing follows). Returns int32 path (B, T), the
     accepted nodes and then -1; n_keep (B,), their number; next_token (B,), the
     token sampled after the last of them. None for T > 64."""
-    _require_cuda(tokens, parents, samples)
-    if tokens.dim() != 2:
-        raise ValueError("tree_accept: tokens must be (B, T)")
+    if not tokens.is_cuda:
+        raise ValueError("tsb operators take CUDA tensors (there is no CPU path)")
     dev = tokens.device
-    if dev.index != torch.cuda.current_device():
+    if dev.index != _GET_DEVICE():
         with torch.cuda.device(dev):
             return tree_accept(tokens, parents, samples)
-    b, t = shape = tokens.shape
+    shape = tokens.shape
+    if len(shape) != 2:
+        raise ValueError("tree_accept: tokens must be (B, T)")
+    b, t = shape
     if t > 64:
         return None
     if t < 1:
@@ -132,12 +137,14 @@ def tree_accept(tokens, parents, samples):
     tok = _i32(tokens, shape, "tree_accept: tokens", dev)
     par = _i32(parents, shape, "tree_accept: parents", dev)
     smp = _i32(samples, shape, "tree_accept: samples", dev)
-    path = torch.empty((b, t), dtype=torch.int32, device=dev)
-    n_keep = torch.empty(b, dtype=torch.int32, device=dev)
-    nxt = torch.empty(b, dtype=torch.int32, device=dev)
+    path = torch.empty_like(tok)
+    n_keep = tok.new_empty(b)
+    nxt = tok.new_empty(b)
     if b:
-        check(_lib.load().tsb_tree_accept(_ptr(tok), _ptr(par), _ptr(smp), b, t, _ptr(path), _ptr(n_keep), _ptr(nxt),
-                                          _stream(tok)), "tsb_tree_accept")
+        status = _lib.load().tsb_tree_accept(tok.data_ptr(), par.data_ptr(), smp.data_ptr(), b, t, path.data_ptr(),
+                                             n_keep.data_ptr(), nxt.data_ptr(), _stream(tok))
+        if status:
+            check(status, "tsb_tree_accept")
     return path, n_keep, nxt
 
 
@@ -191,7 +198,7 @@ class PathCommit:
 
     def __call__(self, lengths, path, n_keep):
         dev, b = self._device, self._batch
-        if dev.index != torch.cuda.current_device():
+        if dev.index != _GET_DEVICE():
             with torch.cuda.device(dev):
                 return self(lengths, path, n_keep)
         if path.dim() != 2:
@@ -202,11 +209,12 @@ class PathCommit:
         p = _i32(path, (b, t), "PathCommit: path", dev)
         n = _i32(n_keep, (b,), "PathCommit: n_keep", dev)
         cur = _i32(lengths, (b,), "PathCommit: lengths", dev)
-        new = torch.empty(b, dtype=torch.int32, device=dev)
-        lib = _lib.load()
-        for i, args in enumerate(self._launches):
-            st = lib.tsb_kv_commit_paths(*args, t, _ptr(cur), _ptr(p), _ptr(n), _ptr(new) if i == 0 else None, _stream(p))
-            if check(st, "tsb_kv_commit_paths") == TSB_EUNSUPPORTED:
+        new = torch.empty_like(cur)
+        commit, stream, out = _lib.load().tsb_kv_commit_paths, _stream(p), new.data_ptr()
+        for args in self._launches:
+            status = commit(*args, t, cur.data_ptr(), p.data_ptr(), n.data_ptr(), out, stream)
+            out = None  # one launch writes the lengths
+            if status and check(status, "tsb_kv_commit_paths") == TSB_EUNSUPPORTED:
                 raise ValueError("PathCommit: unsupported caches")
         return new
 
