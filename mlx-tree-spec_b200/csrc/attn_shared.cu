@@ -467,16 +467,21 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         if (lane >= o) up += v;
       }
       const int before = up - mine, total = __shfl_sync(0xffffffffu, up, 31);
-      // pairs with one prefix segment more carry that much less of the rest
-      const long long G = pairs, more = a.more;
-      const long long seg = a.tps + SH_SEG_COST, all = (long long)total * (a.chunk * SH_OWN_COST + SH_SEG_COST);
-      const long long need = more ? (G - more) * seg : 0;  // brings the others up to them
-      const long long q_more = all > need ? all - need : 0;
-      const long long q_less = all > need ? q_more + (more ? seg * G : 0) : 1;  // shares, in proportion
-      const double per_q = (double)total / (double)(more * q_more + (G - more) * q_less);
+      // Pairs with one prefix segment more carry that much less of the rest: first the
+      // number of chunks of the others that evens the loads out, then whole chunks.
+      const long long G = pairs, more = a.more, less = G - more;
+      const long long seg = a.tps + SH_SEG_COST, cost = a.chunk * SH_OWN_COST + SH_SEG_COST;
+      const long long all = total * cost, need = more ? less * seg : 0;
+      long long few = total;  // chunks of the pairs without the extra segment
+      if (more) {
+        const long long each = all > need ? (all - need) / G + seg : all / less;  // their load beyond the others'
+        few = each * less / cost;
+        const long long up_to = (each + cost - 1) / cost;  // rounded up, where no pair of the others would do better
+        if (up_to * cost <= seg + cost) few = up_to * less;
+        few = min(few, (long long)total);
+      }
       auto start = [&](int i) -> int {
-        const long long q = min((long long)i, more) * q_more + max(i - more, 0ll) * q_less;
-        return i == pairs ? total : min((int)((double)q * per_q), total);
+        return i < more ? (int)((total - few) * i / more) : (int)((total - few) + (less ? few * (i - more) / less : 0));
       };
       const int w0 = start(pair), w1 = start(pair + 1);
       if (lane == 0) *sShare = ShShare{0, 0, 0, 0, 0};
@@ -807,54 +812,66 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
 // The valid rows of an 8-bit cache as bf16 rows [heads][rows][D]: MLX values
 // bf16(fmaf(code, s, b)), or the int8 codes themselves. 16 lanes have a row; bound
 // by memory (272 or 256 bytes read and 512 written per row).
+constexpr int SH_CV_ROWS = 64;  // rows of a CTA
+
 struct ShConvert {
-  const unsigned char *src[2];    // K, V codes
-  const uint2 *scale[2], *bias[2];  // MLX: four bf16 per row
-  uint16_t *dst[2];
-  const int32_t *lengths;  // per request, or NULL
-  int heads;               // KV heads per request
-  int cap, rows;           // of the source per (request, head); of the copy
+  struct Cache {
+    const unsigned char *src[2];      // K, V codes
+    const uint2 *scale[2], *bias[2];  // MLX: four bf16 per row
+    uint16_t *dst[2];
+    int cap, rows;          // rows of a head in the source, and (at most) in the copy
+    int blocks;
+  } cache[2];               // prefix, own
+  const int32_t *lengths;   // own rows of each request, or NULL
+  int hkv;
 };
 
-constexpr int SH_CV_ROWS = 64;  // rows of a CTA
 
 template <bool MLX>
 __global__ void __launch_bounds__(256) tree_attn_shared_convert_kernel(const __grid_constant__ ShConvert a) {
   griddep_wait();  // programmatic dependent: the caches are the previous kernels'
   griddep_launch_dependents();
-  const int head = blockIdx.y, v = blockIdx.z;
-  const int n = own_rows_of(a.lengths, head / a.heads, a.rows);
-  const int row0 = blockIdx.x * SH_CV_ROWS;
+  // blocks of the prefix, then of the own rows: (head, K or V, run of rows)
+  const int own = (int)blockIdx.x >= a.cache[0].blocks;
+  const ShConvert::Cache &c = a.cache[own];
+  const int block = blockIdx.x - (own ? a.cache[0].blocks : 0), runs = ceil_to(c.rows, SH_CV_ROWS);
+  const int head = block / (2 * runs), v = block / runs & 1;
+  const int n = own ? own_rows_of(a.lengths, head / a.hkv, c.rows) : c.rows;
+  const int row0 = block % runs * SH_CV_ROWS;
   if (row0 >= n) return;
-  const int c = threadIdx.x & 15;
+  const int c16 = threadIdx.x & 15;
+  uint4 w[SH_CV_ROWS / 16];
+#pragma unroll
+  for (int i = 0; i < SH_CV_ROWS / 16; ++i) {
+    const int row = row0 + i * 16 + (threadIdx.x >> 4);
+    w[i] = row < n ? ldg_nc_v4(c.src[v] + ((size_t)head * c.cap + row) * SH_D + c16 * 16) : make_uint4(0u, 0u, 0u, 0u);
+  }
 #pragma unroll
   for (int i = 0; i < SH_CV_ROWS / 16; ++i) {
     const int row = row0 + i * 16 + (threadIdx.x >> 4);
     if (row >= n) break;
-    const size_t at = (size_t)head * a.cap + row;
-    const uint4 w = ldg_nc_v4(a.src[v] + at * SH_D + c * 16);
+    const size_t at = (size_t)head * c.cap + row;
     uint4 lo, hi;
     if (MLX) {
-      const uint16_t *sc = reinterpret_cast<const uint16_t *>(a.scale[v] + at), *bi = reinterpret_cast<const uint16_t *>(a.bias[v] + at);
-      const float s = bf16_bits_to_float(__ldg(sc + (c >> 2))), b = bf16_bits_to_float(__ldg(bi + (c >> 2)));
-      lo = dequant8_mlx(make_uint2(w.x, w.y), s, b);
-      hi = dequant8_mlx(make_uint2(w.z, w.w), s, b);
+      const uint16_t *sc = reinterpret_cast<const uint16_t *>(c.scale[v] + at), *bi = reinterpret_cast<const uint16_t *>(c.bias[v] + at);
+      const float s = bf16_bits_to_float(__ldg(sc + (c16 >> 2))), b = bf16_bits_to_float(__ldg(bi + (c16 >> 2)));
+      lo = dequant8_mlx(make_uint2(w[i].x, w[i].y), s, b);
+      hi = dequant8_mlx(make_uint2(w[i].z, w[i].w), s, b);
     } else {
-      lo = convert8_s8(make_uint2(w.x, w.y));
-      hi = convert8_s8(make_uint2(w.z, w.w));
+      lo = convert8_s8(make_uint2(w[i].x, w[i].y));
+      hi = convert8_s8(make_uint2(w[i].z, w[i].w));
     }
-    uint4 *dst = reinterpret_cast<uint4 *>(a.dst[v] + ((size_t)head * a.rows + row) * SH_D) + c * 2;
+    uint4 *dst = reinterpret_cast<uint4 *>(c.dst[v] + ((size_t)head * c.rows + row) * SH_D) + c16 * 2;
     dst[0] = lo;
     dst[1] = hi;
   }
 }
 
 template <bool MLX>
-int launch_convert(const ShConvert &a, int requests, cudaStream_t st) {
-  const long long heads = (long long)requests * a.heads;
-  if (heads > 65535) return TSB_EUNSUPPORTED;
-  const dim3 grid((unsigned)((a.rows + SH_CV_ROWS - 1) / SH_CV_ROWS), (unsigned)heads, 2);
-  const cudaError_t e = launch_pdl(tree_attn_shared_convert_kernel<MLX>, grid, dim3(256), 0, st, a);
+int launch_convert(const ShConvert &a, cudaStream_t st) {
+  const int blocks = a.cache[0].blocks + a.cache[1].blocks;
+  if (blocks == 0) return TSB_OK;
+  const cudaError_t e = launch_pdl(tree_attn_shared_convert_kernel<MLX>, dim3((unsigned)blocks), dim3(256), 0, st, a);
   return e == cudaSuccess ? TSB_OK : TSB_ECUDA;
 }
 
@@ -1057,7 +1074,6 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   }
   if ((long long)Hkv * prefix->capacity > 0x7fffffc0LL || (long long)B * Hkv * own->capacity > 0x7fffffc0LL)
     return TSB_EUNSUPPORTED;  // tensor-map row coordinates are 32-bit
-  if (kv_format != TSB_KV_BF16 && (long long)B * Hkv > 65535) return TSB_EUNSUPPORTED;  // the converting grid
   const ShPlan p = plan_shared(B, T, Hq, Hkv, P, own_rows);
   const size_t part = partial_bytes(p, B, T, Hq);
   const size_t need = tsb_tree_attn_shared_workspace_bytes(B, T, Hq, Hkv, D, P, own_rows, kv_format);
@@ -1070,36 +1086,41 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   CUtensorMap maps[4] = {};
   // the bf16 rows to attend to: the caches themselves, or copies of them
   char *copy = (char *)ws + part;
+  ShConvert cv = {};
+  cv.lengths = lengths;
+  cv.hkv = Hkv;
   for (int i = 0; i < 2; ++i) {
     const tsb_kv_t *c = srcs[i];
+    if (!c->rows) continue;
     const int requests = i ? B : 1;
-    const void *kv[2] = {c->k, c->v};
+    const void *kv[2] = {c->k, c->v}, *scales[2] = {c->k_scales, c->v_scales}, *biases[2] = {c->k_biases, c->v_biases};
     int cap = c->capacity;
-    if (kv_format != TSB_KV_BF16 && c->rows > 0) {
-      ShConvert cv = {};
-      const size_t bytes = (size_t)requests * Hkv * c->rows * SH_D * 2;
-      const void *scales[2] = {c->k_scales, c->v_scales}, *biases[2] = {c->k_biases, c->v_biases};
+    if (kv_format != TSB_KV_BF16) {
+      ShConvert::Cache &to = cv.cache[i];
+      to.cap = cap;
+      to.rows = cap = c->rows;
+      const long long blocks = 2LL * requests * Hkv * ((c->rows + SH_CV_ROWS - 1) / SH_CV_ROWS);
+      if (blocks > 0x3fffffffLL) return TSB_EUNSUPPORTED;
+      to.blocks = (int)blocks;
       for (int v = 0; v < 2; ++v) {
-        cv.src[v] = (const unsigned char *)kv[v];
-        cv.scale[v] = (const uint2 *)scales[v];
-        cv.bias[v] = (const uint2 *)biases[v];
-        cv.dst[v] = (uint16_t *)(copy + v * bytes);
-        kv[v] = cv.dst[v];
+        to.src[v] = (const unsigned char *)kv[v];
+        to.scale[v] = (const uint2 *)scales[v];
+        to.bias[v] = (const uint2 *)biases[v];
+        to.dst[v] = (uint16_t *)copy;
+        kv[v] = copy;
+        copy += (size_t)requests * Hkv * to.rows * SH_D * 2;
       }
-      copy += 2 * bytes;
-      cv.lengths = i ? lengths : nullptr;
-      cv.heads = Hkv;
-      cv.cap = cap;
-      cv.rows = cap = c->rows;
-      const int e = kv_format == TSB_KV_MLX_Q8_G64 ? launch_convert<true>(cv, requests, stm) : launch_convert<false>(cv, requests, stm);
-      if (e != TSB_OK) return e;
     }
     a.src[i] = ShSource{(const float *)c->k_scales, (const float *)c->v_scales, c->capacity, cap, c->rows};
-    for (int v = 0; v < 2 && c->rows > 0; ++v)
+    for (int v = 0; v < 2; ++v)
       if (make_tmap_2d(&maps[2 * i + v], kv[v], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, SH_D,
                        (uint64_t)requests * Hkv * cap, SH_D * 2, 64, v ? SH_KT : SH_KT / 2,
                        CU_TENSOR_MAP_SWIZZLE_128B) != TSB_OK)
         return TSB_ECUDA;
+  }
+  if (kv_format != TSB_KV_BF16) {
+    const int e = kv_format == TSB_KV_MLX_Q8_G64 ? launch_convert<true>(cv, stm) : launch_convert<false>(cv, stm);
+    if (e != TSB_OK) return e;
   }
   a.q = (const uint16_t *)q;
   a.q_sb = q_stride_b;
