@@ -719,13 +719,16 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         // scores in eight independent chains; the scale is applied in the exp
         const int key0 = (sg.j0 + j) * SH_KT;
         if ((key0 + SH_KT > sg.tail_lo) || (key0 + SH_KT > sg.n_kv)) {
+          const int before = sg.tail_lo - key0, keys = sg.n_kv - key0;  // keys of the tile before the tree, and in all
+          unsigned long long vis = before >= 64   ? ~0ull
+                                   : before > 0   ? (mybits << before) | ((1ull << before) - 1)
+                                   : before > -64 ? mybits >> -before
+                                                  : 0ull;
+          if (keys < 64) vis &= (1ull << keys) - 1;  // at least one key
+          const uint32_t v2[2] = {(uint32_t)vis, (uint32_t)(vis >> 32)};
 #pragma unroll
-          for (int e = 0; e < 64; ++e) {
-            const int key = key0 + e;
-            bool vis = key < sg.n_kv;
-            if (vis && key >= sg.tail_lo) vis = (mybits >> (key - sg.tail_lo)) & 1ull;
-            if (!vis) sr[e] = __float_as_uint(-INFINITY);
-          }
+          for (int e = 0; e < 64; ++e)
+            if (!(v2[e >> 5] >> (e & 31) & 1u)) sr[e] = __float_as_uint(-INFINITY);
         }
         float mx[8];
 #pragma unroll
