@@ -70,9 +70,9 @@ constexpr int SH_SOFT0 = 4, SH_NSOFT = 8;    // softmax warps
 constexpr int SH_MAX_SPLITS = 64;            // key splits of a prefix unit
 constexpr int SH_MAX_CHUNKS = 16;            // chunks of a request's own rows
 constexpr int SH_MIN_CHUNK = 4;              // tiles
-// What a segment costs beside its tiles (Q in, partials out, ~9000 cycles of ~1060 a
-// tile), and an own tile in units of a prefix tile (shorter runs, masks, cold rows).
-constexpr int SH_SEG_COST = 9, SH_OWN_COST = 2;
+// What a segment costs beside its tiles, in tiles of ~1060 cycles: Q in and partials out
+// (~10,000 cycles measured); of own rows the node masks and a cold walk besides.
+constexpr int SH_SEG_COST = 10, SH_OWN_SEG_COST = 12;
 
 template <bool SCALED>
 struct ShCfg {
@@ -116,6 +116,22 @@ TSB_HD int own_rows_of(const int32_t *lengths, int b, int most) {
   return lengths ? min(max(lengths[b], 0), most) : most;
 }
 TSB_HD int ceil_to(int a, int b) { return (a + b - 1) / b; }
+
+// Deals `total` own chunks of cost c to pairs of which `more` have a prefix segment (cost
+// seg) more than the others: either all to those others, or as many as even them out, and
+// then the same number to each. `few`: the chunks of the pairs without the extra segment.
+struct ShDeal {
+  long long few, level;  // level: the longest pair's load beyond the segments that all have
+};
+__host__ __device__ inline ShDeal deal_chunks(long long total, int pairs, int more, long long seg, long long c) {
+  const int less = pairs - more;  // never 0
+  const long long k = (total + less - 1) / less, alone = k * c > seg || !more ? k * c : seg;
+  if (!more || k * c <= seg) return {total, alone};
+  const long long f = seg / c, r = (total - less * f + pairs - 1) / pairs;  // r >= 1
+  if (alone <= seg + r * c) return {total, alone};
+  const long long few = less * (f + r);
+  return {few < total ? few : total, seg + r * c};
+}
 
 // A pair's share of the own chunks: `left` chunks from (b, u, ch) on; len = b's rows.
 struct ShShare {
@@ -467,19 +483,8 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         if (lane >= o) up += v;
       }
       const int before = up - mine, total = __shfl_sync(0xffffffffu, up, 31);
-      // Pairs with one prefix segment more carry that much less of the rest: first the
-      // number of chunks of the others that evens the loads out, then whole chunks.
-      const long long G = pairs, more = a.more, less = G - more;
-      const long long seg = a.tps + SH_SEG_COST, cost = a.chunk * SH_OWN_COST + SH_SEG_COST;
-      const long long all = total * cost, need = more ? less * seg : 0;
-      long long few = total;  // chunks of the pairs without the extra segment
-      if (more) {
-        const long long each = all > need ? (all - need) / G + seg : all / less;  // their load beyond the others'
-        few = each * less / cost;
-        const long long up_to = (each + cost - 1) / cost;  // rounded up, where no pair of the others would do better
-        if (up_to * cost <= seg + cost) few = up_to * less;
-        few = min(few, (long long)total);
-      }
+      const int more = a.more, less = pairs - more;
+      const long long few = deal_chunks(total, pairs, more, a.tps + SH_SEG_COST, a.chunk + SH_OWN_SEG_COST).few;
       auto start = [&](int i) -> int {
         return i < more ? (int)((total - few) * i / more) : (int)((total - few) + (less ? few * (i - more) / less : 0));
       };
@@ -955,31 +960,35 @@ ShPlan plan_shared(int B, int T, int Hq, int Hkv, int P, int own_rows) {
   const int pairs = std::max(1, sm_count() / 2), R = (Hq / Hkv) * T;
   p.rb_p = (int)(((long long)B * R + SH_ROWS - 1) / SH_ROWS);
   p.rb_o = (R + SH_ROWS - 1) / SH_ROWS;
-  // prefix: the number of key splits with the shortest longest pair
-  const int tiles = (P + SH_KT - 1) / SH_KT;
-  if (tiles > 0) {
-    const long long units = (long long)Hkv * p.rb_p;
-    long long best = -1;
-    for (int s = 1; s <= std::min(SH_MAX_SPLITS, std::max(1, tiles / 4)); ++s) {
-      const int tps = (tiles + s - 1) / s, n = (tiles + tps - 1) / tps;
-      const long long cost = ((units * n + pairs - 1) / pairs) * (tps + SH_SEG_COST);
+  // The number of key splits of the prefix and the chunks of the own rows with the
+  // shortest longest pair, were all requests as long as the longest. A prefix in one
+  // round that leaves pairs to the own rows beats one that fills all pairs evenly
+  // (8 x 16 nodes over 8K + 512 rows: 37 us with 48 segments of 32 tiles on 74 pairs,
+  // 41 with 72 of 22 and the own rows behind them).
+  const int tiles = (P + SH_KT - 1) / SH_KT, own_tiles = (own_rows + SH_KT - 1) / SH_KT;
+  const long long units = tiles > 0 ? (long long)Hkv * p.rb_p : 0;
+  const long long own_units = own_tiles > 0 ? (long long)B * Hkv * p.rb_o : 0;
+  p.chunk = std::max(1, own_tiles);
+  int s_most = std::min(SH_MAX_SPLITS, std::max(1, tiles / 2));
+  if (units > 0) s_most = (int)std::min<long long>(s_most, 1 + 4LL * pairs / units);  // at most four rounds
+  long long best = -1;
+  for (int s = 1; s <= s_most; ++s) {
+    const int tps = (tiles + s - 1) / s, n = tps ? (tiles + tps - 1) / tps : 0;
+    const long long rounds = units * n / pairs, seg = tps + SH_SEG_COST;
+    const int more = (int)(units * n % pairs);
+    for (int ch = 1; ch <= SH_MAX_CHUNKS && (ch == 1 || own_tiles >= ch * SH_MIN_CHUNK); ch *= 2) {
+      const int chunk = std::max(1, (own_tiles + ch - 1) / ch), chunks = (own_tiles + chunk - 1) / chunk;
+      const long long cost = rounds * seg + deal_chunks(own_units * chunks, pairs, more, seg, chunk + SH_OWN_SEG_COST).level;
       if (best < 0 || cost < best) {
         best = cost;
         p.splits = n;
         p.tps = tps;
+        p.chunk = chunk;
+        p.chunks = chunks;
       }
     }
-    p.items = (int)std::min(units * p.splits, 0x7fffffffLL);
   }
-  // own rows: chunks small enough to even the pairs out, at most SH_MAX_CHUNKS a request
-  const int own_tiles = (own_rows + SH_KT - 1) / SH_KT;
-  const long long own_units = (long long)B * Hkv * p.rb_o;
-  p.chunk = SH_MIN_CHUNK;
-  if (own_tiles > 0) {
-    p.chunk = std::max(p.chunk, (own_tiles + SH_MAX_CHUNKS - 1) / SH_MAX_CHUNKS);
-    p.chunk = std::max(p.chunk, (int)std::min<long long>(own_tiles, own_units * own_tiles / (2LL * pairs)));
-    p.chunks = (own_tiles + p.chunk - 1) / p.chunk;
-  }
+  p.items = (int)std::min(units * p.splits, 0x7fffffffLL);
   p.pairs = (int)std::min<long long>(pairs, (long long)p.items + own_units * p.chunks);
   return p;
 }
