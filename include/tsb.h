@@ -242,7 +242,7 @@ typedef struct {
  * out[b, h, t, :] = softmax over the rows of `prefix` (one cache [1, Hkv, cap,
  * D], every row visible to every node) and request b's own rows (`own`, [B,
  * Hkv, cap, D]), with G = Hq / Hkv query heads per KV head. The prefix is read
- * once per 128 packed query rows of the whole batch, not once per request. The
+ * once per 256 packed query rows of the whole batch, not once per request. The
  * reference has no counterpart (its batched decoding keeps a whole cache per
  * request, mlx-tree-spec src/mlx_tree_spec/tree_verify.py:340-367); the result
  * is that of tsb_tree_attn on each request's concatenated cache.
@@ -255,6 +255,10 @@ typedef struct {
  *            A request with fewer own rows than `tail` has the last ones of them.
  *   out      bf16 [B, Hq, T, D]; lse float [B, Hq, T] or NULL: as tsb_tree_attn.
  *            A node that sees nothing gets zeros and -inf.
+ *   sums     float [B, Hq, T] or NULL: ones, the weights' sums relative to lse
+ *            (the third member of a (out, max, sum) triple to be merged)
+ * 8-bit caches are converted to bf16 in the workspace first (the valid rows of
+ * both, 1 KB per row and KV head), the int8 rows' scales staying in float32.
  * Either cache may have no rows (its planes are then not read). Planes 16-byte
  * aligned, MLX scales and biases 8, row scales 4. Requirements: D == 256,
  * Hq % Hkv == 0, 1 <= T <= 64, tail <= 64, scale > 0, B*Hq*T <= 2^22. No host
@@ -267,7 +271,8 @@ size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D
 int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride_h, long long q_stride_t,
                          int kv_format, const tsb_kv_t *prefix, const tsb_kv_t *own, const int32_t *lengths,
                          const int32_t *parents, const uint64_t *bits, int B, int T, int Hq, int Hkv, int D, int tail,
-                         float scale, void *out, float *lse, void *ws, size_t ws_bytes, tsb_stream_t stream);
+                         float scale, void *out, float *lse, float *sums, void *ws, size_t ws_bytes,
+                         tsb_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * After the logits: sampling, the walk down the draft tree, and the commit of

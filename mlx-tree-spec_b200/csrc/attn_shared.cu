@@ -892,7 +892,7 @@ constexpr int SH_CB_WARPS = 4;
 __global__ void __launch_bounds__(SH_CB_WARPS * 32)
 tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *__restrict__ part_ml, int splits,
                                 const int32_t *__restrict__ lengths, int own_rows, int chunk_rows, int rows_per_b,
-                                int rows, uint16_t *__restrict__ out, float *__restrict__ lse) {
+                                int rows, uint16_t *__restrict__ out, float *__restrict__ lse, float *__restrict__ sums) {
   griddep_wait();  // programmatic dependent: the partials are the attention kernel's
   griddep_launch_dependents();
   const int lane = threadIdx.x % 32;
@@ -947,6 +947,7 @@ tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *_
   uint2 *dst = reinterpret_cast<uint2 *>(out + (size_t)row * SH_D) + lane;
   dst[0] = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   dst[32] = make_uint2(pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
+  if (sums && lane == 0) sums[row] = 1.f;
   if (lse && lane == 0) lse[row] = den > 0.f ? (m + log2f(den)) * 0.69314718055994531f : -INFINITY;
 }
 
@@ -1064,7 +1065,7 @@ extern "C" size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int
 extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride_h, long long q_stride_t,
                                     int kv_format, const tsb_kv_t *prefix, const tsb_kv_t *own, const int32_t *lengths,
                                     const int32_t *parents, const uint64_t *bits, int B, int T, int Hq, int Hkv, int D,
-                                    int tail, float scale, void *out, float *lse, void *ws, size_t ws_bytes,
+                                    int tail, float scale, void *out, float *lse, float *sums, void *ws, size_t ws_bytes,
                                     tsb_stream_t stream) {
   if (!q || !prefix || !own || !out) return TSB_EINVAL;
   const int P = prefix->rows, own_rows = own->rows;
@@ -1078,7 +1079,7 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   if (kv_format < 0 || kv_format > 2) return TSB_EUNSUPPORTED;
   if (!(scale > 0.f)) return TSB_EUNSUPPORTED;  // the kernel takes row maxima of unscaled scores
   if (!aligned(q, 16) || q_stride_b % 8 || q_stride_h % 8 || q_stride_t % 8) return TSB_EINVAL;
-  if (!aligned(out, 16) || !aligned(lse, 4)) return TSB_EINVAL;
+  if (!aligned(out, 16) || !aligned(lse, 4) || !aligned(sums, 4)) return TSB_EINVAL;
   const tsb_kv_t *srcs[2] = {prefix, own};
   for (int i = 0; i < 2; ++i) {
     const int st = check_source(kv_format, srcs[i], srcs[i]->rows > 0);
@@ -1157,6 +1158,6 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   const cudaError_t e =
       launch_pdl(tree_attn_shared_combine_kernel, dim3((unsigned)((rows + SH_CB_WARPS - 1) / SH_CB_WARPS)),
                  dim3(SH_CB_WARPS * 32), 0, stm, (const float *)a.part_o, (const float *)a.part_ml, p.splits, lengths,
-                 own_rows, p.chunk * SH_KT, Hq * T, (int)rows, (uint16_t *)out, lse);
+                 own_rows, p.chunk * SH_KT, Hq * T, (int)rows, (uint16_t *)out, lse, sums);
   return e == cudaSuccess ? TSB_OK : TSB_ECUDA;
 }

@@ -73,8 +73,8 @@ SIGNATURES = {
     "tsb_kv_commit": (_I, [_I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P]),
     "tsb_kv_commit_layers": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P]),
     "tsb_tree_attn_shared_workspace_bytes": (_Z, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    "tsb_tree_attn_shared": (_I, [_P, _LL, _LL, _LL, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _Z,
-                                  _P]),
+    "tsb_tree_attn_shared": (_I, [_P, _LL, _LL, _LL, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _P, _P,
+                                  _Z, _P]),
     "tsb_sample": (_I, [_P, _I, _I, _I, _LL, _P, _P, _D, _P, _I, _P, _D, _P, _D, _P, _P, _P]),
     "tsb_tree_accept": (_I, [_P, _P, _P, _I, _I, _P, _P, _P, _P]),
     "tsb_kv_commit_paths": (_I, [_I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P]),

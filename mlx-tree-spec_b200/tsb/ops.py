@@ -404,19 +404,19 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
         out = torch.empty((bsz, hq, n, d), dtype=torch.bfloat16, device=dev)
     elif out.shape != queries.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise ValueError("tree_flash_shared: out must be a contiguous bf16 tensor of the queries' shape")
-    lse = torch.empty((bsz, hq, n), dtype=torch.float32, device=dev) if stats else None
+    lse, sums = torch.empty((2, bsz, hq, n, 1), dtype=torch.float32, device=dev) if stats else (None, None)
     lib = _lib.load()
     # a workspace of this call's own: calls on other streams and captured graphs share nothing
     nbytes = _shared_ws_bytes(lib, bsz, n, hq, hkv, d, pre.rows, own.rows, fmt, dev.index)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     status = lib.tsb_tree_attn_shared(q.data_ptr(), sb, sh, st, fmt, ctypes.byref(pre), ctypes.byref(own), _ptr(lengths),
                                       _ptr(p), _ptr(bits_t), bsz, n, hq, hkv, d, tail_v, scale, out.data_ptr(), _ptr(lse),
-                                      ws.data_ptr(), nbytes, _stream(q))
+                                      _ptr(sums), ws.data_ptr(), nbytes, _stream(q))
     if status:
         check(status, "tsb_tree_attn_shared")
         return None
     if stats:
-        return out, lse[..., None], torch.ones_like(lse)[..., None]
+        return out, lse, sums
     return out
 
 
