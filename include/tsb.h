@@ -340,7 +340,8 @@ int tsb_add_rms_norm(const void *x, const void *r, const void *w, void *h_out, v
  * (q_norm / k_norm weights [D]) and mx.fast.rope (non-traditional, the first
  * rope_dims dims, base, scale) at positions[b*T + t]; queries go to q_out
  * [B, Hq, T, D]; keys and values are appended to the caches at rows
- * offsets[b] + t (capacity rows per (request, head)) in kv_format, quantized on
+ * offsets[b] + t (capacity rows per (request, head); a row outside the cache
+ * is not written) in kv_format, quantized on
  * append for the 8-bit formats (TSB_KV_REF_Q8_ROW as kv8.py:39-43, MLX g64 as
  * this library's quantizer). D == 256; rope_dims % 16 == 0. */
 int tsb_qkv_prep(const void *qkv, int ld, int B, int T, int Hq, int Hkv, int D, const void *q_norm,

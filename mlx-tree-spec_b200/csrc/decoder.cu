@@ -200,7 +200,8 @@ __global__ void __launch_bounds__(PREP_THREADS) qkv_prep_kernel(PrepArgs a) {
   const int b = m / a.T, t = m - b * a.T;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int pos = a.positions[m];
-  const size_t cache_row0 = (size_t)a.offsets[b] + t;
+  const long long cache_row0 = (long long)a.offsets[b] + t;
+  const bool in_cache = cache_row0 >= 0 && cache_row0 < a.cap;  // other rows are not written
   const uint16_t *row = a.qkv + (size_t)m * a.ld;
   const int nh = a.Hq + 2 * a.Hkv;
   // the node's rope angles pos * scale * base^(-j/half), j < half, once
@@ -224,12 +225,12 @@ __global__ void __launch_bounds__(PREP_THREADS) qkv_prep_kernel(PrepArgs a) {
       unpack8(*reinterpret_cast<const uint4 *>(row + (size_t)a.Hq * 512 + (size_t)g * 256 + 8 * lane), f);
       warp_rms_norm(f, a.k_norm, lane, a.eps);
       warp_rope(f, lane, a.rope_dims, cs_t, sn_t);
-      warp_append(a, a.k, a.ks, a.kb, ((size_t)b * a.Hkv + g) * a.cap + cache_row0, f, lane);
+      if (in_cache) warp_append(a, a.k, a.ks, a.kb, ((size_t)b * a.Hkv + g) * a.cap + cache_row0, f, lane);
     } else {
       const int g = hv - a.Hq - a.Hkv;
       unpack8(*reinterpret_cast<const uint4 *>(row + (size_t)a.Hq * 512 + (size_t)(a.Hkv + g) * 256 + 8 * lane),
               f);
-      warp_append(a, a.v, a.vs, a.vb, ((size_t)b * a.Hkv + g) * a.cap + cache_row0, f, lane);
+      if (in_cache) warp_append(a, a.v, a.vs, a.vb, ((size_t)b * a.Hkv + g) * a.cap + cache_row0, f, lane);
     }
   }
 }

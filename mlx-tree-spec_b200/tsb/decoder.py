@@ -21,10 +21,17 @@ is a synthetic model): N(0, 0.02) quantized to 4-bit g64, norm weights
 1 + N(0, 0.1). Rope follows a Qwen3-Next-style partial rotary layout (the
 first `rope_dims` of each head, base `rope_base`); the reference reads both
 from its model's config.
+
+`step` has all requests at one length. `step_shared` is the same layer stack for
+requests that share a long prefix and have their own rows behind it, of lengths
+that live on the device; `verify` goes on from there to the LM head, samples a
+token at every node, walks the trees and keeps the accepted rows, without a host
+read: the lengths it returns are the next step's, plus the next tree.
 """
 
 from __future__ import annotations
 
+from collections import namedtuple
 from dataclasses import dataclass
 
 import torch
@@ -33,6 +40,11 @@ from . import _lib, ops
 from ._lib import TSB_KV_BF16, TSB_KV_MLX_Q8_G64, TSB_KV_REF_Q8_ROW, check
 from .cache import KVCache, MLXQ8KVCache, Q8KVCache
 from .quant import quantize, quantize_g64, quantize_rows
+from .verify import sample, tree_accept
+
+# of VerifyDecoder.verify: tree_accept's path (B, T), n_keep (B,) and next_token (B,), the
+# sampled tokens (B, T) and the lengths (B,) after the commit, all int32 on the device
+Verified = namedtuple("Verified", "path n_keep next_token samples lengths")
 
 
 @dataclass
@@ -125,16 +137,74 @@ class VerifyDecoder:
         request and room for T more (their offset is set to prefix + T). The
         nodes' K/V are written at rows prefix .. prefix+T-1. Returns the final
         normed hidden states (B*T, hidden), a buffer reused by the next step."""
-        c = self.cfg
         b, t = parents.shape
-        m = b * t
-        dev = h_in.device
-        buf = self._buffers(b, t, dev)
-        lib = _lib.load()
-        st = torch.cuda.current_stream(dev).cuda_stream
+        buf = self._buffers(b, t, h_in.device)
         _, depth = ops.ancestor_bits(parents, depth=True)
         buf["positions"].copy_((depth + prefix).reshape(-1))
         buf["offsets"].fill_(prefix)
+
+        def attend(i, q, cache, scale, out):
+            return ops.tree_flash(q, cache, scale, parents=parents, out=out)
+
+        for cache in caches[:len(self.layers)]:
+            cache.offset = prefix + t
+        return self._layer_loop(h_in, b, t, buf, caches, attend)
+
+    def step_shared(self, h_in: torch.Tensor, parents: torch.Tensor, prefixes, caches,
+                    lengths: torch.Tensor) -> torch.Tensor:
+        """step for requests that share a prefix: prefixes, one cache of batch 1
+        per layer (all of one offset P), and each request's own rows in caches,
+        one per layer with the prefix's format. lengths int32 (B,) on the device:
+        a request's own rows with this step's T nodes, whose K/V are written at
+        own rows lengths[b] - T .. lengths[b] - 1 and which stand at positions
+        P + lengths[b] - T + depth. caches[i].offset bounds the lengths and is left
+        as it is (the capacity will do). The lengths are read on the device, so a
+        captured step serves every later one; they must lie in [T, offset] (rows
+        outside the cache are not written, whatever the lengths are)."""
+        b, t = parents.shape
+        shared = int(prefixes[0].offset)
+        if any(int(p.offset) != shared for p in prefixes):
+            raise ValueError("step_shared: every layer's prefix must have the same rows")
+        if len(prefixes) != len(self.layers) or len(caches) != len(self.layers):
+            raise ValueError(f"step_shared: {len(self.layers)} layers need as many prefixes and caches")
+        if (lengths.dtype != torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous()
+                or lengths.device != h_in.device):
+            raise ValueError(f"step_shared: lengths must be a contiguous int32 tensor ({b},) on {h_in.device}")
+        buf = self._buffers(b, t, h_in.device)
+        _, depth = ops.ancestor_bits(parents, depth=True)
+        torch.sub(lengths, t, out=buf["offsets"])
+        buf["positions"].copy_((depth + (buf["offsets"] + shared)[:, None]).reshape(-1))
+
+        def attend(i, q, cache, scale, out):
+            return ops.tree_flash_shared(q, prefixes[i], cache, scale, parents=parents, lengths=lengths, out=out)
+
+        return self._layer_loop(h_in, b, t, buf, caches, attend)
+
+    def verify(self, h_in: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, prefixes, caches,
+               lengths: torch.Tensor, lm_head, u: torch.Tensor, commit, temperature=1.0, top_k=0, top_p=1.0,
+               min_p=0.0) -> Verified:
+        """A whole verify step: step_shared, the LM head (lm_head: its quantized
+        (wq, scales, biases)), a token drawn at every node with the random numbers u
+        (B, T) (tsb.sample's filters; one value per node where a tensor), the walk
+        along the drafted tokens (B, T), and the commit of the accepted rows.
+        commit: PathCommit(caches), made once. Nothing is read on the host, so the
+        step can be captured and replayed."""
+        b, t = parents.shape
+        x = self.step_shared(h_in, parents, prefixes, caches, lengths)
+        logits = ops.quantized_matmul(x, *lm_head)
+        if logits is None:
+            raise RuntimeError("the quantized matmul declined the LM head's shape")
+        samples = sample(logits.view(b, t, -1), u, temperature, top_k, top_p, min_p)
+        if samples is None:
+            raise ValueError("verify: the vocabulary is larger than tsb.sample takes")
+        path, n_keep, next_token = tree_accept(tokens, parents, samples)
+        return Verified(path, n_keep, next_token, samples, commit(lengths, path, n_keep))
+
+    def _layer_loop(self, h_in, b: int, t: int, buf, caches, attend) -> torch.Tensor:
+        c = self.cfg
+        m = b * t
+        lib = _lib.load()
+        st = torch.cuda.current_stream(h_in.device).cuda_stream
         h, x, r = buf["h"], buf["x"], buf["r"]
         h.copy_(h_in)
         check(lib.tsb_add_rms_norm(_ptr(h), None, _ptr(self.layers[0]["input_norm"]), None, _ptr(x), m, c.hidden,
@@ -142,14 +212,13 @@ class VerifyDecoder:
         scale = c.d ** -0.5
         for i, lw in enumerate(self.layers):
             cache = caches[i]
-            cache.offset = prefix + t
             k, ks, kb, v, vs, vb = _planes(cache)
             ops.quantized_matmul_into(x, *lw["qkv"], buf["qkv"], c.qkv_rows)
             check(lib.tsb_qkv_prep(_ptr(buf["qkv"]), c.qkv_rows, b, t, c.hq, c.hkv, c.d, _ptr(lw["q_norm"]),
                                    _ptr(lw["k_norm"]), c.eps, _ptr(buf["positions"]), c.rope_dims, c.rope_base, 1.0,
                                    _ptr(buf["q"]), cache.kv_format, _ptr(k), _ptr(ks), _ptr(kb), _ptr(v), _ptr(vs),
                                    _ptr(vb), k.shape[2], _ptr(buf["offsets"]), st), "tsb_qkv_prep")
-            if ops.tree_flash(buf["q"], cache, scale, parents=parents, out=buf["attn"]) is None:
+            if attend(i, buf["q"], cache, scale, buf["attn"]) is None:
                 raise RuntimeError("tree attention declined the decoder's shape")
             check(lib.tsb_attn_gate(_ptr(buf["attn"]), _ptr(buf["qkv"]), c.qkv_rows, _ptr(buf["gated"]), b, t, c.hq,
                                     c.d, st), "tsb_attn_gate")
@@ -165,5 +234,5 @@ class VerifyDecoder:
         return x
 
 
-__all__ = ["DecoderConfig", "random_weights", "make_cache", "VerifyDecoder",
+__all__ = ["DecoderConfig", "random_weights", "make_cache", "VerifyDecoder", "Verified",
            "TSB_KV_BF16", "TSB_KV_MLX_Q8_G64", "TSB_KV_REF_Q8_ROW"]
