@@ -40,6 +40,8 @@ def _per_row(v, rows: int, dtype, name: str, device):
     if v.numel() != rows:
         raise ValueError(f"sample: {name} must have one value per row ({rows}), got {tuple(v.shape)}")
     if v.dtype != dtype:
+        if dtype == torch.int32 and v.dtype == torch.int64:
+            v = v.clamp(0, 2**31 - 1)  # a larger top_k is as good as none
         v = v.to(dtype)
     if not v.is_contiguous():
         v = v.contiguous()

@@ -245,3 +245,13 @@ def test_frequencies():
     p = torch.softmax(x[0].double(), 0)
     counts = torch.bincount(tokens.long(), minlength=5).double()
     assert ((counts - n * p).abs() <= 5 * (n * p * (1 - p)).sqrt()).all()
+
+
+def test_top_k_of_64_bits():
+    """Values past 32 bits keep everything, as any k past the vocabulary does."""
+    import tsb
+
+    x = torch.randn(4, 500, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3))
+    u = torch.tensor([0.9, 0.99, 0.3, 0.999], device="cuda")
+    k = torch.tensor([2**32 + 1, 2**40, -5, 2**31], device="cuda")
+    assert torch.equal(tsb.sample(x, u, top_k=k), tsb.sample(x, u))

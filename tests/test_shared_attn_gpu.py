@@ -309,3 +309,74 @@ def test_agrees_with_tree_flash():
     torch.cuda.synchronize()
     # each is off by at most 2^-8 (sum p|v| + |out|), and sum p|v| <= max|v|
     assert (one.float() - two.float()).abs().max() <= 4 * 2.0**-8 * v.float().abs().max()
+
+
+@pytest.mark.parametrize("fmt,b,n,hq,hkv,p_rows,lengths", [
+    ("bf16", 70, 1, 4, 2, 130, [1 + (37 * i) % 90 for i in range(70)]),        # single tokens, many requests to a block
+    ("bf16", 40, 3, 3, 3, 5, [3] * 39 + [2500]),                               # one request far longer than the others
+    ("bf16", 33, 2, 8, 8, 700, [2 + (101 * i) % 260 for i in range(33)]),      # 264 own units, more than pairs of CTAs
+    ("mlx_q8", 12, 32, 6, 1, 64, [32 + 64 * i for i in range(12)]),            # own rows outweigh the prefix
+    ("ref_q8", 3, 1, 2, 1, 6000, [900, 1, 0]),                                 # many splits of few rows
+    ("bf16", 5, 4, 4, 4, 3000, [0] * 5),                                       # no own rows at all
+    ("bf16", 1, 64, 64, 8, 1, [64]),                                           # two row blocks to a request, one prefix row
+], ids=lambda v: str(len(v)) if isinstance(v, list) else str(v))
+def test_schedules(fmt, b, n, hq, hkv, p_rows, lengths):
+    """Splits, chunks and their dealing out to the CTAs at the ends of what is possible."""
+    _run(fmt, b, n, hq, hkv, p_rows, lengths, seed=21)
+
+
+def test_a_request_does_not_touch_another():
+    """NaN and infinite queries of one request, whose rows are packed with the others', leave those as they were."""
+    import tsb
+
+    b, n, hq, hkv = 6, 5, 4, 2
+    prefix, cache, _ = _make("bf16", hkv, b, 400, 90, 400, 90, seed=13)
+    q = torch.randn(b, hq, n, D, device="cuda").bfloat16()
+    parents = torch.arange(-1, n - 1, device="cuda", dtype=torch.int32)
+    lengths = torch.tensor([5, 90, 33, 64, 65, 17], dtype=torch.int32, device="cuda")
+    want, lse, _ = tsb.tree_flash_shared(q, prefix, cache, D**-0.5, parents=parents, lengths=lengths, stats=True)
+    bad = q.clone()
+    bad[2] = float("nan")
+    bad[4, 0, 0, :3] = torch.tensor([float("inf"), -float("inf"), 1.0])
+    out, got, _ = tsb.tree_flash_shared(bad, prefix, cache, D**-0.5, parents=parents, lengths=lengths, stats=True)
+    torch.cuda.synchronize()
+    for i in (0, 1, 3, 5):
+        assert torch.equal(out[i], want[i]) and torch.equal(got[i], lse[i])
+    assert torch.equal(out[4, 1:], want[4, 1:]) and torch.equal(out[4, 0, 1:], want[4, 0, 1:])
+
+
+def test_refusals():
+    import tsb
+
+    b, n, hq, hkv = 2, 4, 4, 2
+    prefix, cache, _ = _make("bf16", hkv, b, 64, 32, 50, 20)
+    q8, _, _ = _make("ref_q8", hkv, b, 64, 32, 50, 20)
+    q = torch.randn(b, hq, n, D, device="cuda").bfloat16()
+    parents = torch.arange(-1, n - 1, device="cuda", dtype=torch.int32)
+    lengths = torch.full((b,), 9, dtype=torch.int32, device="cuda")
+    call = lambda q=q, prefix=prefix, cache=cache, parents=parents, **kw: tsb.tree_flash_shared(  # noqa: E731
+        q, prefix, cache, D**-0.5, parents=parents, **kw)
+    assert call() is not None
+    assert call(q=q.half()) is None and call(q=q[..., :128]) is None and call(q=q[:, :3]) is None and call(parents=None) is None
+    assert call(q=torch.zeros(b, hq, 65, D, device="cuda", dtype=torch.bfloat16), parents=torch.zeros(65, device="cuda", dtype=torch.int32)) is None
+    for bad in (lengths.long(), lengths[:1], lengths.cpu(), lengths.repeat(2)[::2]):
+        with pytest.raises(ValueError):
+            call(lengths=bad)
+    with pytest.raises(ValueError):  # mixed formats
+        call(prefix=q8)
+    with pytest.raises(ValueError):  # a prefix of two requests
+        call(prefix=cache)
+    with pytest.raises(ValueError):  # a cache of another batch
+        call(cache=prefix)
+    with pytest.raises(ValueError):
+        call(parents=parents[:3])
+    with pytest.raises(ValueError):
+        call(prefix=tsb.KVCache(prefix.keys, prefix.values, 65))
+    with pytest.raises(ValueError):
+        call(prefix=tsb.KVCache(prefix.keys[:, :, ::2], prefix.values[:, :, ::2], 3))
+    with pytest.raises(ValueError):
+        call(cache=tsb.KVCache(cache.keys.half(), cache.values.half(), 3))
+    with pytest.raises(ValueError):
+        call(out=torch.empty(b, hq, n, D, device="cuda"))
+    with pytest.raises(ValueError):
+        call(out=torch.empty(b, n, hq, D, device="cuda", dtype=torch.bfloat16).transpose(1, 2))
