@@ -304,9 +304,9 @@ def _kv_struct(cache, planes, bsz: int, hkv: int, d: int, device):
         raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
     words = fmt == TSB_KV_MLX_Q8_G64
     shape = (bsz, hkv, cap, d // 4 if words else d)
-    for name, t in (("keys", k), ("values", v)):
-        if t.shape != shape or not t.is_contiguous() or t.device != device:
-            raise _bad_plane(name, t, shape, device)
+    if (k.shape != shape or v.shape != shape or not k.is_contiguous() or not v.is_contiguous() or k.device != device
+            or v.device != device):
+        raise _bad_plane("keys and values", v if k.shape == shape and k.is_contiguous() else k, shape, device)
     if fmt == TSB_KV_BF16:
         if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
             raise _bad_plane("keys and values in bf16", v, shape, device)
@@ -401,10 +401,13 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
         q = q.clone(memory_format=torch.contiguous_format)
         sb, sh, st, sd = q.stride()
     if out is None:
-        out = torch.empty((bsz, hq, n, d), dtype=torch.bfloat16, device=dev)
+        out = torch.empty_strided((bsz, hq, n, d), (hq * n * d, n * d, d, 1), dtype=torch.bfloat16, device=dev)  # quicker than empty
     elif out.shape != queries.shape or out.dtype != torch.bfloat16 or not out.is_contiguous() or out.device != dev:
         raise ValueError("tree_flash_shared: out must be a contiguous bf16 tensor of the queries' shape")
-    lse, sums = torch.empty((2, bsz, hq, n, 1), dtype=torch.float32, device=dev) if stats else (None, None)
+    lse = sums = None
+    if stats:
+        lse = torch.empty_strided((bsz, hq, n, 1), (hq * n, n, 1, 1), dtype=torch.float32, device=dev)
+        sums = torch.empty_like(lse)
     lib = _lib.load()
     # a workspace of this call's own: calls on other streams and captured graphs share nothing
     nbytes = _shared_ws_bytes(lib, bsz, n, hq, hkv, d, pre.rows, own.rows, fmt, dev.index)

@@ -90,11 +90,11 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: 
     k_p, k_s, k_ref = _per_row(top_k, rows, torch.int32, "top_k", dev)
     p_p, p_s, p_ref = _per_row(top_p, rows, torch.float32, "top_p", dev)
     m_p, m_s, m_ref = _per_row(min_p, rows, torch.float32, "min_p", dev)
-    token = torch.empty(lead, dtype=torch.int32, device=dev)
-    logprob = torch.empty(lead, dtype=torch.float32, device=dev) if logprobs else None
+    if not u.is_contiguous():
+        u = u.contiguous()
+    token = torch.empty_like(u, dtype=torch.int32)
+    logprob = torch.empty_like(u) if logprobs else None
     if rows:
-        if not u.is_contiguous():
-            u = u.contiguous()
         status = _lib.load().tsb_sample(x.data_ptr(), dt, rows, vocab, stride, u.data_ptr(), t_p, t_s, k_p,
                                         min(max(int(k_s), 0), vocab), p_p, p_s, m_p, m_s, token.data_ptr(), _ptr(logprob),
                                         _stream(x))
