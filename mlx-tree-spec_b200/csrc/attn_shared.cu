@@ -849,20 +849,24 @@ __global__ void __launch_bounds__(256) tree_attn_shared_convert_kernel(const __g
   if (row0 >= n) return;
   const int c16 = threadIdx.x & 15;
   uint4 w[SH_CV_ROWS / 16];
+  uint16_t sc[SH_CV_ROWS / 16], bi[SH_CV_ROWS / 16];
 #pragma unroll
-  for (int i = 0; i < SH_CV_ROWS / 16; ++i) {
+  for (int i = 0; i < SH_CV_ROWS / 16; ++i) {  // all loads before the first use
     const int row = row0 + i * 16 + (threadIdx.x >> 4);
-    w[i] = row < n ? ldg_nc_v4(c.src[v] + ((size_t)head * c.cap + row) * SH_D + c16 * 16) : make_uint4(0u, 0u, 0u, 0u);
+    const size_t at = (size_t)head * c.cap + min(row, n - 1);
+    w[i] = ldg_nc_v4(c.src[v] + at * SH_D + c16 * 16);
+    if (MLX) {
+      sc[i] = __ldg(reinterpret_cast<const uint16_t *>(c.scale[v] + at) + (c16 >> 2));
+      bi[i] = __ldg(reinterpret_cast<const uint16_t *>(c.bias[v] + at) + (c16 >> 2));
+    }
   }
 #pragma unroll
   for (int i = 0; i < SH_CV_ROWS / 16; ++i) {
     const int row = row0 + i * 16 + (threadIdx.x >> 4);
     if (row >= n) break;
-    const size_t at = (size_t)head * c.cap + row;
     uint4 lo, hi;
     if (MLX) {
-      const uint16_t *sc = reinterpret_cast<const uint16_t *>(c.scale[v] + at), *bi = reinterpret_cast<const uint16_t *>(c.bias[v] + at);
-      const float s = bf16_bits_to_float(__ldg(sc + (c16 >> 2))), b = bf16_bits_to_float(__ldg(bi + (c16 >> 2)));
+      const float s = bf16_bits_to_float(sc[i]), b = bf16_bits_to_float(bi[i]);
       lo = dequant8_mlx(make_uint2(w[i].x, w[i].y), s, b);
       hi = dequant8_mlx(make_uint2(w[i].z, w[i].w), s, b);
     } else {
