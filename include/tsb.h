@@ -264,7 +264,7 @@ typedef struct {
  * Hq % Hkv == 0, 1 <= T <= 64, tail <= 64, scale > 0, B*Hq*T <= 2^22. No host
  * read of the lengths: the call can be captured in a graph and replayed with
  * others. `own->rows` bounds the lengths and sizes the launch. Workspace:
- * tsb_tree_attn_shared_workspace_bytes(), 16-byte aligned, for this call alone
+ * tsb_tree_attn_shared_workspace_bytes(), 32-byte aligned, for this call alone
  * until it completes. */
 size_t tsb_tree_attn_shared_workspace_bytes(int B, int T, int Hq, int Hkv, int D, int P, int own_rows,
                                             int kv_format);

@@ -820,7 +820,7 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
 // The valid rows of an 8-bit cache as bf16 rows [heads][rows][D]: MLX values
 // bf16(fmaf(code, s, b)), or the int8 codes themselves. 16 lanes have a row; bound
 // by memory (272 or 256 bytes read and 512 written per row).
-constexpr int SH_CV_ROWS = 64;  // rows of a CTA
+constexpr int SH_CV_ROWS = 32;  // rows of a CTA
 
 struct ShConvert {
   struct Cache {
@@ -873,9 +873,10 @@ __global__ void __launch_bounds__(256) tree_attn_shared_convert_kernel(const __g
       lo = convert8_s8(make_uint2(w[i].x, w[i].y));
       hi = convert8_s8(make_uint2(w[i].z, w[i].w));
     }
-    uint4 *dst = reinterpret_cast<uint4 *>(c.dst[v] + ((size_t)head * c.rows + row) * SH_D) + c16 * 2;
-    dst[0] = lo;
-    dst[1] = hi;
+    uint16_t *dst = c.dst[v] + ((size_t)head * c.rows + row) * SH_D + c16 * 16;
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(lo.x), "r"(lo.y), "r"(lo.z),
+                 "r"(lo.w), "r"(hi.x), "r"(hi.y), "r"(hi.z), "r"(hi.w)
+                 : "memory");
   }
 }
 
@@ -1095,7 +1096,7 @@ extern "C" int tsb_tree_attn_shared(const void *q, long long q_stride_b, long lo
   const size_t part = partial_bytes(p, B, T, Hq);
   const size_t need = tsb_tree_attn_shared_workspace_bytes(B, T, Hq, Hkv, D, P, own_rows, kv_format);
   if (need && (!ws || ws_bytes < need)) return TSB_EWORKSPACE;
-  if (!aligned(ws, 16)) return TSB_EINVAL;
+  if (!aligned(ws, 32)) return TSB_EINVAL;
 
   const size_t rows = (size_t)B * Hq * T;
   cudaStream_t stm = (cudaStream_t)stream;
