@@ -627,7 +627,7 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
       }
       // ---- the partial of the segment before, normalised
       if (had) {
-        const float inv = sum > 0.f ? 1.f / sum : 0.f;
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
         const long long off = had_valid ? (long long)(had_row * SH_D + odd * 128) : -1ll;
 #pragma unroll 1
         for (int c = 0; c < SH_D / 2 && had_rows; c += 32) {
@@ -654,7 +654,7 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
         if (lane == 0) cluster_arrive_on(o_free0);
         if (had_valid && odd == 0) {
           float2 *ml = reinterpret_cast<float2 *>(a.part_ml);
-          ml[had_row] = make_float2(m_ref, sum);  // sum 0: nothing visible, the partial is not read
+          ml[had_row] = make_float2(m_ref, sum);  // sum 0: nothing visible, the partial counts for nothing
           for (int s = 1; s < had_slots; ++s) ml[had_row + s * rows_all] = make_float2(-INFINITY, 0.f);
         }
       }
@@ -890,7 +890,7 @@ int launch_convert(const ShConvert &a, cudaStream_t st) {
 
 // ---------------------------------------------------------------- combine
 // out = sum_s w_s o_s, w_s = l_s 2^(m_s - m) / sum, over the prefix's splits and the
-// chunks that the request's length has. Partials with l = 0 are not read. A warp
+// chunks that the request's length has. Partials with l = 0 count for nothing. A warp
 // per row, eight of the 256 columns per lane; bound by the partials' bytes (from L2).
 constexpr int SH_CB_WARPS = 4;
 
@@ -905,55 +905,53 @@ tree_attn_shared_combine_kernel(const float *__restrict__ part_o, const float *_
   if (row >= rows) return;
   const int slots = splits + ceil_to(own_rows_of(lengths, row / rows_per_b, own_rows), chunk_rows);
   const float2 *ml = reinterpret_cast<const float2 *>(part_ml) + row;
-  float m = -INFINITY;
-  for (int s = lane; s < slots; s += 32) {
-    const float2 v = ml[(size_t)s * rows];
-    if (v.y > 0.f) m = fmaxf(m, v.x);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float den = 0.f;
+  float m = -INFINITY, den = 0.f;
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < slots; s0 += 32) {
-    float w = 0.f;
-    if (s0 + lane < slots) {
-      const float2 v = ml[(size_t)(s0 + lane) * rows];
-      if (v.y > 0.f) w = v.y * exp2f(v.x - m);
-    }
+    const int n = min(32, slots - s0);
+    const float2 v = lane < n ? ml[(size_t)(s0 + lane) * rows] : make_float2(-INFINITY, 0.f);
+    float4 x[4], y[4];  // four partials' loads in flight
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)(s0 + min(s + i, n - 1)) * rows + row) * SH_D) + lane;
+        x[i] = __ldg(src);
+        y[i] = __ldg(src + 32);
+      }
+    };
+    fetch(0);  // beside the weights, which may turn out to be 0
+    float top = v.y != 0.f ? v.x : -INFINITY;  // a sum of NaN stays one
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = fmaxf(top, m);
+    const float w = v.y != 0.f ? v.y * exp2f(v.x - top) : 0.f;
+    const float before = m == -INFINITY ? 0.f : exp2f(m - top);
+    m = top;
     float part = w;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) part += __shfl_xor_sync(0xffffffffu, part, o);
-    den += part;
-    const int n = min(32, slots - s0);
-    for (int s = 0; s < n; s += 4) {  // four partials' loads in flight
-      float ws[4];
-      float4 x[4], y[4];
+    den = fmaf(den, before, part);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] *= before;
+    for (int s = 0; s < n; s += 4) {
+      if (s > 0) fetch(s);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ws[i] = __shfl_sync(0xffffffffu, w, (s + i) & 31);
-        if (s + i >= n) ws[i] = 0.f;
-        x[i] = y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (ws[i] != 0.f) {
-          const float4 *src = reinterpret_cast<const float4 *>(part_o + ((size_t)(s0 + s + i) * rows + row) * SH_D) + lane;
-          x[i] = __ldg(src);
-          y[i] = __ldg(src + 32);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        acc[0] = fmaf(ws[i], x[i].x, acc[0]); acc[1] = fmaf(ws[i], x[i].y, acc[1]);
-        acc[2] = fmaf(ws[i], x[i].z, acc[2]); acc[3] = fmaf(ws[i], x[i].w, acc[3]);
-        acc[4] = fmaf(ws[i], y[i].x, acc[4]); acc[5] = fmaf(ws[i], y[i].y, acc[5]);
-        acc[6] = fmaf(ws[i], y[i].z, acc[6]); acc[7] = fmaf(ws[i], y[i].w, acc[7]);
+        const float ws = __shfl_sync(0xffffffffu, w, (s + i) & 31);
+        if (s + i >= n || ws == 0.f) continue;  // a partial of no weight may hold anything
+        acc[0] = fmaf(ws, x[i].x, acc[0]); acc[1] = fmaf(ws, x[i].y, acc[1]);
+        acc[2] = fmaf(ws, x[i].z, acc[2]); acc[3] = fmaf(ws, x[i].w, acc[3]);
+        acc[4] = fmaf(ws, y[i].x, acc[4]); acc[5] = fmaf(ws, y[i].y, acc[5]);
+        acc[6] = fmaf(ws, y[i].z, acc[6]); acc[7] = fmaf(ws, y[i].w, acc[7]);
       }
     }
   }
-  const float inv = den > 0.f ? 1.f / den : 0.f;
+  const float inv = den != 0.f ? 1.f / den : 0.f;
   uint2 *dst = reinterpret_cast<uint2 *>(out + (size_t)row * SH_D) + lane;
   dst[0] = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
   dst[32] = make_uint2(pack_bf16x2(acc[4] * inv, acc[5] * inv), pack_bf16x2(acc[6] * inv, acc[7] * inv));
   if (sums && lane == 0) sums[row] = 1.f;
-  if (lse && lane == 0) lse[row] = den > 0.f ? (m + log2f(den)) * 0.69314718055994531f : -INFINITY;
+  if (lse && lane == 0) lse[row] = den != 0.f ? (m + log2f(den)) * 0.69314718055994531f : -INFINITY;
 }
 
 // ---------------------------------------------------------------- plan

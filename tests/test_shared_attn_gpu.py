@@ -342,6 +342,7 @@ def test_a_request_does_not_touch_another():
     torch.cuda.synchronize()
     for i in (0, 1, 3, 5):
         assert torch.equal(out[i], want[i]) and torch.equal(got[i], lse[i])
+    assert torch.isnan(out[2]).all() and torch.isnan(got[2]).all()  # not passed off as a row that sees nothing
     assert torch.equal(out[4, 1:], want[4, 1:]) and torch.equal(out[4, 0, 1:], want[4, 0, 1:])
 
 
