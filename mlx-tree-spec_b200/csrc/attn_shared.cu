@@ -21,7 +21,7 @@
 // Measured (graph replay, 24 query and 4 KV heads): 12 requests x 32 nodes over 32K shared
 // rows + 1K own 216 us, 1.45 PFLOP/s, 0.87 of what a large matrix product reaches in a
 // burst and more than it sustains; 8 x 16 over 8K + 512: 37 us; 4 x 1 over 1K + 64:
-// 14 us, two launches of one tile each; 5 x 32 over 32K in 8 bits 135 us, 34 of them the
+// 14 us, two dependent launches around a tile or two; 5 x 32 over 32K in 8 bits 135 us, 34 of them the
 // conversion at 6.0 TB/s.
 //
 // With many packed rows the work is bound by the tensor cores: 64 keys x 128 rows
@@ -845,7 +845,6 @@ struct ShConvert {
   int hkv;
 };
 
-
 template <bool MLX>
 __global__ void __launch_bounds__(256) tree_attn_shared_convert_kernel(const __grid_constant__ ShConvert a) {
   griddep_wait();  // programmatic dependent: the caches are the previous kernels'
@@ -904,7 +903,7 @@ int launch_convert(const ShConvert &a, cudaStream_t st) {
 // chunks that the request's length has. Partials with l = 0 count for nothing. A warp
 // per row, eight of the 256 columns per lane. Bound by latency: a round trip to L2 for
 // the weights, with the first partials' loads beside it, and one for every four more
-// partials (3.5 us for 96 rows, 4.5 us for 3072 rows of 5 partials, 16 MB).
+// partials (3.5 us for 96 rows, 4.5 us for 24 heads of 8 x 16 nodes, 5 partials each).
 constexpr int SH_CB_WARPS = 4;
 
 __global__ void __launch_bounds__(SH_CB_WARPS * 32)

@@ -381,3 +381,22 @@ def test_refusals():
         call(out=torch.empty(b, hq, n, D, device="cuda"))
     with pytest.raises(ValueError):
         call(out=torch.empty(b, n, hq, D, device="cuda", dtype=torch.bfloat16).transpose(1, 2))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_no_rows_at_all(fmt):
+    """Both caches empty, their planes not read: zeros and -inf, where a call is the first to be captured too."""
+    import tsb
+
+    prefix, cache, _ = _make(fmt, 2, 3, 4, 4, 0, 0)
+    for c in (prefix, cache):
+        _poison([t for t in vars(c).values() if isinstance(t, torch.Tensor)], 0)
+    q = torch.randn(3, 4, 2, D, device="cuda").bfloat16()
+    parents = torch.tensor([-1, 0], dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse, _ = tsb.tree_flash_shared(q, prefix, cache, D**-0.5, parents=parents, stats=True)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not out.any() and torch.isneginf(lse).all()
