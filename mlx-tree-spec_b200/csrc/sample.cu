@@ -79,6 +79,7 @@ constexpr size_t kSliceBytes = 48 * 1024;  // of logits in a CTA, while there ar
 constexpr int kSliceMin = 4096;            // logits of a slice that is not split further
 constexpr double kMinTemperature = 8.673617379884035e-19;  // 2^-60
 constexpr double kMaxTemperature = 1.2676506002282294e30;  // 2^100
+constexpr double kMinTopP = 2.2250738585072014e-308;       // 2^-1022
 
 struct SampleArgs {
   const void *logits;
@@ -542,9 +543,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     if (a.staged) data = stage;  // a thread reads back what it wrote itself
   }
   double temperature = a.temperature ? (double)temperature_row : a.temperature_s;
-  const double p = a.top_p ? (double)p_row : a.top_p_s;
+  double p = a.top_p ? (double)p_row : a.top_p_s;
   const double floor_w = a.min_p ? (double)floor_row : a.min_p_s;
   const bool greedy = !(temperature > 0.0), use_p = p < 1.0, use_floor = floor_w > 0.0;
+  p = fmax(p, kMinTopP);  // top-p keeps at least the first token: no sum starts below a bound of zero
   bool use_k = k > 0 && k < a.vocab;
   temperature = fmin(fmax(temperature, kMinTemperature), kMaxTemperature);
   RowScale r;

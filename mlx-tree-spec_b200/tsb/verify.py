@@ -57,7 +57,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, logprobs: 
     prefix whose weight reaches top_p times theirs, of those the tokens with
     w_i >= min_p (always the first). The token is the first kept one whose
     cumulative weight exceeds u times the kept weight: u near 0 gives the likeliest.
-    temperature 0 is greedy. top_k <= 0, top_p >= 1 and min_p <= 0 are off.
+    temperature 0 is greedy. top_k <= 0, top_p >= 1 and min_p <= 0 are off; top_p <= 0 leaves the first token.
     Each parameter is a number or a tensor of one value per row.
 
     Returns int32 tokens (...,), or (tokens, logprobs) with float32 log
