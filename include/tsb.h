@@ -289,13 +289,13 @@ int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride
  * token's share of the kept weight. Each parameter is a device array [rows] or,
  * where that is NULL, the value beside it. temperature <= 0 or NaN: the first
  * token (greedy). Off: top_k <= 0 or >= vocab, top_p >= 1 or NaN, min_p <= 0 or
- * NaN. top_p <= 0 keeps the first token. u is clamped to [0, 1]. NaN and -inf
- * logits are never chosen, +inf ones share all the weight; a row with nothing to
- * choose gives token -1 and logprob -inf. Weights are integers of 23 bits times a power of 2^(1/32);
- * those of one power are summed as integers, the sums of the powers as 64-bit
- * floats in a fixed order, so results repeat bit for bit. Weights below 2^-43 of
- * the largest count as zero, and temperatures as the nearest in [2^-60, 2^100].
- * vocab <= 2^20. */
+ * NaN. top_p <= 0 keeps the first token. u is clamped to [0, 1]; 1 takes the last
+ * kept token. NaN and -inf logits are never chosen, +inf ones share all the
+ * weight; a row with nothing to choose gives token -1 and logprob -inf. Weights
+ * are integers of 23 bits times a power of 2^(1/32); those of one power are
+ * summed as integers, the sums of the powers as whole numbers of 2^-43 of the
+ * largest weight, so results repeat bit for bit. Weights below 2^-43 count as
+ * zero, and temperatures as the nearest in [2^-60, 2^100]. vocab <= 2^20. */
 int tsb_sample(const void *logits, int logits_dtype, int rows, int vocab, long long row_stride, const float *u,
                const float *temperature, double temperature_all, const int32_t *top_k, int top_k_all,
                const float *top_p, double top_p_all, const float *min_p, double min_p_all, int32_t *token,

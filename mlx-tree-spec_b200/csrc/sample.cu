@@ -30,10 +30,14 @@
 // 2^(-bin / 32) with m an integer of 23 bits: a float32 series of the exactly
 // reduced t, whose roundings are independent from token to token and do not add
 // up. Sums over a bin's tokens are sums of integers, so they do not depend on the
-// order of the atomics and results repeat bit for bit; sums over bins are taken in
-// 64-bit floats in a fixed order. m goes into two 32-bit shared-memory atomics of 12
-// and 11 bits (2^20 tokens do not overflow them); a 64-bit one would be a
-// compare-and-swap loop.
+// order of the atomics and results repeat bit for bit. m goes into two 32-bit
+// shared-memory atomics of 12 and 11 bits (2^20 tokens do not overflow them); a
+// 64-bit one would be a compare-and-swap loop.
+//   The running mass at a token is a whole number of 2^-43 too: the sum over the
+// bins before its own, and its bin's tokens up to it, whose sum of m is rounded to
+// such units once (`reach`). Whoever asks gets the same number, it never falls along
+// the order, and a bin without tokens adds nothing; so a bound that is itself a
+// running mass (what a filter keeps, at u = 1) is met at the token that it came from.
 //
 // Measured: one row of 131072 bf16 logits with top-k 50 and top-p 0.95 10.3 us; 128 such
 // rows with settings of their own 52 us (the bytes alone: 5.2 us); 48 rows of 100003
@@ -79,7 +83,6 @@ constexpr size_t kSliceBytes = 48 * 1024;  // of logits in a CTA, while there ar
 constexpr int kSliceMin = 4096;            // logits of a slice that is not split further
 constexpr double kMinTemperature = 8.673617379884035e-19;  // 2^-60
 constexpr double kMaxTemperature = 1.2676506002282294e30;  // 2^100
-constexpr double kMinTopP = 2.2250738585072014e-308;       // 2^-1022
 
 struct SampleArgs {
   const void *logits;
@@ -143,7 +146,7 @@ TSB_HD uint32_t logit_m(float x, uint32_t bin, const RowScale &r) {
   const float p = fmaf(fmaf(fmaf(z, 1.f / 6.f, 0.5f), z, 1.f), z * (float)kUnitM, 8388608.f + (float)kUnitM);
   return __float_as_uint(p) & 0x7FFFFFu;
 }
-// Weight of one unit of m in a bin.
+// Powers 2^(-i / 32).
 __constant__ double kOctave[kStep] = {
     1.0, 0.97857206208770013, 0.9576032806985737, 0.93708381705514999, 0.91700404320467123, 0.89735453750155359,
     0.8781260801866497, 0.85930964906123897, 0.8408964152537145, 0.82287773907698243, 0.80524516597462714,
@@ -152,17 +155,29 @@ __constant__ double kOctave[kStep] = {
     0.63452547859586661, 0.62092890603674202, 0.60762367999023449, 0.59460355750136054, 0.58186242938878875,
     0.5693943173783458, 0.55719337129794622, 0.54525386633262887, 0.53357020033841180, 0.52213689121370688,
     0.51094857432705836};
+// A mass is a whole number of 2^-43, the first token's 2^43; those of 2^20 tokens add
+// up to 2^63 and a little.
+constexpr u64 kOne = 1ull << 43;
+constexpr double kPerUnit = 1.1368683772161603e-13;  // 2^-43
+// What one unit of m is in a bin: of the first token's weight, and in units of a mass.
 // `octave` is a copy of kOctave in shared memory: lanes ask for different ones.
 TSB_HD double bin_unit(uint32_t bin, const double *octave) {
   return octave[bin % kStep] * __hiloint2double((int)(1023u - 22u - bin / kStep) << 20, 0);
+}
+TSB_HD double bin_scale(uint32_t bin, const double *octave) {
+  return octave[bin % kStep] * __hiloint2double((int)(1023u + 43u - 22u - bin / kStep) << 20, 0);
+}
+// The running mass (or, with a scale of 1, count) at a token: `before` its bin, and m of
+// its bin's tokens up to it.
+TSB_HD u64 reach(u64 before, u64 m, double scale) {
+  return before + (scale == 1.0 ? m : __double2ull_rn((double)m * scale));
 }
 TSB_HD double logit_mass(float x, const RowScale &r, const double *octave) {
   const uint32_t bin = logit_bin(x, r);
   return bin < (uint32_t)kBins ? (double)logit_m(x, bin, r) * bin_unit(bin, octave) : 0.0;
 }
 
-// Masses of tokens of several bins are added up as whole numbers of 2^-40, whose
-// sums do not depend on the list's order either.
+// With small top-k, weights are added up as whole numbers of 2^-40.
 constexpr double kListUnit = 1099511627776.0;
 TSB_HD u64 list_units(double mass) { return (u64)__double2ll_rn(mass * kListUnit); }
 
@@ -174,7 +189,7 @@ struct Shared {
     struct {
       unsigned int h0[kBins], h1[kBins];  // histogram: counts, or the low 12 and the high bits of m
     };
-    double sums[kBins];                   // CTA 0: running counts or masses up to and including a bin
+    u64 sums[kBins];                      // CTA 0: running counts or masses up to and including a bin
   };
   u64 list[kList];                        // tokens found; in CTA 0 its own from the front, the others' from the back
   ulonglong2 few[kFewest];                // tokens and their units of count or mass
@@ -183,13 +198,12 @@ struct Shared {
   double octave[kStep];
   float peer_top[kMaxCluster];
   float peer_cut[kMaxCluster];            // CTA 0
-  double peer_floor[kMaxCluster];         // CTA 0
+  unsigned int floor0[3], floor1[3];      // min-p's part of three bins: the low 12 and the high bits of m
+  u64 peer_floor[kMaxCluster][3];         // CTA 0
   unsigned int peer_ties[kMaxCluster];
   u64 red[kWarps], red2[kWarps];
-  double scan[kWarps];
-  u64 scan_units[kWarps];
-  double found_mass;
-  u64 found_token, temp;
+  u64 scan[kWarps];
+  u64 found_mass, found_token, temp, last;
   int found;
   unsigned int mine, others, base, few_n, first;
   // written by CTA 0 into every CTA
@@ -260,32 +274,31 @@ TSB_HD void for_hits(const T *data, int off, int n, P test, F f) {
       });
 }
 
-// Sum and inclusive scans over the block, in a fixed order.
-TSB_HD double block_sum(double v, Shared &s) {
+// Sums and inclusive scans over the block.
+TSB_HD u64 block_sum(u64 v, Shared &s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   __syncthreads();
   if (threadIdx.x % 32 == 0) s.scan[threadIdx.x / 32] = v;
   __syncthreads();
-  double all = 0.0;
+  u64 all = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) all += s.scan[w];
   return all;
 }
-template <typename V>
-TSB_HD V block_scan(V v, V *per_warp) {
+TSB_HD u64 block_scan(u64 v, Shared &s) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const V up = __shfl_up_sync(0xffffffffu, v, o);
+    const u64 up = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += up;
   }
   __syncthreads();
-  if (lane == 31) per_warp[warp] = v;
+  if (lane == 31) s.scan[warp] = v;
   __syncthreads();
-  V before = V(0);
+  u64 before = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) before += w < warp ? per_warp[w] : V(0);
+  for (int w = 0; w < kWarps; ++w) before += w < warp ? s.scan[w] : 0ull;
   return before + v;
 }
 
@@ -329,25 +342,26 @@ __device__ __noinline__ void put_in_order(Shared &s, int n) {
   }
   __syncthreads();
 }
-// The place in that order of the token with which before + running units * unit
-// reaches bound: the last one that starts below it.
-TSB_HD int cross(Shared &s, int n, double before, double unit, double bound) {
+// The place in that order of the token with which the running count or mass reaches
+// bound: the last one that starts below it. `m`: the units before the first of them.
+TSB_HD int cross(Shared &s, int n, u64 before, u64 m, double scale, u64 bound) {
   if (threadIdx.x == 0) s.found = 0;
   __syncthreads();
   const int i = threadIdx.x;
-  if (i > 0 && i < n && s.up_to[i] > s.up_to[i - 1] && before + (double)s.up_to[i - 1] * unit < bound) atomicMax(&s.found, i);
+  if (i > 0 && i < n && s.up_to[i] > s.up_to[i - 1] && reach(before, m + s.up_to[i - 1], scale) < bound) atomicMax(&s.found, i);
   __syncthreads();
   return s.found;
 }
 
 // CTA 0: the first of the n listed tokens of `bin` (of any bin for bin < 0, counts
-// only) at or above floor_token, along the order, with which `before` plus the
-// running count or mass reaches bound; into s.found_token and s.found_mass (what has
+// only) at or above floor_token, along the order, with which the running count or
+// mass (`before` the bin) reaches bound; into s.found_token and s.found_mass (what has
 // been reached with it).
-__device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, bool by_count, double bound,
-                                    double before, const RowScale &r) {
+__device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, bool by_count, u64 bound, u64 before,
+                                    const RowScale &r) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const double unit = by_count ? 1.0 : bin_unit((uint32_t)bin, s.octave);
+  const double scale = by_count ? 1.0 : bin_scale((uint32_t)bin, s.octave);
+  u64 base = 0;  // units of the bin's tokens that have been passed
   u64 lo = floor_token, hi = ~0ull;
   bool by_t = bin >= 0;  // first by t inside the bin, which is known; then by the tokens' own range
   // a token's sub-bin by t: the fraction that logit_bin rounds away, of 256 parts
@@ -401,16 +415,16 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
     }
     __syncthreads();
     const u64 own = (u64)s.sub0[tid] + ((u64)s.sub1[tid] << 12);
-    const u64 up = block_scan(own, s.scan_units);
+    const u64 up = base + block_scan(own, s);
     // the last sub-bin that starts below the bound holds it
-    if (own && before + (double)(up - own) * unit < bound) atomicMax(&s.found, tid);
+    if (own && reach(before, up - own, scale) < bound) atomicMax(&s.found, tid);
     __syncthreads();
     if (tid == s.found) {
-      s.found_mass = before + (double)(up - own) * unit;
+      s.last = up - own;
       s.temp = by_count ? own : own / (kUnitM - (kUnitM >> 6)) + 1;  // no more tokens than this: m > 2^22 * 63 / 64
     }
     __syncthreads();
-    before = s.found_mass;
+    base = s.last;
     few = s.temp <= (u64)kFewest || (!by_t && shift == 0);
     if (by_t) {
       by_t_sub = s.found;
@@ -434,24 +448,24 @@ __device__ __noinline__ void narrow(Shared &s, int n, int bin, u64 floor_token, 
   __syncthreads();
   const int have = (int)s.few_n;
   put_in_order(s, have);
-  const int at = cross(s, have, before, unit, bound);
+  const int at = cross(s, have, before, base, scale, bound);
   if (tid == 0) {
     s.found_token = have ? s.order[at] : 0;
-    s.found_mass = have ? before + (double)s.up_to[at] * unit : before;
+    s.found_mass = reach(before, have ? base + s.up_to[at] : base, scale);
   }
   __syncthreads();
 }
 
 // CTA 0: running sums of the histogram; returns the whole.
-__device__ __noinline__ double run_sums(Shared &s, bool masses) {
-  double v[kBinsPerThread], run = 0.0;
+__device__ __noinline__ u64 run_sums(Shared &s, bool masses) {
+  u64 v[kBinsPerThread], run = 0;
 #pragma unroll
   for (int i = 0; i < kBinsPerThread; ++i) {
     const int bin = threadIdx.x * kBinsPerThread + i;
-    v[i] = bin >= kBins ? 0.0 : masses ? (double)((u64)s.h0[bin] + ((u64)s.h1[bin] << 12)) * bin_unit(bin, s.octave) : (double)s.h0[bin];
+    v[i] = bin >= kBins ? 0ull : masses ? reach(0, (u64)s.h0[bin] + ((u64)s.h1[bin] << 12), bin_scale(bin, s.octave)) : (u64)s.h0[bin];
     run += v[i];
   }
-  double up = block_scan(run, s.scan) - run;
+  u64 up = block_scan(run, s) - run;
 #pragma unroll
   for (int i = 0; i < kBinsPerThread; ++i) {
     const int bin = threadIdx.x * kBinsPerThread + i;
@@ -461,16 +475,16 @@ __device__ __noinline__ double run_sums(Shared &s, bool masses) {
   __syncthreads();
   return s.sums[kBins - 1];
 }
-TSB_HD double before_bin(const Shared &s, int bin) { return bin ? s.sums[bin - 1] : 0.0; }
+TSB_HD u64 before_bin(const Shared &s, int bin) { return bin > 0 ? s.sums[bin - 1] : 0ull; }
 // CTA 0: the bin in which the running sum reaches bound (the last that adds to it, if none does).
-__device__ __noinline__ int find_bin(Shared &s, double bound) {
+__device__ __noinline__ int find_bin(Shared &s, u64 bound) {
   if (threadIdx.x == 0) s.found = 0;
   __syncthreads();
-  bound = fmin(bound, s.sums[kBins - 1]);
+  bound = min(bound, s.sums[kBins - 1]);
 #pragma unroll
   for (int bin = threadIdx.x; bin < kBins; bin += kThreads) {
-    const double here = s.sums[bin], before = before_bin(s, bin);
-    if (here > before && here >= bound && before < bound) atomicMax(&s.found, bin);
+    const u64 here = s.sums[bin], before = before_bin(s, bin);
+    if (here >= bound && before < bound) atomicMax(&s.found, bin);
   }
   __syncthreads();
   const int bin = s.found;
@@ -479,16 +493,28 @@ __device__ __noinline__ int find_bin(Shared &s, double bound) {
 }
 
 // u's bound on the running mass, which the sample's cumulative mass exceeds: the
-// next number above u * total. Past the last token it is the total.
-TSB_HD double sample_bound(float u, double total) {
-  const double want = u > 0.f ? (double)u * total : 0.0;
-  return fmin(__longlong_as_double(__double_as_longlong(want) + 1), total);
+// next whole number above u * total. Past the last token it is the total.
+TSB_HD u64 sample_bound(float u, u64 total) {
+  const double want = u > 0.f ? (double)u * (double)total : 0.0;
+  return want < (double)total ? min(__double2ull_rd(want) + 1, total) : total;
 }
-// Tokens of equal weight w that make up `mass`, at least one.
-TSB_HD double ties_for(double mass, double w) { return fmax(ceil(mass / w), 1.0); }
-// No more tokens than this make up `mass` in a bin (2^-22 * 0.97 is below any m's share of a unit).
-TSB_HD float most_tokens(double mass, int bin) {
-  return (float)mass * exp2f((float)bin * (1.f / kStep)) * 1.03f + 1.f;
+// top-p's bound on it, which the mass of the kept tokens reaches: at least one, which
+// keeps the first token.
+TSB_HD u64 top_p_bound(double p, u64 total) {
+  return min(max(__double2ull_ru(fmax(p, 0.0) * (double)total), 1ull), total);
+}
+// Of tokens of m each in one bin, behind `base` units of it: how many reach bound, one of `most` at least.
+TSB_HD u64 ties_for(u64 before, u64 base, uint32_t m, u64 most, double scale, u64 bound) {
+  const double missing = bound > reach(before, base, scale) ? (double)(bound - reach(before, base, scale)) : 0.0;
+  u64 j = min(max(__double2ull_ru(missing / ((double)m * scale)), 1ull), most);
+  while (j > 1 && reach(before, base + (j - 1) * m, scale) >= bound) --j;  // the rounding of a unit: a step or two
+  while (j < most && reach(before, base + j * m, scale) < bound) ++j;
+  return j;
+}
+// No more tokens than this make up `mass` in a bin: m > 0.989 * 2^22, and the mass was
+// rounded by half a unit, half of the smallest weight.
+TSB_HD uint32_t most_tokens(u64 mass, int bin) {
+  return (uint32_t)((float)mass * (float)kPerUnit * exp2f((float)bin * (1.f / kStep)) * 1.03f) + 1;
 }
 
 TSB_HD void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
@@ -507,7 +533,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
   const int row = (int)blockIdx.x / ctas;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   if (tid == 0) { s.mine = 0; s.others = 0; s.first = 0xffffffffu; s.overflow = 0; }
-  for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;  // h0 and h1
+  if (tid < 3) s.floor0[tid] = s.floor1[tid] = 0;
+  for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;  // h0 and h1
   if (tid < kStep) s.octave[tid] = kOctave[tid];
   cluster_arrive();  // waited for before the first access to another CTA's shared memory
   griddep_wait();    // programmatic dependent: the logits are the previous kernel's
@@ -543,10 +570,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     if (a.staged) data = stage;  // a thread reads back what it wrote itself
   }
   double temperature = a.temperature ? (double)temperature_row : a.temperature_s;
-  double p = a.top_p ? (double)p_row : a.top_p_s;
+  const double p = a.top_p ? (double)p_row : a.top_p_s;
   const double floor_w = a.min_p ? (double)floor_row : a.min_p_s;
   const bool greedy = !(temperature > 0.0), use_p = p < 1.0, use_floor = floor_w > 0.0;
-  p = fmax(p, kMinTopP);  // top-p keeps at least the first token: no sum starts below a bound of zero
   bool use_k = k > 0 && k < a.vocab;
   temperature = fmin(fmax(temperature, kMinTemperature), kMaxTemperature);
   RowScale r;
@@ -637,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
       __syncthreads();
       for (int e = tid; e < m; e += kThreads) atomicAdd(&s.sub0[sub_of(listed(s, e))], 1u);
       __syncthreads();
-      const u64 own = s.sub0[tid], up = block_scan(own, s.scan_units);
+      const u64 own = s.sub0[tid], up = block_scan(own, s);
       if (own && up - own < (u64)k) atomicMax(&s.found, tid);
       __syncthreads();
       int last = s.found;
@@ -645,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
       __syncthreads();
       u64 floor_token = 0;
       if (s.temp > (u64)kFewest) {  // many in one part of the histogram: find the k-th itself
-        narrow(s, m, -1, 0, true, (double)k, 0.0, r);
+        narrow(s, m, -1, 0, true, (u64)k, 0, r);
         floor_token = s.found_token;
         last = kSub;
         if (tid == 0) s.few_n = 0;
@@ -665,19 +691,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
       if (have == 0) {
         if (tid == 0) nothing();
       } else {
-        double kept = (double)s.up_to[have - 1];
-        if (use_p) kept = (double)s.up_to[cross(s, have, 0.0, 1.0, p * kept)];
+        u64 kept = s.up_to[have - 1];
+        if (use_p) kept = s.up_to[cross(s, have, 0, 0, 1.0, top_p_bound(p, kept))];
         if (use_floor) {  // of those in order the ones up to the last of weight >= min_p, at least the first
           __syncthreads();
           if (tid == 0) s.found = 0;
           __syncthreads();
           if (tid < have && (double)(s.up_to[tid] - (tid ? s.up_to[tid - 1] : 0ull)) >= floor_w * kListUnit) atomicMax(&s.found, tid);
           __syncthreads();
-          kept = fmin(kept, (double)s.up_to[s.found]);
+          kept = min(kept, s.up_to[s.found]);
         }
         __syncthreads();
-        const int at = cross(s, have, 0.0, 1.0, sample_bound(u, kept));
-        if (tid == 0) emit(token_logit(s.order[at]), token_index(s.order[at]), kept / kListUnit);
+        const int at = cross(s, have, 0, 0, 1.0, sample_bound(u, kept));
+        if (tid == 0) emit(token_logit(s.order[at]), token_index(s.order[at]), (double)kept / kListUnit);
       }
       return;
     }
@@ -730,10 +756,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     }
   };
   // All CTAs: token number `tie` (CTA 0 knows it) of those with this logit, in index order.
-  auto pick = [&](float v, double kept, auto tie_of) {
+  auto pick = [&](float v, u64 kept, auto tie_of) {
     unsigned int ties = 0;
     for_logits<T>(data, off, n, [&](int, float e) { ties += e == v; });
-    ties = (unsigned int)block_sum((double)ties, s);
+    ties = (unsigned int)block_sum(ties, s);
     if (tid == 0) head->peer_ties[rank] = ties;
     cluster_barrier();
     if (rank == 0 && tid == 0) {
@@ -747,14 +773,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
         peer->pick_rank = q;
         peer->pick_tie = (int)tie;
       }
-      emit(v, -1, kept);
+      emit(v, -1, (double)kept * kPerUnit);
     }
     cluster_barrier();
     if (rank != s.pick_rank) return;
     unsigned int seen = 0;  // ties before this block of tokens
     for (int at = 0; at < n; at += kThreads) {
       const bool hit = at + tid < n && to_float(data[off + at + tid]) == v;
-      const unsigned int up = (unsigned int)block_scan(hit ? 1.0 : 0.0, s.scan);
+      const unsigned int up = (unsigned int)block_scan(hit ? 1ull : 0ull, s);
       if (hit && seen + up - 1 == (unsigned int)s.pick_tie) a.token[row] = lo + at + tid;
       for (int q = 0; q < kWarps; ++q) seen += (unsigned int)s.scan[q];
       if (seen > (unsigned int)s.pick_tie) return;
@@ -762,11 +788,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
   };
 
   if (top == INFINITY) {  // the +inf logits share all the weight equally
-    pick(top, 0.0, [&](unsigned int all, double &kept) {
-      kept = use_k ? fmin((double)all, (double)k) : (double)all;
-      if (use_p) kept = ties_for(p * kept, 1.0);
-      if (use_floor && floor_w > 1.0) kept = 1.0;
-      return ties_for(sample_bound(u, kept), 1.0) - 1.0;
+    pick(top, 0, [&](unsigned int all, u64 &kept) {
+      u64 n = use_k ? min((u64)all, (u64)k) : (u64)all;
+      if (use_p) n = top_p_bound(p, n);
+      if (use_floor && floor_w > 1.0) n = 1;
+      kept = n * kOne;
+      return sample_bound(u, n) - 1;
     });
     return;
   }
@@ -800,24 +827,63 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     });
     push(true);
   };
-  // The mass of the weights that min-p keeps, added up in CTA 0: a prefix of the bins, and part of one.
+  // The mass of the weights that min-p keeps, a prefix of the bins and part of one, which
+  // is one of three: t of min_p, in steps of 1 / kStep, is known to a small part of a step,
+  // and a bin's tokens are within half of one. What of their m stays, of the tokens that
+  // for_each gives, is added up once a row, into floor0 and floor1.
+  int floor_bin = 0;  // the first of the three
+  if (use_floor) {
+    const float t = -log2f((float)floor_w) * (float)kStep;
+    floor_bin = (int)fminf(fmaxf(rintf(t), 0.f), (float)(kBins + 1)) - 1;
+  }
+  auto floor_units = [&](auto for_each) {
+    uint32_t m0[3] = {0, 0, 0}, m1[3] = {0, 0, 0};
+    for_each([&](float v) {
+      const uint32_t bin = logit_bin(v, r), at = bin - (uint32_t)floor_bin;
+      if (at >= 3u || bin >= (uint32_t)kBins) return;
+      const uint32_t m = logit_m(v, bin, r);
+      if ((double)m * bin_unit(bin, s.octave) < floor_w) return;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        m0[i] += at == (uint32_t)i ? m & 4095u : 0u;
+        m1[i] += at == (uint32_t)i ? m >> 12 : 0u;
+      }
+    });
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      if (!__any_sync(0xffffffffu, m1[i] != 0)) continue;  // m has 22 bits and more
+      const uint32_t low = __reduce_add_sync(0xffffffffu, m0[i]), high = __reduce_add_sync(0xffffffffu, m1[i]);
+      if (lane == 0) {
+        atomicAdd(&s.floor0[i], low);
+        atomicAdd(&s.floor1[i], high);
+      }
+    }
+    __syncthreads();
+  };
+  auto floor_of = [&](int i) { return (u64)s.floor0[i] + ((u64)s.floor1[i] << 12); };
+  auto floor_mass = [&](auto units) {  // CTA 0: with the running masses
+    u64 mass = before_bin(s, floor_bin);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const u64 m = units(i);
+      if (m) mass = reach(before_bin(s, floor_bin + i), m, bin_scale(floor_bin + i, s.octave));
+    }
+    return max(mass, kOne);  // always the first
+  };
   auto add_floor = [&]() {
-    // tokens past this bin weigh less (log2 is good to a small part of a bin)
-    const uint32_t floor_bin = (uint32_t)fminf(fmaxf(-log2f((float)floor_w), 0.f) * kStep + 2.f, (float)(kBins - 1));
-    double above = 0.0;
-    for_hits<T>(
-        data, off, n, [&](float v) { return logit_bin(v, r) <= floor_bin; },
-        [&](int, float v) {
-          const double w = logit_mass(v, r, s.octave);
-          if (w >= floor_w) above += w;
-        });
-    above = block_sum(above, s);
-    if (tid == 0) head->peer_floor[rank] = above;
+    floor_units([&](auto take) {
+      for_hits<T>(
+          data, off, n, [&](float v) { return logit_bin(v, r) - (uint32_t)floor_bin < 3u; }, [&](int, float v) { take(v); });
+    });
+    if (tid < 3) head->peer_floor[rank][tid] = floor_of(tid);
   };
   auto floor_sum = [&]() {
-    double above = 0.0;
-    for (int q = 0; q < ctas; ++q) above += s.peer_floor[q];
-    return above;
+    return floor_mass([&](int i) {
+      u64 m = 0;
+      for (int q = 0; q < ctas; ++q) m += s.peer_floor[q][i];
+      return m;
+    });
   };
   auto gather = [&](int b0, int b1) {  // all CTAs, into CTA 0's list
     for_hits<T>(
@@ -835,32 +901,31 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
   cluster_barrier();
 
   // ---- 3. what to gather: CTA 0 decides
-  double total = 0.0, above_floor = 0.0;
+  u64 total = 0, above_floor = 0;
   int k_bin = 0;
-  double k_before = 0.0, k_in = 0.0;  // tokens before and in top-k's bin
+  u64 k_before = 0, k_in = 0;  // tokens before and in top-k's bin
   if (rank == 0) {
     total = run_sums(s, !use_k);
     if (use_k) {
-      use_k = (double)k < total;  // else every token with a mass is among the first k
-      k_bin = use_k ? find_bin(s, (double)k) : kBins - 1;
+      use_k = (u64)k < total;  // else every token with a mass is among the first k
+      k_bin = use_k ? find_bin(s, (u64)k) : kBins - 1;
       k_before = before_bin(s, k_bin);
       k_in = s.sums[k_bin] - k_before;
-      tell(k_before + k_in <= (double)kList ? kFew : kSlow, 0, k_bin);
+      tell(k_before + k_in <= (u64)kList ? kFew : kSlow, 0, k_bin);
     } else {
       int b0 = 0, b1;
       if (use_p) {
-        b1 = find_bin(s, p * total);
+        b1 = find_bin(s, top_p_bound(p, total));
       } else {
         if (use_floor) above_floor = floor_sum();
-        b0 = b1 = find_bin(s, sample_bound(u, use_floor ? fmin(total, fmax(above_floor, 1.0)) : total));
+        b0 = b1 = find_bin(s, sample_bound(u, use_floor ? min(total, above_floor) : total));
       }
-      double tokens = 0.0;  // a bound on the tokens of the bins
+      uint32_t tokens = 0;  // a bound on the tokens of the bins
       for (int bin = b0 + tid; bin <= b1; bin += kThreads) {
-        const double mass = s.sums[bin] - before_bin(s, bin);
-        if (mass > 0.0) tokens += (double)most_tokens(mass, bin);
+        const u64 mass = s.sums[bin] - before_bin(s, bin);
+        if (mass) tokens += most_tokens(mass, bin);
       }
-      tokens = block_sum(tokens, s);
-      tell(tokens <= (double)kList ? kFew : kSlow, b0, b1);
+      tell(block_sum(tokens, s) <= (u64)kList ? kFew : kSlow, b0, b1);
     }
   }
   cluster_barrier();
@@ -870,14 +935,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     if (rank != 0) return;
     const int m = min((int)(s.mine + s.others), kList);
     u64 floor_token = 0;
-    double kept = total;
+    u64 kept = total;
     if (counted) {
       // the list holds the first k, or every token with a mass: their masses by bin
       if (use_k) {
-        narrow(s, m, k_bin, 0, true, (double)k, k_before, r);
+        narrow(s, m, k_bin, 0, true, (u64)k, k_before, r);
         floor_token = s.found_token;
       }
-      for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;
+      for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;
       __syncthreads();
       for (int e = tid; e < m; e += kThreads) {
         const u64 t = listed(s, e);
@@ -890,34 +955,34 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
       kept = run_sums(s, true);
     }
     if (use_p) {
-      const double bound = p * kept;
+      const u64 bound = top_p_bound(p, kept);
       const int bin = find_bin(s, bound);
       narrow(s, m, bin, floor_token, false, bound, before_bin(s, bin), r);
-      kept = fmin(kept, s.found_mass);
+      kept = s.found_mass;
     }
     if (use_floor) {
       if (counted || use_p) {  // min-p keeps a prefix of the order: what of it is in the list decides
-        double above = 0.0;
+        floor_units([&](auto take) {
 #pragma unroll 1
-        for (int e = tid; e < m; e += kThreads) {
-          const u64 t = listed(s, e);
-          const double w = t >= floor_token ? logit_mass(token_logit(t), r, s.octave) : 0.0;
-          above += w >= floor_w ? (double)list_units(w) : 0.0;
-        }
-        above_floor = block_sum(above, s) / kListUnit;
+          for (int e = tid; e < m; e += kThreads) {
+            const u64 t = listed(s, e);
+            if (t >= floor_token) take(token_logit(t));
+          }
+        });
+        above_floor = floor_mass(floor_of);
       }
-      kept = fmin(kept, fmax(above_floor, 1.0));
+      kept = min(kept, above_floor);
     }
-    const double bound = sample_bound(u, kept);
+    const u64 bound = sample_bound(u, kept);
     const int bin = find_bin(s, bound);
     narrow(s, m, bin, floor_token, false, bound, before_bin(s, bin), r);
-    if (tid == 0) emit(token_logit(s.found_token), token_index(s.found_token), kept);
+    if (tid == 0) emit(token_logit(s.found_token), token_index(s.found_token), (double)kept * kPerUnit);
     return;
   }
 
   // ---- many candidates: one bound after the other, each resolved inside its bin
   if (counted) {  // the masses are still to be added up
-    for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0.0;
+    for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;
     cluster_barrier();
     add_masses();
   }
@@ -927,31 +992,32 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     if (counted) total = run_sums(s, true);
     if (use_floor) above_floor = floor_sum();
   }
-  double kept = total;  // CTA 0
+  u64 kept = total;  // CTA 0
   for (int stage = 0; stage < 3; ++stage) {  // top-k, top-p, u
     if (stage == 0 ? !counted : stage == 1 && !use_p) continue;
-    double bound = 0.0, mass_before = 0.0, count_before = 0.0;
+    u64 bound = 0, mass_before = 0, count_before = 0;
     if (rank == 0) {
-      if (stage == 2 && use_floor) kept = fmin(kept, fmax(above_floor, 1.0));
+      if (stage == 2 && use_floor) kept = min(kept, above_floor);
       int bin;
       if (stage == 0) {
-        bound = (double)k;
+        bound = (u64)k;
         bin = k_bin;
         count_before = k_before;
       } else {
-        bound = stage == 1 ? p * kept : sample_bound(u, kept);
+        bound = stage == 1 ? top_p_bound(p, kept) : sample_bound(u, kept);
         bin = find_bin(s, bound);
       }
       mass_before = before_bin(s, bin);
-      const double tokens = stage == 0 ? k_in : (double)most_tokens(s.sums[bin] - mass_before, bin);
+      const u64 tokens = stage == 0 ? k_in : most_tokens(s.sums[bin] - mass_before, bin);
       // nothing to resolve where every token with a mass is kept
-      const int mode = stage == 0 && !use_k ? kNoMass : tokens <= (double)kList ? kOneBin : kRadix;
+      const int mode = stage == 0 && !use_k ? kNoMass : tokens <= (u64)kList ? kOneBin : kRadix;
       if (tid == 0) s.others = 0;
       tell(mode, bin, bin);
     }
     if (tid == 0) s.mine = 0;
     cluster_barrier();
     const int mode = s.mode, bin = s.lo;
+    const double scale = bin_scale((uint32_t)bin, s.octave);
     if (mode == kNoMass) {
       cluster_barrier();  // the plan has been read: CTA 0 may write the next one
       continue;
@@ -964,16 +1030,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
       narrow(s, m, bin, 0, stage == 0, bound, stage == 0 ? count_before : mass_before, r);
       const u64 token = s.found_token;
       if (stage == 2) {
-        if (tid == 0) emit(token_logit(token), token_index(token), kept);
+        if (tid == 0) emit(token_logit(token), token_index(token), (double)kept * kPerUnit);
       } else if (stage == 1) {
-        kept = fmin(kept, s.found_mass);
+        kept = s.found_mass;
       } else {  // the mass of the first k
-        double mass = 0.0;
+        u64 units = 0;
         for (int e = tid; e < m; e += kThreads) {
           const u64 t = listed(s, e);
-          if (t >= token) mass += (double)list_units(logit_mass(token_logit(t), r, s.octave));
+          if (t >= token) units += logit_m(token_logit(t), (uint32_t)bin, r);
         }
-        kept = mass_before + block_sum(mass, s) / kListUnit;
+        kept = reach(mass_before, block_sum(units, s), scale);
       }
       __syncthreads();
       continue;
@@ -981,8 +1047,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     // radix descent over the keys of the bin, eight bits at a time: counts in the
     // narrowing histogram's first half, m in two words of the list
     unsigned int *const low = reinterpret_cast<unsigned int *>(s.list), *const high = low + kSub;
-    const double unit = bin_unit((uint32_t)bin, s.octave);
     uint32_t prefix = 0;
+    u64 base_m = 0, base_c = 0, ties = 0;  // CTA 0: of the bin's tokens before the prefix's, and (at the end) how many have it
     for (int shift = 24; shift >= 0; shift -= 8) {
       s.sub0[tid] = 0;
       low[tid] = 0;
@@ -1007,18 +1073,17 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
           c += peer->sub0[digit];
           m += (u64)words[digit] + ((u64)words[kSub + digit] << 12);
         }
-        const double own_m = (double)m * unit, own_c = (double)c;
         if (tid == 0) s.found = 0;
-        const double up_m = mass_before + block_scan(own_m, s.scan);
-        const double up_c = count_before + block_scan(own_c, s.scan);
-        const double here = stage == 0 ? up_c : up_m, own = stage == 0 ? own_c : own_m;
+        const u64 from_m = base_m + block_scan(m, s) - m, from_c = base_c + block_scan(c, s) - c;
+        const u64 start = stage == 0 ? count_before + from_c : reach(mass_before, from_m, scale);
         // the last digit with a token that starts below the bound holds it
-        if (c && here - own < bound) atomicMax(&s.found, tid);
+        if (c && start < bound) atomicMax(&s.found, tid);
         __syncthreads();
-        if (tid == s.found) { s.found_mass = up_m - own_m; s.temp = (u64)(up_c - own_c); }
+        if (tid == s.found) { s.found_mass = from_m; s.temp = from_c; s.last = c; }
         __syncthreads();
-        mass_before = s.found_mass;
-        count_before = (double)s.temp;
+        base_m = s.found_mass;
+        base_c = s.temp;
+        ties = s.last;
         if (tid < ctas) cluster.map_shared_rank(&s, tid)->prefix = prefix << 8 | (uint32_t)(255 - s.found);
       }
       cluster_barrier();
@@ -1026,13 +1091,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) sample_kernel(const __gr
     }
     // every token left has the same logit: some of them come before the one wanted
     const float v = key_logit(prefix);
-    const double w = logit_mass(v, r, s.octave);
-    const double ties = stage == 0 ? bound - count_before : ties_for(bound - mass_before, w);
-    if (stage < 2) {
-      kept = fmin(kept, mass_before + ties * w);
-      continue;
+    u64 wanted = 0;
+    if (rank == 0) {
+      const uint32_t m = logit_m(v, (uint32_t)bin, r);
+      wanted = stage == 0 ? min(bound - count_before - base_c, ties) : ties_for(mass_before, base_m, m, ties, scale, bound);
+      if (stage < 2) kept = reach(mass_before, base_m + wanted * m, scale);
     }
-    pick(v, kept, [&](unsigned int, double) { return ties - 1.0; });
+    if (stage < 2) continue;
+    pick(v, kept, [&](unsigned int, u64) { return wanted - 1; });
     return;
   }
 }
