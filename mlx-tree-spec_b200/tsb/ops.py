@@ -291,37 +291,37 @@ def tree_flash(queries, cache, scale: float, bits=None, tail: int | None = None,
 _GET_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def _bad_plane(name: str, t, shape, device):
-    return ValueError(f"tree_flash_shared: {name} must be a contiguous tensor of shape {tuple(shape)} on {device}, "
-                      f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-
-
-def _kv_struct(cache, planes, bsz: int, hkv: int, d: int, device):
-    """tsb_kv_t of a cache of `bsz` requests, its planes checked."""
+def _check_planes(who: str, planes, bsz: int, hkv: int | None, d: int, device) -> None:
+    """Types, shapes and layout of a cache's tensors, which the kernels take for granted
+    (hkv None: the keys' own)."""
     fmt, k, ks, kb, v, vs, vb = planes
-    cap, rows = k.shape[2], int(cache.offset)
-    if not 0 <= rows <= cap:
-        raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
+    if k.dim() != 4:
+        raise ValueError(f"{who}: keys must be (B, Hkv, capacity, ...), got {tuple(k.shape)}")
     words = fmt == TSB_KV_MLX_Q8_G64
-    shape = (bsz, hkv, cap, d // 4 if words else d)
-    if (k.shape != shape or v.shape != shape or not k.is_contiguous() or not v.is_contiguous() or k.device != device
-            or v.device != device):
-        raise _bad_plane("keys and values", v if k.shape == shape and k.is_contiguous() else k, shape, device)
+    shape = (bsz, k.shape[1] if hkv is None else hkv, k.shape[2], d // 4 if words else d)
+    types = (torch.bfloat16,) if fmt == TSB_KV_BF16 else (torch.int32, torch.uint32) if words else (torch.int8,)
+    for t in (k, v):
+        if t.shape != shape or t.dtype not in types or not t.is_contiguous() or t.device != device:
+            raise ValueError(f"{who}: keys and values must be contiguous {' or '.join(map(str, types))} tensors of shape "
+                             f"{shape} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
     if fmt == TSB_KV_BF16:
-        if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
-            raise _bad_plane("keys and values in bf16", v, shape, device)
-        return _lib.KVT(k.data_ptr(), None, None, v.data_ptr(), None, None, cap, rows)
-    types = (torch.int32, torch.uint32) if words else (torch.int8,)
-    if k.dtype not in types or v.dtype not in types:
-        raise _bad_plane("keys and values in 8-bit codes", v, shape, device)
-    shape = (bsz, hkv, cap, d // 64) if words else (bsz, hkv, cap)
-    dt = torch.bfloat16 if words else torch.float32
+        return
+    shape, dt = (shape[:3] + (d // 64,), torch.bfloat16) if words else (shape[:3], torch.float32)
     for name, t in (("scales", ks), ("scales", vs), ("biases", kb), ("biases", vb)):
         if name == "biases" and not words:
             continue
         if t is None or t.shape != shape or t.dtype != dt or not t.is_contiguous() or t.device != device:
-            raise ValueError(f"tree_flash_shared: {name} must be a contiguous {dt} tensor of shape {shape} on {device}")
-    return _lib.KVT(k.data_ptr(), ks.data_ptr(), _ptr(kb), v.data_ptr(), vs.data_ptr(), _ptr(vb), cap, rows)
+            raise ValueError(f"{who}: {name} must be a contiguous {dt} tensor of shape {shape} on {device}")
+
+
+def _kv_struct(cache, planes, bsz: int, hkv: int, d: int, device):
+    """tsb_kv_t of a cache of `bsz` requests, its planes checked."""
+    _check_planes("tree_flash_shared", planes, bsz, hkv, d, device)
+    _, k, ks, kb, v, vs, vb = planes
+    cap, rows = k.shape[2], int(cache.offset)
+    if not 0 <= rows <= cap:
+        raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
+    return _lib.KVT(k.data_ptr(), _ptr(ks), _ptr(kb), v.data_ptr(), _ptr(vs), _ptr(vb), cap, rows)
 
 
 def _tree_rows(t, bsz: int, n: int, dtype, what: str, device):

@@ -23,8 +23,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import TSB_EUNSUPPORTED, TSB_KV_MLX_Q8_G64, TSB_MASK_BF16, TSB_MASK_F16, TSB_MASK_F32, check
-from .ops import _GET_DEVICE, _kv_planes, _ptr, _require_cuda, _stream
+from ._lib import TSB_EUNSUPPORTED, TSB_MASK_BF16, TSB_MASK_F16, TSB_MASK_F32, check
+from .ops import _GET_DEVICE, _check_planes, _kv_planes, _ptr, _require_cuda, _stream
 
 _LOGIT_TYPES = {torch.bfloat16: TSB_MASK_BF16, torch.float16: TSB_MASK_F16, torch.float32: TSB_MASK_F32}
 _MAX_LAYERS_PER_LAUNCH = 48
@@ -163,7 +163,8 @@ class PathCommit:
 
     The plan holds the caches' tensors (not their `offset`): make it once per
     set of caches, and again if a cache gets new tensors. The caches of one
-    request batch B may differ in format, heads and capacity."""
+    request batch B may differ in format, heads and capacity; every tensor must
+    be contiguous, of its format's type and shape."""
 
     def __init__(self, caches):
         self._caches = [(c, _kv_planes(c)) for c in caches]
@@ -175,19 +176,10 @@ class PathCommit:
         if len(set(planes_seen)) < len(planes_seen):
             raise ValueError("PathCommit: a tensor appears twice: its rows would move twice")
         for _, planes in self._caches:
-            k, v = planes[1], planes[4]
             _require_cuda(*planes[1:])
-            if any(t is not None and not t.is_contiguous() for t in planes[1:]):
-                raise ValueError("PathCommit: cache tensors must be contiguous")
-            width = k.shape[3] * (4 if planes[0] == TSB_KV_MLX_Q8_G64 else 1)
-            if width != 256 or k.shape != v.shape:
-                raise ValueError(f"PathCommit: unsupported cache of shape {tuple(k.shape)}")
-            for t in planes[2:]:
-                if t is not None and (t.device != k0.device or t.shape[:3] != k.shape[:3]):
-                    raise ValueError("PathCommit: a cache's planes must agree in shape and device")
-            if k.device != k0.device or k.shape[0] != k0.shape[0]:
-                raise ValueError("PathCommit: every cache must hold the same requests on the same device")
-            groups.setdefault((planes[0], k.shape[1], k.shape[2]), []).append(planes)
+            # the same requests on the same device in every cache
+            _check_planes("PathCommit", planes, k0.shape[0], None, 256, k0.device)
+            groups.setdefault((planes[0], *planes[1].shape[1:3]), []).append(planes)
         self._device, self._batch = k0.device, k0.shape[0]
         self._launches = []
         vp = ctypes.c_void_p

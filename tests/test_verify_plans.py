@@ -1,0 +1,71 @@
+"""What a commit plan and a verify step refuse before they touch a cache, on the CPU:
+the checks of the caches' tensors need no device."""
+
+import pytest
+import torch
+
+HKV, CAP = 2, 12
+
+
+@pytest.fixture
+def plan(lib_built, monkeypatch):
+    """PathCommit of caches that lie in host memory (the plan itself launches nothing)."""
+    import tsb
+    from tsb import verify
+
+    monkeypatch.setattr(verify, "_require_cuda", lambda *ts: None)
+    return tsb.PathCommit
+
+
+def _cache(fmt, b=2, **other):
+    """A cache of zeros, with some of its tensors replaced."""
+    import tsb
+
+    z = lambda *s, dtype: torch.zeros(b, HKV, CAP, *s, dtype=dtype)  # noqa: E731
+    if fmt == "bf16":
+        kind, t = tsb.KVCache, dict(keys=z(256, dtype=torch.bfloat16), values=z(256, dtype=torch.bfloat16))
+    elif fmt == "ref_q8":
+        kind, t = tsb.Q8KVCache, dict(keys=z(256, dtype=torch.int8), values=z(256, dtype=torch.int8),
+                                      k_scale=z(dtype=torch.float32), v_scale=z(dtype=torch.float32))
+    else:
+        kind, t = tsb.MLXQ8KVCache, dict(keys=z(64, dtype=torch.int32), values=z(64, dtype=torch.int32))
+        t.update({n: z(4, dtype=torch.bfloat16) for n in ("k_scales", "k_biases", "v_scales", "v_biases")})
+    for name, change in other.items():
+        t[name] = change(t[name])
+    return kind(**t, offset=CAP)
+
+
+BAD = [
+    ("bf16", "keys", lambda t: t.float()), ("bf16", "values", lambda t: t.half()), ("bf16", "keys", lambda t: t.to(torch.int8)),
+    ("bf16", "values", lambda t: t[:, :1].contiguous()), ("bf16", "keys", lambda t: t[0]),
+    ("ref_q8", "keys", lambda t: t.to(torch.bfloat16)), ("ref_q8", "values", lambda t: t.float()),
+    ("ref_q8", "k_scale", lambda t: t.half()), ("ref_q8", "v_scale", lambda t: t.bfloat16()),
+    ("ref_q8", "v_scale", lambda t: t.double()), ("ref_q8", "k_scale", lambda t: t[:, :, :-1].contiguous()),
+    ("ref_q8", "k_scale", lambda t: t[..., None].expand(-1, -1, -1, 2).contiguous()), ("ref_q8", "v_scale", lambda t: None),
+    ("mlx_q8", "keys", lambda t: t.long()), ("mlx_q8", "values", lambda t: t.float()),
+    ("mlx_q8", "k_scales", lambda t: t.float()), ("mlx_q8", "v_biases", lambda t: t.half()),
+    ("mlx_q8", "v_scales", lambda t: t[..., :2].contiguous()), ("mlx_q8", "k_biases", lambda t: torch.cat([t, t], -1)),
+    ("mlx_q8", "k_biases", lambda t: t[..., 0].contiguous()), ("mlx_q8", "v_scales", lambda t: None),
+    ("bf16", "keys", lambda t: t.reshape(-1)), ("mlx_q8", "k_scales", lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)),
+]
+
+
+@pytest.mark.parametrize("fmt,name,change", BAD, ids=[f"{i}-{f}-{n}" for i, (f, n, _) in enumerate(BAD)])
+def test_plan_refuses_tensors_of_another_kind(plan, fmt, name, change):
+    """A row is moved by its format's width: tensors of another type or shape would lose
+    rows, or be written past their ends."""
+    good = _cache(fmt)
+    plan([good])
+    for caches in ([_cache(fmt, **{name: change})], [good, _cache(fmt, **{name: change})]):
+        with pytest.raises(ValueError):
+            plan(caches)
+
+
+def test_plan_takes_every_format(plan):
+    import tsb
+
+    words = _cache("mlx_q8", keys=lambda t: t.view(torch.uint32), values=lambda t: t.view(torch.uint32))
+    plan([_cache("bf16"), _cache("ref_q8"), _cache("mlx_q8"), words])
+    c = _cache("bf16")
+    past = tsb.KVCache(c.keys, c.values, CAP + 5)  # a plan does not read the offset
+    plan([past])
