@@ -40,7 +40,7 @@ from . import _lib, ops
 from ._lib import TSB_KV_BF16, TSB_KV_MLX_Q8_G64, TSB_KV_REF_Q8_ROW, check
 from .cache import KVCache, MLXQ8KVCache, Q8KVCache
 from .quant import quantize, quantize_g64, quantize_rows
-from .verify import sample, tree_accept
+from .verify import PathCommit, sample, tree_accept
 
 # of VerifyDecoder.verify: tree_accept's path (B, T), n_keep (B,) and next_token (B,), the
 # sampled tokens (B, T) and the lengths (B,) after the commit, all int32 on the device
@@ -187,8 +187,11 @@ class VerifyDecoder:
         (wq, scales, biases)), a token drawn at every node with the random numbers u
         (B, T) (tsb.sample's filters; one value per node where a tensor), the walk
         along the drafted tokens (B, T), and the commit of the accepted rows.
-        commit: PathCommit(caches), made once. Nothing is read on the host, so the
+        commit: PathCommit(caches), made once; a plan of other tensors than these
+        caches' raises, before anything is written. Nothing is read on the host, so the
         step can be captured and replayed."""
+        if isinstance(commit, PathCommit) and not commit.is_of(caches):
+            raise ValueError("verify: commit must be the plan of these caches' tensors (PathCommit(caches))")
         b, t = parents.shape
         x = self.step_shared(h_in, parents, prefixes, caches, lengths)
         logits = ops.quantized_matmul(x, *lm_head)

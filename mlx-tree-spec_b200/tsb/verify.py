@@ -150,6 +150,10 @@ def tree_accept(tokens, parents, samples):
     return path, n_keep, nxt
 
 
+def _pointers(planes) -> list:
+    return [t.data_ptr() for p in planes for t in p[1:] if t is not None]
+
+
 class PathCommit:
     """The tree commit of a list of caches (every layer's; tree_verify.py:499-516)
     by lengths and paths on the device.
@@ -172,8 +176,9 @@ class PathCommit:
             raise ValueError("PathCommit: no caches")
         groups: dict = {}
         k0 = self._caches[0][1][1]
-        planes_seen = [t.data_ptr() for _, planes in self._caches for t in planes[1:] if t is not None]
-        if len(set(planes_seen)) < len(planes_seen):
+        pointers = _pointers(planes for _, planes in self._caches)
+        self._pointers = frozenset(pointers)
+        if len(self._pointers) < len(pointers):
             raise ValueError("PathCommit: a tensor appears twice: its rows would move twice")
         for _, planes in self._caches:
             _require_cuda(*planes[1:])
@@ -189,6 +194,10 @@ class PathCommit:
                 arrays = [(vp * len(part))(*[_ptr(p[j]) for p in part]) if part[0][j] is not None else None
                           for j in range(1, 7)]
                 self._launches.append((fmt, len(part), *arrays, self._batch, hkv, 256, cap))
+
+    def is_of(self, caches) -> bool:
+        """Whether these caches' tensors, as they are now, are the plan's."""
+        return self._pointers.issuperset(now := _pointers(map(_kv_planes, caches))) and len(now) == len(self._pointers)
 
     def __call__(self, lengths, path, n_keep):
         dev, b = self._device, self._batch

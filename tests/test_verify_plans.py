@@ -69,3 +69,48 @@ def test_plan_takes_every_format(plan):
     c = _cache("bf16")
     past = tsb.KVCache(c.keys, c.values, CAP + 5)  # a plan does not read the offset
     plan([past])
+
+
+# ---------------------------------------------------------------- the decoder's verify step
+
+class _Reached(Exception):
+    pass
+
+
+@pytest.fixture
+def decoder(monkeypatch):
+    """A decoder of two layers whose layer stack ends the call: nothing runs on a device."""
+    from tsb import decoder as tdec
+
+    dec = tdec.VerifyDecoder.__new__(tdec.VerifyDecoder)
+    dec.layers = [None, None]
+
+    def stop(self, *args):
+        raise _Reached
+
+    monkeypatch.setattr(tdec.VerifyDecoder, "step_shared", stop)
+    return dec
+
+
+def _verify(dec, caches, commit):
+    i = torch.zeros(2, 3, dtype=torch.int32)
+    return dec.verify(torch.zeros(6, 8), i, i, [], caches, torch.zeros(2, dtype=torch.int32), None, torch.zeros(2, 3), commit)
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "ref_q8", "mlx_q8"])
+def test_verify_takes_its_caches_plan_only(plan, decoder, fmt):
+    """A plan of other caches would move those caches' rows and keep these as they are."""
+    import copy
+
+    caches = [_cache(fmt), _cache(fmt)]
+    for good in (plan(caches), plan(caches[::-1]), plan([copy.copy(c) for c in caches])):
+        with pytest.raises(_Reached):
+            _verify(decoder, caches, good)
+    clones = [type(c)(**{k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in vars(c).items()}) for c in caches]
+    for other in (clones, [caches[0], clones[1]], caches[:1], caches + clones[:1]):
+        with pytest.raises(ValueError, match="commit"):
+            _verify(decoder, caches, plan(other))
+    stale = plan(caches)
+    caches[1].values = caches[1].values.clone()  # a cache got a new tensor: the plan still has the old one
+    with pytest.raises(ValueError, match="commit"):
+        _verify(decoder, caches, stale)
