@@ -170,6 +170,13 @@ class VerifyDecoder:
         if (lengths.dtype != torch.int32 or lengths.shape != (b,) or not lengths.is_contiguous()
                 or lengths.device != h_in.device):
             raise ValueError(f"step_shared: lengths must be a contiguous int32 tensor ({b},) on {h_in.device}")
+        # a layer's rows are written before its attention looks at the caches
+        for prefix, cache in zip(prefixes, caches):
+            pre, own = ops._kv_planes(prefix), ops._kv_planes(cache)
+            if pre[0] != own[0]:
+                raise ValueError("step_shared: a layer's prefix and cache must share a format")
+            ops._kv_struct("step_shared", prefix, pre, 1, self.cfg.hkv, self.cfg.d, h_in.device)
+            ops._kv_struct("step_shared", cache, own, b, self.cfg.hkv, self.cfg.d, h_in.device)
         buf = self._buffers(b, t, h_in.device)
         _, depth = ops.ancestor_bits(parents, depth=True)
         torch.sub(lengths, t, out=buf["offsets"])

@@ -314,13 +314,13 @@ def _check_planes(who: str, planes, bsz: int, hkv: int | None, d: int, device) -
             raise ValueError(f"{who}: {name} must be a contiguous {dt} tensor of shape {shape} on {device}")
 
 
-def _kv_struct(cache, planes, bsz: int, hkv: int, d: int, device):
+def _kv_struct(who: str, cache, planes, bsz: int, hkv: int, d: int, device):
     """tsb_kv_t of a cache of `bsz` requests, its planes checked."""
-    _check_planes("tree_flash_shared", planes, bsz, hkv, d, device)
+    _check_planes(who, planes, bsz, hkv, d, device)
     _, k, ks, kb, v, vs, vb = planes
     cap, rows = k.shape[2], int(cache.offset)
     if not 0 <= rows <= cap:
-        raise ValueError(f"tree_flash_shared: offset {rows} outside the cache's capacity {cap}")
+        raise ValueError(f"{who}: offset {rows} outside the cache's capacity {cap}")
     return _lib.KVT(k.data_ptr(), _ptr(ks), _ptr(kb), v.data_ptr(), _ptr(vs), _ptr(vb), cap, rows)
 
 
@@ -381,8 +381,8 @@ def tree_flash_shared(queries, prefix, cache, scale: float, bits=None, tail: int
     hkv = pre_planes[1].shape[1]
     if d != 256 or hq % hkv or n > 64 or bsz < 1 or n < 1:
         return None
-    pre = _kv_struct(prefix, pre_planes, 1, hkv, d, dev)
-    own = _kv_struct(cache, own_planes, bsz, hkv, d, dev)
+    pre = _kv_struct("tree_flash_shared", prefix, pre_planes, 1, hkv, d, dev)
+    own = _kv_struct("tree_flash_shared", cache, own_planes, bsz, hkv, d, dev)
     p = bits_t = None
     if parents is not None:
         p = _tree_rows(parents, bsz, n, torch.int32, "tree_flash_shared: parents", dev)

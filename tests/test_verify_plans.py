@@ -114,3 +114,48 @@ def test_verify_takes_its_caches_plan_only(plan, decoder, fmt):
     caches[1].values = caches[1].values.clone()  # a cache got a new tensor: the plan still has the old one
     with pytest.raises(ValueError, match="commit"):
         _verify(decoder, caches, stale)
+
+
+@pytest.fixture
+def stack(lib_built, monkeypatch):
+    """A decoder of two layers whose first work on the device ends the call."""
+    from tsb import decoder as tdec
+
+    def stop(self, *args):
+        raise _Reached
+
+    dec = tdec.VerifyDecoder.__new__(tdec.VerifyDecoder)
+    dec.layers = [None, None]
+    dec.cfg = tdec.DecoderConfig(layers=2, hidden=8, hq=4, hkv=HKV, d=256, inter=8)
+    monkeypatch.setattr(tdec.VerifyDecoder, "_buffers", stop)
+    return dec
+
+
+def _step(dec, prefixes, caches, b=2):
+    return dec.step_shared(torch.zeros(b * 3, 8), torch.zeros(b, 3, dtype=torch.int32), prefixes, caches,
+                           torch.full((b,), 4, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "ref_q8", "mlx_q8"])
+def test_step_shared_refuses_caches_that_it_would_write_past(stack, fmt):
+    """Every layer's nodes are written by the batch, heads and format that the call
+    implies: a cache of fewer requests or heads, or of another type, is refused before
+    the first layer runs."""
+    pre, own = [_cache(fmt, b=1) for _ in range(2)], [_cache(fmt) for _ in range(2)]
+    with pytest.raises(_Reached):
+        _step(stack, pre, own)
+    name = "keys" if fmt == "bf16" else "k_scale" if fmt == "ref_q8" else "k_biases"
+    half = lambda t: t[:, :1].contiguous()  # noqa: E731
+    tensors = [n for n, v in vars(own[0]).items() if isinstance(v, torch.Tensor)]
+    bad = [_cache(fmt, b=1), _cache(fmt, b=3), _cache(fmt, **{n: half for n in tensors}),
+           _cache(fmt, values=lambda t: t.double()), _cache(fmt, **{name: lambda t: t[:, :, :-1].contiguous()}),
+           _cache("ref_q8" if fmt == "bf16" else "bf16")]
+    for c in bad:
+        with pytest.raises(ValueError):
+            _step(stack, pre, [own[0], c])
+    for p in (_cache(fmt), _cache(fmt, b=1, **{n: half for n in tensors}), _cache("mlx_q8" if fmt == "bf16" else "bf16", b=1)):
+        with pytest.raises(ValueError):
+            _step(stack, [pre[0], p], own)
+    own[1].offset = CAP + 1
+    with pytest.raises(ValueError):
+        _step(stack, pre, own)
