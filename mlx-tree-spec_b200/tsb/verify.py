@@ -163,7 +163,8 @@ class PathCommit:
     lengths[b] - T + path[b, i], i < n_keep[b], move to lengths[b] - T + i in
     every cache, and the new length is lengths[b] - T + n_keep[b]. path (B, T)
     and n_keep (B,) are tree_accept's; a path must increase and ends where it
-    does not. A request whose length is not in [T, capacity] is left as it is.
+    does not. A request whose length is not in [T, capacity] is left as it is, in
+    every cache: where capacities differ, the smallest counts.
 
     The plan holds the caches' tensors (not their `offset`): make it once per
     set of caches, and again if a cache gets new tensors. The caches of one
@@ -186,6 +187,8 @@ class PathCommit:
             _check_planes("PathCommit", planes, k0.shape[0], None, 256, k0.device)
             groups.setdefault((planes[0], *planes[1].shape[1:3]), []).append(planes)
         self._device, self._batch = k0.device, k0.shape[0]
+        caps = {cap for _, _, cap in groups}
+        self._least = min(caps) if len(caps) > 1 else None
         self._launches = []
         vp = ctypes.c_void_p
         for (fmt, hkv, cap), members in groups.items():
@@ -213,13 +216,17 @@ class PathCommit:
         n = _i32(n_keep, (b,), "PathCommit: n_keep", dev)
         cur = _i32(lengths, (b,), "PathCommit: lengths", dev)
         new = torch.empty_like(cur)
+        given = cur
+        if self._least is not None:  # each launch knows its own caches' capacity
+            fits = given <= self._least
+            cur = torch.where(fits, given, 0)  # no tree ends there: left as it is
         commit, stream, out = _lib.load().tsb_kv_commit_paths, _stream(p), new.data_ptr()
         for args in self._launches:
             status = commit(*args, t, cur.data_ptr(), p.data_ptr(), n.data_ptr(), out, stream)
             out = None  # one launch writes the lengths
             if status and check(status, "tsb_kv_commit_paths") == TSB_EUNSUPPORTED:
                 raise ValueError("PathCommit: unsupported caches")
-        return new
+        return new if cur is given else torch.where(fits, new, given)
 
 
 def commit_paths(caches, lengths, path, n_keep):
