@@ -1114,13 +1114,16 @@ int launch_sample(SampleArgs a, int rows, cudaStream_t st) {
     ctas *= 2;
   a.slice = ((a.vocab + ctas - 1) / ctas + 7) & ~7;
   const size_t stage = ((size_t)a.slice + 16 / sizeof(T)) * sizeof(T);
-  // Rows that are all at work at once without their logits in shared memory, but not with
-  // them, read them again from L2 instead (48 rows of 100003 float32: 28.7 us, 36.5 in two
-  // rounds; 128 rows of 131072 bf16, in several rounds either way: 59.5 us, 51.8 staged).
-  const auto at_once = [&](size_t smem) {
-    return (long long)sm_count() * (long long)std::min<size_t>(kCtasPerSm, kSmemPerSm / (smem + 1024)) / ctas;
-  };
-  a.staged = stage <= kMaxStage && (rows <= at_once(kSharedBytes + stage) || rows > at_once(kSharedBytes));
+  // The logits stay in shared memory while two CTAs fit an SM that way, and where a CTA has
+  // the SM to itself for two rounds of rows; else the later passes read them from L2, with
+  // three CTAs an SM. Inputs that come from DRAM, vocabularies of 32003 to 600011: two to an SM,
+  // staged is up to 25% faster at 1 to 256 rows (48 x 100003 float32: flat 36.7 us against 38.6,
+  // mixed settings 34.1 / 40.1; 128 x 151936 bf16 73 / 87 and 61 / 75). One to an SM: 16 x 262144
+  // float32 91 / 134 and 38 / 62, 36 rows 146 / 148 and 60 / 72, 48 rows 184 / 151 and 78 / 78,
+  // 90 rows 287 / 233 and 122 / 101. (An input that is sampled again while it is in L2 hides the
+  // later passes: 48 x 100003 float32, replayed, 28.7 us unstaged.)
+  const size_t per_sm = kSmemPerSm / (kSharedBytes + stage + 1024);
+  a.staged = stage <= kMaxStage && (per_sm >= 2 || (long long)rows * ctas <= 2LL * sm_count());
   const size_t smem = kSharedBytes + (a.staged ? stage : 0);
   static std::atomic<unsigned long long> ready{0};  // devices on which the attribute is set
   int dev = 0;
