@@ -294,8 +294,11 @@ int tsb_tree_attn_shared(const void *q, long long q_stride_b, long long q_stride
  * weight; a row with nothing to choose gives token -1 and logprob -inf. Weights
  * are integers of 23 bits times a power of 2^(1/32); those of one power are
  * summed as integers, the sums of the powers as whole numbers of 2^-43 of the
- * largest weight, so results repeat bit for bit. Weights below 2^-43 count as
- * zero, and temperatures as the nearest in [2^-60, 2^100]. vocab <= 2^20. */
+ * largest weight, so results repeat bit for bit. A weight is within 2^-23 of
+ * itself (plus 2^-24 d / temperature where the difference d to the largest logit
+ * is no float32), a border between two shares within 2^-24. Weights below 2^-43
+ * (2^-41 with top_k <= 64) count as zero, and temperatures as the nearest in
+ * [2^-60, 2^100]. vocab <= 2^20. */
 int tsb_sample(const void *logits, int logits_dtype, int rows, int vocab, long long row_stride, const float *u,
                const float *temperature, double temperature_all, const int32_t *top_k, int top_k_all,
                const float *top_p, double top_p_all, const float *min_p, double min_p_all, int32_t *token,

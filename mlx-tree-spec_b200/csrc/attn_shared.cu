@@ -16,13 +16,15 @@
 // a combine kernel merges those of each row. (One list of tiles per row block, its
 // requests' own rows behind the prefix in the same segments, does without the own
 // segments' ~10,000 cycles each, but masks other requests' rows in every own tile and
-// starts later: 12 x 32 nodes over 32K rows 246 us against 216.)
+// starts later: 12 x 32 nodes over 32K rows 246 us against 216, after an idle time.)
 //
-// Measured (graph replay, 24 query and 4 KV heads): 12 requests x 32 nodes over 32K shared
-// rows + 1K own 216 us, 1.45 PFLOP/s, 0.87 of what a large matrix product reaches in a
-// burst and more than it sustains; 8 x 16 over 8K + 512: 37 us; 4 x 1 over 1K + 64:
-// 14 us, two dependent launches around a tile or two; 5 x 32 over 32K in 8 bits 135 us, 34 of them the
-// conversion at 6.0 TB/s.
+// Measured (24 query and 4 KV heads; calls one after the other, and a replayed graph): 12
+// requests x 32 nodes over 32K shared rows + 1K own 251 and 248 us, 1.27 PFLOP/s, 0.92 of
+// what a large matrix product sustains at the clock that the power limit leaves (1.43
+// GHz); 216 and 213 us in the first milliseconds after an idle time, 1.47 PFLOP/s, 0.89 of such
+// a product's burst. 8 x 16 over 8K + 512: 35 and 35 us; 4 x 1 over 1K + 64: 22 (the host's
+// time) and 12 us, two dependent launches around a tile or two; 5 x 32 over 32K in 8 bits 158
+// and 155 us, after an idle time 136 and 133, 34 of them the conversion.
 //
 // With many packed rows the work is bound by the tensor cores: 64 keys x 128 rows
 // are ~1024 cycles of MMA per SM. One SM by itself cannot feed them: a tile's 64 KB of
@@ -46,9 +48,11 @@
 // shared memory (two buffers), so S_{g+2} waits only until S_g has been read.
 // g counts a pair's tiles over all its segments.
 //
-// 8-bit caches are converted to bf16 in the workspace first, by a kernel at memory
-// speed: each row block would convert every tile again in here, which held a tile to
-// 2.1 us where bf16 takes 1 (5 x 32 nodes over 32K rows: 264 us in all, 135 now).
+// 8-bit caches are converted to bf16 in the workspace first: each row block would
+// convert every tile again in here, which held a tile to 2.1 us where bf16 takes 1 (5 x 32
+// nodes over 32K rows: 264 us in all against 135, both after an idle time). With a single row block
+// (B G T <= 256) no tile would be converted twice; the copy is made there too, and was not
+// measured against converting in here.
 // MLX: the values. int8 rows: the codes, exact in bf16, with the row scales applied in
 // float32 to scores and weights.
 //
@@ -827,10 +831,11 @@ tree_attn_shared_kernel(const __grid_constant__ CUtensorMap tmap_kp, const __gri
 
 // ---------------------------------------------------------------- 8-bit caches
 // The valid rows of an 8-bit cache as bf16 rows [heads][rows][D]: MLX values
-// bf16(fmaf(code, s, b)), or the int8 codes themselves. 16 lanes have a row; bound
-// by memory (272 or 256 bytes read and 512 written per row): 4 x 32K rows of K and V,
-// 205 MB, in 34.3 us or 6.0 TB/s. All loads stand before the first use, a lane's 32 bytes
-// go out in one store (64-row blocks, 16-byte stores and late scale loads: 43.5 us).
+// bf16(fmaf(code, s, b)), or the int8 codes themselves. 16 lanes have a row (272 or 256
+// bytes read and 512 written): 4 x 32K rows of K and V, 205 MB, in 34.3 us. Of the bytes
+// written 59 MB stay in L2, and what goes through DRAM, 148 MB, is 54% of its rate: memory is
+// not shown to be the limit. All loads stand before the first use, a lane's 32 bytes go
+// out in one store (64-row blocks, 16-byte stores and late scale loads: 43.5 us).
 constexpr int SH_CV_ROWS = 32;  // rows of a CTA
 
 struct ShConvert {

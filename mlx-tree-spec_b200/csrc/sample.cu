@@ -27,21 +27,26 @@
 // nearly equal logits, by a radix descent over their bits.
 //
 // Masses. Inside a bin (t within 1/64 of bin / 32) a token's weight is m * 2^-22 *
-// 2^(-bin / 32) with m an integer of 23 bits: a float32 series of the exactly
-// reduced t, whose roundings are independent from token to token and do not add
-// up. Sums over a bin's tokens are sums of integers, so they do not depend on the
-// order of the atomics and results repeat bit for bit. m goes into two 32-bit
-// shared-memory atomics of 12 and 11 bits (2^20 tokens do not overflow them); a
-// 64-bit one would be a compare-and-swap loop.
+// 2^(-bin / 32) with m an integer of 23 bits, from a float32 series of the reduced t.
+// Sums over a bin's tokens are sums of integers, so they do not depend on the order of
+// the atomics and results repeat bit for bit. m goes into two 32-bit shared-memory
+// atomics of 12 and 11 bits (2^20 tokens do not overflow them), which is why it has no
+// more bits; a 64-bit one would be a compare-and-swap loop.
+//   Half a unit of m is 2^-23 of the weight, equal logits having the same rounding: a
+// border between two tokens' shares is off by 2^-24 at most (half of the weights high,
+// half low), by far less where many different logits come before it. The difference to the
+// largest logit is a float32: exact for 16-bit logits but for those of very different
+// exponents, else a rounding of 2^-24 d / temperature of the weight.
 //   The running mass at a token is a whole number of 2^-43 too: the sum over the
 // bins before its own, and its bin's tokens up to it, whose sum of m is rounded to
 // such units once (`reach`). Whoever asks gets the same number, it never falls along
 // the order, and a bin without tokens adds nothing; so a bound that is itself a
 // running mass (what a filter keeps, at u = 1) is met at the token that it came from.
 //
-// Measured: one row of 131072 bf16 logits with top-k 50 and top-p 0.95 10.3 us; 128 such
-// rows with settings of their own 52 us (the bytes alone: 5.2 us); 48 rows of 100003
-// float32 with temperature alone 29 us (3.0). A row's steps take 15-60 thousand cycles
+// Measured, in calls one after the other (and as a replayed graph), inputs in turn: one row
+// of 131072 bf16 logits with top-k 50 and top-p 0.95 11.5 us (8.9); 128 such rows with
+// settings of their own 55.6 us (54.9; the bytes alone: 5.2 us); 48 rows of 100003 float32
+// with temperature alone 37.3 us (36.7; 3.0). One input that stays in L2: 49 and 34 us. A row's steps take 15-60 thousand cycles
 // (load 3, maximum 3, histogram 8, plan 5, gather 6, each bound 6), mostly waits for shared
 // memory and for the other CTAs, and 55 rows are at work at once.
 //
@@ -138,7 +143,7 @@ TSB_HD uint32_t logit_bin(float x, const RowScale &r) {
 }
 // m of a token of bin < kBins: 2^22 * 2^(-g / 32), g = kStep * t - bin in [-1/2, 1/2]
 // up to the roundings of t, from the series of e^z at |z| <= 0.011 (the next term is
-// below 2^-31). The last addition leaves the rounded integer in the mantissa.
+// below 2^-30). The last addition leaves the rounded integer in the mantissa.
 TSB_HD uint32_t logit_m(float x, uint32_t bin, const RowScale &r) {
   const float d = r.top - x;
   const float b = __uint_as_float(0x4B000000u | bin) - 8388608.f;
@@ -177,7 +182,8 @@ TSB_HD double logit_mass(float x, const RowScale &r, const double *octave) {
   return bin < (uint32_t)kBins ? (double)logit_m(x, bin, r) * bin_unit(bin, octave) : 0.0;
 }
 
-// With small top-k, weights are added up as whole numbers of 2^-40.
+// With small top-k, weights are rounded to whole numbers of 2^-40 and added up: at most
+// 64 tokens count, so what that changes of their sum is below 2^-35.
 constexpr double kListUnit = 1099511627776.0;
 TSB_HD u64 list_units(double mass) { return (u64)__double2ll_rn(mass * kListUnit); }
 
